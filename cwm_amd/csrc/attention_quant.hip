@@ -1,0 +1,594 @@
+// Paged causal attention over a cache held in 4 or 8 bits (layout and formulas: quant_cache.h), on the matrix cores, for
+// decoded tokens and prompt portions in one launch.  Compiled per head size: -DHEAD_DIM=<multiple of 32, at most 256>.
+//
+// The query at position p reads keys max(0, p - window_left) .. p; scores scale (q . k), softmax, sum of the values; query
+// head h reads key/value head h / (Hq / Hkv).  Rows are (new token, query head of the group) pairs, 16 to a tile; work items
+// as of the attention over a cache in the activations' type: {sequence, first row, first key, end key, partial slot or -1, 0}.
+//
+// Codes go to the matrix instruction as they are: a code of 4 bits under the exponent of 128 is the bfloat16 number 128 + c,
+// one mask and one "or" for two of them, and exact.  With the key k_d = z_g + s_g (c_d - H) of group g of 32 elements,
+//     q . k = sum_g s_g (sum_d q_d (OFF' + c_d)) + sum_g (z_g - OFF s_g) sum_d q_d,   OFF = OFF' + H
+// where the second sum is one more matrix product, of the words (offset, step) of a key, which are already pairs of
+// bfloat16 numbers in a register, with the query's sums in three bfloat16 parts; and a product of the words with a column
+// that is 1 at one place brings a group's step to the lanes that hold its scores.  No vector instruction touches a word.
+//     o = sum_j p_j v_j = sum_j b_j (OFF' + c_j) - OFF sum_j b_j + sum_j p_j z_j,   b_j = p_j s_j rounded to bfloat16
+// The sum of the b_j is one more matrix product (a row of ones), so that it holds the same rounded numbers; the last sum is
+// kept in float32.  The rounding of b is that of p in the attention over a bfloat16 cache, and multiplies c - H, not c.
+// float32 queries: q and b in three bfloat16 parts each, codes without an offset (c - H is exact in bfloat16).
+//
+// Lanes as in the attention over a bfloat16 cache (lane 16 j + n): S^T = K Q^T leaves lane (row n, j) the keys 8 j .. 8 j + 7
+// of 32, which is the operand of O^T = V^T P^T, so probabilities never move.
+#include "quant_cache.h"
+#include "three_parts.h"
+
+CWM_DEFINE_ERROR_API
+
+#ifndef HEAD_DIM
+#error "compile with -DHEAD_DIM=<head size>"
+#endif
+#if HEAD_DIM % 32 != 0 || HEAD_DIM > 256 || HEAD_DIM < 32
+#error "HEAD_DIM must be a multiple of 32 between 32 and 256"
+#endif
+
+#define G (HEAD_DIM / 32)  // groups of a key
+#define QUADS ((G + 3) / 4)  // operands that a key's words fill, four words each
+#define D_TILES (HEAD_DIM / 16)
+#define WORK_INTS 6
+#define PARTIAL_STRIDE (HEAD_DIM + 4)  // reference maximum and sum after the output
+#define TEAM 4  // wavefronts of a block
+
+typedef const __attribute__((address_space(4))) int* scalar_ints;  // a uniform index is read by a scalar load
+
+template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 u = *(const uint4*)(p + 4 * i);
+      w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint2 u = *(const uint2*)(p + 4 * i);
+      w[i] = u.x, w[i + 1] = u.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = *(const uint32_t*)(p + 4 * i);
+  }
+}
+
+// How codes become numbers of bfloat16.  EXACT: c - H.  Else OFF' + c, OFF' = 128 for 4 bits and 0 for 8.
+template <int BITS, bool EXACT> struct Codes {
+  static constexpr int H = 1 << (BITS - 1);
+  static constexpr float OFF = EXACT ? 0.f : (BITS == 4 ? 128.f + H : (float)H);
+  // four bits from bit 0 and from bit 16 on
+  static __device__ __forceinline__ uint32_t nibbles(uint32_t w) {
+    if constexpr (EXACT) {
+      const float a = (float)((int)(w & 15u) - H), b = (float)((int)((w >> 16) & 15u) - H);
+      return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    }
+    return (w & 0x000f000fu) | 0x43004300u;
+  }
+  static __device__ __forceinline__ uint32_t bytes(uint32_t w, int first) {  // bytes `first` and `first + 1`
+    float a = (float)((w >> (8 * first)) & 255u), b = (float)((w >> (8 * first + 8)) & 255u);
+    if constexpr (EXACT) a -= H, b -= H;
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  }
+};
+
+// What a wavefront loads of 32 keys: lane (n, j) the codes [j] of keys 8 (n / 4) + n % 4 and + 4 with their words, and of the
+// values of keys 8 j .. 8 j + 7 those of its dimensions, with their words.
+template <int BITS> struct KeyTile {
+  static constexpr int KC = G * BITS / 4;
+  // words of the values' codes: pieces of 16 bytes (four dimensions of 4 bits, two of 8), a last one of 8 where 32 dimensions are left
+  static constexpr int VC = BITS == 4 ? 2 * G : 4 * G;
+  uint32_t kc[2][KC], kw[2][G], vc[VC], vw[8];
+};
+
+__device__ __forceinline__ float not_a_number() { return __uint_as_float(0x7fc00000u); }
+
+// Whether any key of [first_key, last_key] lies in a logical page whose table entry is no page of the pool.
+__device__ __forceinline__ bool span_lacks_page(const int* __restrict__ table, int table_width, int num_pages, int page_size, int first_key,
+                                                int last_key, int lane) {
+  bool bad = false;
+  if (last_key >= first_key && first_key >= 0) {
+    for (int lp = first_key / page_size + lane; lp <= last_key / page_size; lp += 64) {
+      const int page = lp < table_width ? table[lp] : -1;
+      bad = bad || (unsigned)page >= (unsigned)num_pages;
+    }
+  }
+  return __any(bad);
+}
+
+// RT row tiles a wavefront.  SPLIT: the block's wavefronts share 16 RT rows and take the item's tiles of 32 keys in turn, and
+// join their results through LDS; else each has rows of its own and walks all of the item's keys.
+template <typename T, int BITS, int RT, bool SPLIT, bool PAGE32>
+__global__ void __launch_bounds__(256, SPLIT ? 2 : 1)
+attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ out, long out_stride, const uint8_t* __restrict__ cache,
+                       const int* __restrict__ block_table, int table_width, const int* __restrict__ cu_q, const int* __restrict__ kv_len,
+                       const int* __restrict__ work, float* __restrict__ partial, int n_q_heads, int n_kv_heads, int page_size, int page_shift,
+                       int num_pages, int window_left, float scale_log2e) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  constexpr int PARTS = EXACT ? 3 : 1;
+  typedef Codes<BITS, EXACT> C;
+  typedef KeyTile<BITS> Keys;
+  const float neg_inf = -__builtin_inff();
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = blockIdx.x / n_kv_heads;
+  const int g0 = blockIdx.x - item * n_kv_heads;  // key/value head
+  const int* w = work + (size_t)item * WORK_INTS;
+  const int b = w[0], key_begin = w[2], key_end = w[3], slot = w[4], n_chunks = w[5];
+  if (key_begin >= key_end) return;  // a null item: a list of a fixed length is filled up with them
+
+  const int group = n_q_heads / n_kv_heads;
+  const int q0 = cu_q[b];
+  const int n_new = cu_q[b + 1] - q0;
+  const int n_old = kv_len[b] - n_new;
+  const int n_rows = n_new * group;
+  const int n = lane & 15, j = lane >> 4;
+
+  bool row_valid[RT];
+  int ti[RT], hq[RT], row_end[RT], row_start[RT];
+  Frag8 qf[RT][PARTS][G], qs[RT][QUADS];
+  int lo_any = 0x7fffffff, hi_any = -1, lo_all = key_begin, hi_all = key_end - 1;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = w[1] + 16 * (SPLIT ? rt : RT * wave + rt) + n;
+    row_valid[rt] = r < n_rows;
+    ti[rt] = row_valid[rt] ? r / group : 0;
+    hq[rt] = g0 * group + (row_valid[rt] ? r - ti[rt] * group : 0);
+    row_end[rt] = n_old + ti[rt];
+    row_start[rt] = window_left >= 0 ? max(0, row_end[rt] - window_left) : 0;
+    lo_any = min(lo_any, row_valid[rt] ? row_start[rt] : 0x7fffffff);
+    hi_any = max(hi_any, row_valid[rt] ? row_end[rt] : -1);
+    lo_all = max(lo_all, row_valid[rt] ? row_start[rt] : 0x7fffffff);
+    hi_all = min(hi_all, row_valid[rt] ? row_end[rt] : -1);
+
+    // queries: the B operands, and the sums over a group's elements in three parts, one part for each j < 3
+    const T* qrow = q + (size_t)(q0 + ti[rt]) * q_stride + (size_t)hq[rt] * HEAD_DIM + 8 * j;
+    float sum[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float x[8];
+      if constexpr (EXACT) {
+        float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+        if (row_valid[rt]) lo = *(const float4*)(qrow + 32 * g), hi = *(const float4*)(qrow + 32 * g + 4);
+        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+        { Frag8 part[3]; three_parts(x, part); qf[rt][0][g] = part[0], qf[rt][1 % PARTS][g] = part[1], qf[rt][2 % PARTS][g] = part[2]; }
+      } else {
+        qf[rt][0][g].u = row_valid[rt] ? *(const uint4*)(qrow + 32 * g) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = bf16_to_f32(qf[rt][0][g].h[e]);
+      }
+      sum[g] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+      sum[g] += __shfl_xor(sum[g], 16, 64);
+      sum[g] += __shfl_xor(sum[g], 32, 64);
+    }
+#pragma unroll
+    for (int u = 0; u < QUADS; ++u) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = 4 * u + i < G ? sum[(4 * u + i) % G] : 0.f;
+        x[2 * i + 1] = -C::OFF * x[2 * i];
+      }
+      Frag8 part[3];
+      three_parts(x, part);
+      qs[rt][u].u = j == 0 ? part[0].u : j == 1 ? part[1].u : j == 2 ? part[2].u : make_uint4(0, 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 16; off <<= 1) {
+    lo_any = min(lo_any, __shfl_xor(lo_any, off, 64));
+    hi_any = max(hi_any, __shfl_xor(hi_any, off, 64));
+    lo_all = max(lo_all, __shfl_xor(lo_all, off, 64));
+    hi_all = min(hi_all, __shfl_xor(hi_all, off, 64));
+  }
+  lo_any = max(lo_any, key_begin);
+  hi_any = min(hi_any, key_end - 1);
+
+  const int* table = block_table + (size_t)b * table_width;
+  const scalar_ints table_s = (scalar_ints)table;
+  const bool page_missing = span_lacks_page(table, table_width, num_pages, page_size, lo_any, hi_any, lane);
+  const QuantHead at = quant_head(page_size, HEAD_DIM, BITS);
+  const size_t page_bytes = (size_t)at.bytes * n_kv_heads;
+  const uint8_t* base = cache + (size_t)at.bytes * g0;
+
+  // the operands that pick one group's step out of a key's words (element 2 i + 1 of the first eight), and a row of ones
+  Frag8 pick[4], ones;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t one = j == 0 ? 0x3f800000u : 0u;
+    pick[i].u = make_uint4(i == 0 ? one : 0, i == 1 ? one : 0, i == 2 ? one : 0, i == 3 ? one : 0);
+  }
+  ones.u = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+
+  // page of a key; keys outside the item and slots without a page read page 0 and are masked
+  auto page_of = [&](int key, int& slot_in_page) -> int {
+    const int lp = page_shift >= 0 ? (key >> page_shift) : (key / page_size);
+    slot_in_page = key - lp * page_size;
+    const int page = (key < key_end && lp < table_width) ? table[lp] : 0;
+    return (page >= 0 && page < num_pages) ? page : 0;
+  };
+  const int krel = 8 * (n >> 2) + (n & 3);
+  auto issue = [&](Keys& L, int kt) {
+    const uint8_t *kpage, *vpage;
+    int ks, vs;
+    if constexpr (PAGE32) {  // a tile lies in one page, whose number is read as a scalar
+      const int lp = page_shift >= 0 ? (kt >> page_shift) : (kt / page_size);
+      int page = lp < table_width ? table_s[lp] : 0;
+      page = (page >= 0 && page < num_pages) ? page : 0;
+      kpage = vpage = base + (size_t)page * page_bytes;
+      ks = kt - lp * page_size + krel;
+      vs = kt - lp * page_size + 8 * j;
+    } else {
+      kpage = base + (size_t)page_of(kt + krel, ks) * page_bytes;
+      vpage = base + (size_t)page_of(kt + 8 * j, vs) * page_bytes;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      load_words<Keys::KC>(kpage + (uint32_t)((ks + 4 * t) * 4 + j) * (Keys::KC * 4), L.kc[t]);
+      load_words<G>(kpage + at.key_words + (uint32_t)(ks + 4 * t) * (G * 4), L.kw[t]);
+    }
+    load_words<8>(vpage + at.value_words + (uint32_t)vs * 4, L.vw);
+    const uint8_t* vb = vpage + at.values + (uint32_t)(vs >> 3) * (HEAD_DIM * BITS);
+    constexpr int PIECES = Keys::VC / 4;
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c) load_words<4>(vb + 256 * c + 16 * n, *(uint32_t(*)[4])&L.vc[4 * c]);
+    if constexpr (Keys::VC % 4 != 0) load_words<2>(vb + 256 * PIECES + 8 * n, *(uint32_t(*)[2])&L.vc[4 * PIECES]);
+  };
+
+  float4v acc[RT][D_TILES], bsum[RT];
+  float m_run[RT], neg_mc[RT], l_run[RT], z_run[RT];
+  const float lazy_raw = 8.0f / scale_log2e;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+    for (int d = 0; d < D_TILES; ++d) acc[rt][d] = (float4v){0.f, 0.f, 0.f, 0.f};
+    bsum[rt] = (float4v){0.f, 0.f, 0.f, 0.f};
+    m_run[rt] = neg_inf, neg_mc[rt] = 0.f, l_run[rt] = 0.f, z_run[rt] = 0.f;
+  }
+
+  auto compute = [&](const Keys& L, int kt) {
+    const float4v zero = (float4v){0.f, 0.f, 0.f, 0.f};
+    float4v st[RT][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      Frag8 words[QUADS];
+#pragma unroll
+      for (int u = 0; u < QUADS; ++u)
+        words[u].u = make_uint4(L.kw[t][4 * u], 4 * u + 1 < G ? L.kw[t][(4 * u + 1) % G] : 0u, 4 * u + 2 < G ? L.kw[t][(4 * u + 2) % G] : 0u,
+                                4 * u + 3 < G ? L.kw[t][(4 * u + 3) % G] : 0u);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        st[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(words[0].v, qs[rt][0].v, zero, 0, 0, 0);
+        if constexpr (QUADS > 1) st[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(words[QUADS - 1].v, qs[rt][QUADS - 1].v, st[rt][t], 0, 0, 0);
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        Frag8 kf;
+        if constexpr (BITS == 4) {
+          const uint32_t c = L.kc[t][g % Keys::KC];
+          kf.u = make_uint4(C::nibbles(c), C::nibbles(c >> 4), C::nibbles(c >> 8), C::nibbles(c >> 12));
+        } else {
+          const uint32_t c0 = L.kc[t][(2 * g) % Keys::KC], c1 = L.kc[t][(2 * g + 1) % Keys::KC];
+          kf.u = make_uint4(C::bytes(c0, 0), C::bytes(c0, 2), C::bytes(c1, 0), C::bytes(c1, 2));
+        }
+        const float4v step = __builtin_amdgcn_mfma_f32_16x16x32_bf16(words[g / 4].v, pick[g % 4].v, zero, 0, 0, 0);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float4v d = zero;
+#pragma unroll
+          for (int p = PARTS - 1; p >= 0; --p) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.v, qf[rt][p][g].v, d, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st[rt][t][i] = fmaf(step[i], d[i], st[rt][t][i]);
+        }
+      }
+    }
+    const bool need_mask = kt < lo_all || kt + 31 > hi_all;
+    Frag8 bf[RT][PARTS];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float x[8] = {st[rt][0][0], st[rt][0][1], st[rt][0][2], st[rt][0][3], st[rt][1][0], st[rt][1][1], st[rt][1][2], st[rt][1][3]};
+      uint32_t hidden = 0;
+      if (need_mask) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = kt + 8 * j + e;
+          const bool ok = row_valid[rt] && key <= row_end[rt] && key >= row_start[rt] && key >= key_begin && key < key_end;
+          hidden |= ok ? 0u : 1u << e;
+          x[e] = ok ? x[e] : neg_inf;
+        }
+      }
+#define MAXIMUM(a, b) __builtin_elementwise_maximum(a, b)
+      float top = MAXIMUM(MAXIMUM(MAXIMUM(x[0], x[1]), MAXIMUM(x[2], x[3])), MAXIMUM(MAXIMUM(x[4], x[5]), MAXIMUM(x[6], x[7])));
+      // m is a reference, not the maximum: it moves, and what has been summed is rescaled, when a row's scores outgrow it by
+      // a factor of 256 in p
+      if (__any(top - m_run[rt] > lazy_raw)) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float highest = fmaxf(m_run[rt], top);
+        const float m_new = highest - m_run[rt] > lazy_raw ? highest : m_run[rt];
+        const float neg = m_new == neg_inf ? 0.f : -m_new * scale_log2e;
+        const float alpha = __builtin_amdgcn_exp2f(fmaf(m_run[rt], scale_log2e, neg));
+        l_run[rt] *= alpha, z_run[rt] *= alpha;
+        bsum[rt] *= alpha;
+#pragma unroll
+        for (int d = 0; d < D_TILES; ++d) acc[rt][d] *= alpha;
+        m_run[rt] = m_new, neg_mc[rt] = neg;
+      }
+      float bv[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(x[e], scale_log2e, neg_mc[rt]));
+        l_run[rt] += p;
+        bv[e] = p * word_step(L.vw[e]);
+        x[e] = p * word_offset(L.vw[e]);
+      }
+      if (need_mask) {  // a key that a row does not read may hold anything, a NaN among it
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          bv[e] = (hidden >> e) & 1 ? 0.f : bv[e];
+          x[e] = (hidden >> e) & 1 ? 0.f : x[e];
+        }
+      }
+      z_run[rt] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+      if constexpr (EXACT) {
+        Frag8 part[3]; three_parts(bv, part); bf[rt][0] = part[0], bf[rt][1 % PARTS] = part[1], bf[rt][2 % PARTS] = part[2];
+      } else {
+        bf[rt][0].u = make_uint4(pack2_bf16(bv[0], bv[1]), pack2_bf16(bv[2], bv[3]), pack2_bf16(bv[4], bv[5]), pack2_bf16(bv[6], bv[7]));
+        bsum[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones.v, bf[rt][0].v, bsum[rt], 0, 0, 0);
+      }
+    }
+    // tile d of the output: 4 bits: dimension 64 c + 4 m + i of d = 4 c + i (the last two, where 32 are left, 64 c + 2 m + i);
+    // 8 bits: 32 c + 2 m + i of d = 2 c + i
+#pragma unroll
+    for (int d = 0; d < D_TILES; ++d) {
+      Frag8 vf;
+      if constexpr (BITS == 4) {
+        const uint32_t c0 = L.vc[2 * (d / 2)] >> (4 * (d & 1)), c1 = L.vc[2 * (d / 2) + 1] >> (4 * (d & 1));
+        vf.u = make_uint4(C::nibbles(c0), C::nibbles(c0 >> 8), C::nibbles(c1), C::nibbles(c1 >> 8));
+      } else {
+        const uint32_t c0 = L.vc[(2 * d) % Keys::VC], c1 = L.vc[(2 * d + 1) % Keys::VC];
+        vf.u = make_uint4(C::bytes(c0, 0), C::bytes(c0, 2), C::bytes(c1, 0), C::bytes(c1, 2));
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int p = PARTS - 1; p >= 0; --p) acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, bf[rt][p].v, acc[rt][d], 0, 0, 0);
+    }
+  };
+
+  // wavefront w starts at the item's tile w and goes on in steps of TEAM tiles, or takes every tile
+  constexpr int STEP = SPLIT ? TEAM : 1;
+  const int tile0 = key_begin >> 5, tiles = ((key_end + 31) >> 5) - tile0;
+  int tile = SPLIT ? wave : 0;
+  if (tile < tiles) {
+    Keys now, next;
+    issue(now, 32 * (tile0 + tile));
+    for (; tile + STEP < tiles; tile += STEP) {
+      issue(next, 32 * (tile0 + tile + STEP));
+      compute(now, 32 * (tile0 + tile));
+      now = next;
+    }
+    compute(now, 32 * (tile0 + tile));
+  }
+
+  // ---- a row's sums over its lanes, and the output that the sums stand for ------------------- //
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l_run[rt] += __shfl_xor(l_run[rt], 16, 64);
+    l_run[rt] += __shfl_xor(l_run[rt], 32, 64);
+    z_run[rt] += __shfl_xor(z_run[rt], 16, 64);
+    z_run[rt] += __shfl_xor(z_run[rt], 32, 64);
+    const float add = fmaf(-C::OFF, bsum[rt][0], z_run[rt]);
+#pragma unroll
+    for (int d = 0; d < D_TILES; ++d) acc[rt][d] += add;
+  }
+  // calls put(first dimension, values) for the lane's share of a row: four values of neighbouring dimensions, or two
+  auto each_piece = [&](int rt, auto&& put) {
+    constexpr int FOURS = BITS == 4 ? G / 2 : 0;
+#pragma unroll
+    for (int c = 0; c < FOURS; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        put(64 * c + 16 * j + 4 * i, 4, (float4v){acc[rt][4 * c][i], acc[rt][(4 * c + 1) % D_TILES][i], acc[rt][(4 * c + 2) % D_TILES][i], acc[rt][(4 * c + 3) % D_TILES][i]});
+#pragma unroll
+    for (int d = 4 * FOURS; d < D_TILES; d += 2)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) put(16 * d + 8 * j + 2 * i, 2, (float4v){acc[rt][d][i], acc[rt][(d + 1) % D_TILES][i], 0.f, 0.f});
+  };
+  auto store_out = [&](T* row, int d, int count, float4v v) {
+    if constexpr (EXACT) {
+      *(float2*)(row + d) = make_float2(v[0], v[1]);
+      if (count == 4) *(float2*)(row + d + 2) = make_float2(v[2], v[3]);
+    } else {
+      if (count == 4)
+        *(uint2*)(row + d) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+      else
+        *(uint32_t*)(row + d) = pack2_bf16(v[0], v[1]);
+    }
+  };
+
+  if constexpr (!SPLIT) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (!row_valid[rt]) continue;
+      if (slot < 0) {
+        const float inv = page_missing ? not_a_number() : 1.0f / l_run[rt];
+        T* row = out + (size_t)(q0 + ti[rt]) * out_stride + (size_t)hq[rt] * HEAD_DIM;
+        each_piece(rt, [&](int d, int count, float4v v) { store_out(row, d, count, v * inv); });
+      } else {
+        // row tile k of a cut item has the slots from slot + k * (chunks of the item) on
+        float* row = partial + (((size_t)slot + (size_t)(RT * wave + rt) * n_chunks) * n_kv_heads + g0) * 16 * PARTIAL_STRIDE + (size_t)n * PARTIAL_STRIDE;
+        each_piece(rt, [&](int d, int count, float4v v) {
+          *(float2*)(row + d) = make_float2(v[0], v[1]);
+          if (count == 4) *(float2*)(row + d + 2) = make_float2(v[2], v[3]);
+        });
+        if (j == 0) {
+          row[HEAD_DIM] = m_run[rt] * scale_log2e;
+          row[HEAD_DIM + 1] = page_missing ? not_a_number() : l_run[rt];
+        }
+      }
+    }
+  } else {
+    static_assert(!SPLIT || RT == 1, "a team shares one row tile");
+    // the team's wavefronts join: the largest reference, every wavefront's sums and output scaled to it
+    __shared__ float team_m[TEAM][16], team_l[TEAM][16];
+    __shared__ __attribute__((aligned(16))) float team_o[TEAM][16][HEAD_DIM + 4];
+    if (j == 0) {
+      team_m[wave][n] = m_run[0];
+      team_l[wave][n] = l_run[0];
+    }
+    __syncthreads();
+    float m_all = neg_inf;
+#pragma unroll
+    for (int w2 = 0; w2 < TEAM; ++w2) m_all = fmaxf(m_all, team_m[w2][n]);
+    float l_all = 0.f, mine = 0.f;
+#pragma unroll
+    for (int w2 = 0; w2 < TEAM; ++w2) {
+      const float mw = team_m[w2][n];  // -inf: that wavefront had no tile, or none with a key of this row
+      const float f = mw == neg_inf ? 0.f : __builtin_amdgcn_exp2f((mw - m_all) * scale_log2e);
+      l_all += mw == neg_inf ? 0.f : team_l[w2][n] * f;
+      if (w2 == wave) mine = f;
+    }
+    each_piece(0, [&](int d, int count, float4v v) {
+      float* o = &team_o[wave][n][d];
+      if (count == 4)
+        *(float4v*)o = v * mine;
+      else
+        *(float2*)o = make_float2(v[0] * mine, v[1] * mine);
+    });
+    __syncthreads();
+    if (!row_valid[0]) return;
+    const float inv = page_missing ? not_a_number() : 1.0f / l_all;
+    T* orow = out + (size_t)(q0 + ti[0]) * out_stride + (size_t)hq[0] * HEAD_DIM;
+    float* prow = partial + (((size_t)max(slot, 0) * n_kv_heads + g0) * 16 + n) * PARTIAL_STRIDE;
+    for (int d = 16 * wave + 4 * j; d < HEAD_DIM; d += 16 * TEAM) {
+      float4v sum = *(const float4v*)&team_o[0][n][d];
+#pragma unroll
+      for (int w2 = 1; w2 < TEAM; ++w2) sum += *(const float4v*)&team_o[w2][n][d];
+      if (slot < 0)
+        store_out(orow, d, 4, sum * inv);
+      else
+        *(float4v*)(prow + d) = sum;
+    }
+    if (slot >= 0 && wave == 0 && j == 0) {
+      prow[HEAD_DIM] = m_all * scale_log2e;
+      prow[HEAD_DIM + 1] = page_missing ? not_a_number() : l_all;
+    }
+  }
+}
+
+// Joins the partial results of a row: merge item {sequence, first row, first slot, number of partials}; grid (items,
+// key/value heads, 16 rows), a thread for each of 4 neighbouring dimensions and each `blockDim.y`-th partial.
+template <typename T>
+__global__ void attention_quant_merge_kernel(T* __restrict__ out, long out_stride, const float* __restrict__ partial, const int* __restrict__ cu_q,
+                                             const int* __restrict__ merge, int n_q_heads, int n_kv_heads) {
+  const int* item = merge + (size_t)blockIdx.x * 4;
+  const int b = item[0], first = item[2], count = item[3];
+  const int g = blockIdx.y, n = blockIdx.z, group = n_q_heads / n_kv_heads;
+  const int q0 = cu_q[b], r = item[1] + n;
+  if (r >= (cu_q[b + 1] - q0) * group || count <= 0) return;  // also null items, whose first row lies beyond every sequence's
+  const float neg_inf = -__builtin_inff();
+  __shared__ __attribute__((aligned(16))) float o_of[16][HEAD_DIM];
+  __shared__ float l_of[16];
+  const float* rows = partial + ((size_t)first * n_kv_heads + g) * 16 * PARTIAL_STRIDE + (size_t)n * PARTIAL_STRIDE;
+  const size_t stride = (size_t)n_kv_heads * 16 * PARTIAL_STRIDE;
+  float top = neg_inf;
+  for (int p = 0; p < count; ++p) top = fmaxf(top, rows[p * stride + HEAD_DIM]);
+  const int d = 4 * threadIdx.x;
+  float4v sum = (float4v){0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  for (int p = threadIdx.y; p < count; p += blockDim.y) {
+    const float m = rows[p * stride + HEAD_DIM];
+    if (m == neg_inf) continue;  // a chunk with no key of this row
+    const float f = __builtin_amdgcn_exp2f(m - top);
+    l += f * rows[p * stride + HEAD_DIM + 1];
+    sum += f * *(const float4v*)(rows + p * stride + d);
+  }
+  *(float4v*)&o_of[threadIdx.y][d] = sum;
+  if (threadIdx.x == 0) l_of[threadIdx.y] = l;
+  __syncthreads();
+  if (threadIdx.y != 0) return;
+  float total = l_of[0];
+  for (int y = 1; y < (int)blockDim.y; ++y) {
+    total += l_of[y];
+    sum += *(const float4v*)&o_of[y][d];
+  }
+  const int ti = r / group;
+  T* row = out + (size_t)(q0 + ti) * out_stride + (size_t)(g * group + r - ti * group) * HEAD_DIM + d;
+  const float inv = 1.0f / total;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) Elem<T>::store(row + e, sum[e] * inv);
+}
+
+extern "C" int cwm_attention_quant_head_dim() { return HEAD_DIM; }
+
+extern "C" int cwm_attention_quant(const void* q, long q_stride, int dtype, void* out, long out_stride, const void* cache, const int* block_table,
+                                   int table_width, const int* cu_q, const int* kv_len, const int* work, int n_work, const int* work_wide,
+                                   int n_work_wide, int wide_tiles, const int* merge, int n_merge, float* partial, int n_q_heads, int n_kv_heads,
+                                   int head_dim, int page_size, int num_pages, int window_left, float scale, int bits, hipStream_t stream) {
+  QUANT_REQUIRE_SIZES("attention_quant");
+  CWM_REQUIRE(head_dim == HEAD_DIM, "attention_quant: this library is built for head_dim %d, not %d", HEAD_DIM, head_dim);
+  CWM_REQUIRE(n_q_heads > 0 && n_q_heads % n_kv_heads == 0, "attention_quant: %d query heads do not divide into %d key/value heads", n_q_heads, n_kv_heads);
+  const int piece = dtype == CWM_BF16 ? 8 : 4;
+  CWM_REQUIRE(q_stride % piece == 0 && out_stride % 4 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)cache % 16 == 0,
+              "attention_quant: rows must be 16-byte aligned");
+  CWM_REQUIRE(n_work >= 0 && n_work_wide >= 0 && n_merge >= 0, "attention_quant: negative work counts");
+  CWM_REQUIRE(n_work_wide == 0 || wide_tiles == 8, "attention_quant: wide items have 8 row tiles, not %d", wide_tiles);
+  CWM_REQUIRE(n_merge == 0 || partial, "attention_quant: partial buffer missing");
+  CWM_REQUIRE(scale > 0.f, "attention_quant: the scale is positive");
+  CWM_REQUIRE((unsigned long long)quant_token_bytes(head_dim, bits) * page_size < (1ull << 31), "attention_quant: a page of %d keys is too large", page_size);
+  CWM_REQUIRE(n_kv_heads <= 65535 && (long long)(n_work + n_work_wide) * n_kv_heads <= 0x7fffffffLL, "attention_quant: too much work");
+  const float scale_log2e = scale * 1.4426950408889634f;
+  int page_shift = -1;
+  if ((page_size & (page_size - 1)) == 0) {
+    page_shift = 0;
+    while ((1 << page_shift) < page_size) ++page_shift;
+  }
+#define CALL_ATTEND(T, BITS, RT, SPLIT, PAGE32, WORK, COUNT)                                                                                        \
+  hipLaunchKernelGGL((attention_quant_kernel<T, BITS, RT, SPLIT, PAGE32>), dim3((unsigned)((COUNT)*n_kv_heads)), dim3(256), 0, stream, (const T*)q, \
+                     q_stride, (T*)out, out_stride, (const uint8_t*)cache, block_table, table_width, cu_q, kv_len, WORK, partial, n_q_heads,        \
+                     n_kv_heads, page_size, page_shift, num_pages, window_left, scale_log2e)
+#define CALL_BITS(T, RT, SPLIT, PAGE32, WORK, COUNT) \
+  if (bits == 4)                                     \
+    CALL_ATTEND(T, 4, RT, SPLIT, PAGE32, WORK, COUNT); \
+  else                                               \
+    CALL_ATTEND(T, 8, RT, SPLIT, PAGE32, WORK, COUNT)
+#define CALL_PAGES(T, RT, SPLIT, WORK, COUNT)      \
+  if (page_size % 32 == 0) {                       \
+    CALL_BITS(T, RT, SPLIT, true, WORK, COUNT);    \
+  } else {                                         \
+    CALL_BITS(T, RT, SPLIT, false, WORK, COUNT);   \
+  }
+  // float32 queries need three operands for each of theirs: one row tile a wavefront is what its registers hold
+  if (n_work > 0) {
+    if (dtype == CWM_BF16) {
+      CALL_PAGES(bf16_t, 1, true, work, n_work)
+    } else {
+      CALL_PAGES(float, 1, true, work, n_work)
+    }
+    if (int status = cwm_launch_status("attention_quant")) return status;
+  }
+  if (n_work_wide > 0) {
+    if (dtype == CWM_BF16) {
+      CALL_PAGES(bf16_t, 2, false, work_wide, n_work_wide)
+    } else {
+      CALL_PAGES(float, 2, false, work_wide, n_work_wide)
+    }
+    if (int status = cwm_launch_status("attention_quant (rows)")) return status;
+  }
+  if (n_merge > 0) {
+    const dim3 grid(n_merge, n_kv_heads, 16), block(HEAD_DIM / 4, HEAD_DIM <= 128 ? 8 : 4);
+    if (dtype == CWM_BF16)
+      hipLaunchKernelGGL((attention_quant_merge_kernel<bf16_t>), grid, block, 0, stream, (bf16_t*)out, out_stride, partial, cu_q, merge, n_q_heads, n_kv_heads);
+    else
+      hipLaunchKernelGGL((attention_quant_merge_kernel<float>), grid, block, 0, stream, (float*)out, out_stride, partial, cu_q, merge, n_q_heads, n_kv_heads);
+    if (int status = cwm_launch_status("attention_quant (merge)")) return status;
+  }
+  return 0;
+}

@@ -1,0 +1,445 @@
+// Writes keys and values into the cache of 4 or 8 bits (layout and formulas: quant_cache.h) and reads them back.
+//
+// Both kernels take eight tokens of the list at a time, the tokens of one value block where the list follows a sequence.
+// Four lanes share a token's head, lane j with the elements 32 g + 8 j .. + 7 of every group g: a lane's codes of a key are
+// one piece of memory, the largest and smallest of a group are two exchanges between lanes, and the two elements that a
+// rotation turns are the lane's own.
+#include "quant_cache.h"
+
+CWM_DEFINE_ERROR_API
+
+#define HEADS_A_BLOCK 8
+#define CHUNK 8  // tokens of a block
+
+template <typename T> __device__ __forceinline__ void load8(const T* p, bool aligned, float (&x)[8]);
+template <> __device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, bool aligned, float (&x)[8]) {
+  if (aligned) {
+    const uint4 u = *(const uint4*)p;
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = bf16_to_f32(p[e]);
+  }
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, bool aligned, float (&x)[8]) {
+  if (aligned) {
+    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = p[e];
+  }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, bool aligned, const float (&x)[8]);
+template <> __device__ __forceinline__ void store8<bf16_t>(bf16_t* p, bool aligned, const float (&x)[8]) {
+  if (aligned) {
+    *(uint4*)p = make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = f32_to_bf16(x[e]);
+  }
+}
+template <> __device__ __forceinline__ void store8<float>(float* p, bool aligned, const float (&x)[8]) {
+  if (aligned) {
+    *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
+    *(float4*)(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = x[e];
+  }
+}
+// A number of 64 bits rounded to float32.  The empty instruction keeps the compiler from joining this rounding with one to
+// bfloat16 that follows: rounded once or twice, ties fall differently.
+__device__ __forceinline__ float to_float(double x) {
+  float f = (float)x;
+  asm volatile("" : "+v"(f));
+  return f;
+}
+template <typename T> __device__ __forceinline__ float as_stored(float x);
+template <> __device__ __forceinline__ float as_stored<bf16_t>(float x) { return bf16_to_f32(f32_to_bf16(x)); }
+template <> __device__ __forceinline__ float as_stored<float>(float x) { return x; }
+
+// N words at an address that is a multiple of 4 N bytes, in the widest pieces that allows.
+template <int N> __device__ __forceinline__ void put_words(uint32_t* p, const uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *(uint4*)(p + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) *(uint2*)(p + i) = make_uint2(w[i], w[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = w[i];
+  }
+}
+template <int N> __device__ __forceinline__ void get_words(const uint32_t* p, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 u = *(const uint4*)(p + i);
+      w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint2 u = *(const uint2*)(p + i);
+      w[i] = u.x, w[i + 1] = u.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = p[i];
+  }
+}
+
+// Largest and smallest of eight values; a value that is not finite makes the largest infinite.
+__device__ __forceinline__ void extremes(const float (&x)[8], float& hi, float& lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool finite = (__float_as_uint(x[e]) & 0x7f800000u) != 0x7f800000u;
+    hi = fmaxf(hi, finite ? x[e] : __builtin_inff());
+    lo = fminf(lo, finite ? x[e] : hi);
+  }
+}
+__device__ __forceinline__ void over_lanes(float& hi, float& lo) {  // of the four lanes of a token's head
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    hi = fmaxf(hi, __shfl_xor(hi, off, 64));
+    lo = fminf(lo, __shfl_xor(lo, off, 64));
+  }
+}
+
+// Step and offset of a group, in 64 bits: a step that just fits (a quotient without a remainder) is common among bfloat16
+// numbers and must not be taken for the next larger one.
+template <int BITS> __device__ __forceinline__ uint32_t group_word(float hi, float lo) {
+  constexpr double H = 1 << (BITS - 1);
+  if (hi == __builtin_inff()) return 0x7fc07fc0u;
+  uint32_t z = f32_to_bf16(to_float((H * hi + (H - 1) * lo) / (2 * H - 1)));
+  if ((z & 0x7fffu) == 0x7f80u) z -= 1;  // float32 values next to the largest one: the largest of bfloat16
+  const double zd = word_offset(z);
+  const float need = (float)fmax((hi - zd) / (H - 1), (zd - lo) / H);
+  return ((__float_as_uint(need) + 0xffffu) & 0xffff0000u) | z;
+}
+
+// The code of x.  float32 arithmetic decides it except next to a tie, where it may be off by its own rounding (the
+// quotient is at most 2^7 and three roundings of 2^-24 make it, 2.3e-5 in all): there it is the quotient of 64 bits.
+template <int BITS> __device__ __forceinline__ int code_of(float x, float s, float inv, float z) {
+  constexpr int H = 1 << (BITS - 1);
+  const float t = (x - z) * inv;
+  float r = rintf(t);
+  if (!(fabsf(t - r) < 0.4999f)) r = s > 0.f ? (float)rint(((double)x - (double)z) / (double)s) : 0.f;
+  return (int)fminf(fmaxf(r, -(float)H), (float)(H - 1)) + H;  // a NaN gives H
+}
+
+// A token's place in the cache: the first byte of its page and its slot, or no page.
+struct Place {
+  uint8_t* page;
+  int slot;
+};
+__device__ __forceinline__ Place place_of(uint8_t* cache, long page_bytes, int pos, int seq, const int* __restrict__ block_table, int n_seqs,
+                                          int table_width, int page_size, int num_pages) {
+  Place p = {nullptr, 0};
+  if (pos < 0 || seq < 0 || seq >= n_seqs) return p;
+  const int lp = pos / page_size;
+  const int page = lp < table_width ? block_table[(size_t)seq * table_width + lp] : -1;
+  if (page < 0 || page >= num_pages) return p;
+  p.page = cache + (size_t)page * page_bytes;
+  p.slot = pos - lp * page_size;
+  return p;
+}
+
+// grid: (chunks of eight tokens, groups of eight heads: those of the keys, of the values, then of the queries)
+// block: 32 lanes a head: 8 tokens x 4
+// Bound by memory for prompts (2 bytes in and half a byte out a value) and by its latency for decoded tokens.
+template <typename T, int G, int BITS>
+__global__ void __launch_bounds__(256)
+quant_kv_write_kernel(const T* __restrict__ k, long k_stride, const T* __restrict__ v, long v_stride, T* __restrict__ q, long q_stride,
+                      const int* __restrict__ positions, const int* __restrict__ seq_of_token, const float* __restrict__ inv_freq,
+                      uint8_t* __restrict__ cache, const int* __restrict__ block_table, int n_seqs, int table_width, int page_size, int num_pages,
+                      int n_tokens, int n_kv_heads, int n_q_heads, int kv_groups, bool k_aligned, bool v_aligned, bool q_aligned) {
+  constexpr int D = 32 * G;
+  constexpr int UNITS = BITS == 4 ? D / 2 : D;  // rows of eight bytes of a value block
+  __shared__ double turn_s[CHUNK][D / 2], turn_c[CHUNK][D / 2];
+  __shared__ __attribute__((aligned(8))) uint8_t block_codes[HEADS_A_BLOCK][UNITS][8];
+  __shared__ uint8_t* dst_page[CHUNK];
+  __shared__ int dst_slot[CHUNK];
+
+  const int t0 = blockIdx.x * CHUNK;
+  const int kind = blockIdx.y < kv_groups ? 0 : (blockIdx.y < 2 * kv_groups ? 1 : 2);  // keys, values, queries
+  const int head0 = (blockIdx.y - kind * kv_groups) * HEADS_A_BLOCK;
+  const int tid = threadIdx.x;
+  const int head_in_block = tid >> 5, tk = (tid >> 2) & 7, j = tid & 3;
+  const int t = t0 + tk;
+  const int heads = kind == 2 ? n_q_heads : n_kv_heads;
+  const int head = head0 + head_in_block;
+  const bool mine = t < n_tokens && head < heads;
+  const QuantHead at = quant_head(page_size, D, BITS);
+
+  if (kind != 1 && inv_freq) {
+    // the turns of the eight tokens, once for all heads of the block; in 64 bits, so that a turned key is what the formula
+    // gives, rounded once
+    for (int i = tid; i < CHUNK * (D / 2); i += blockDim.x) {
+      const int tt = i / (D / 2), f = i - tt * (D / 2);
+      if (t0 + tt < n_tokens) {
+        const double turns = (double)positions[t0 + tt] * (double)inv_freq[f] * 0.15915494309189535;
+        sincospi(2.0 * (turns - rint(turns)), &turn_s[tt][f], &turn_c[tt][f]);
+      }
+    }
+  }
+  if (kind == 1 && tid < CHUNK) {
+    Place p = {nullptr, 0};
+    if (t0 + tid < n_tokens)
+      p = place_of(cache, at.bytes * n_kv_heads, positions[t0 + tid], seq_of_token[t0 + tid], block_table, n_seqs, table_width, page_size, num_pages);
+    dst_page[tid] = p.page;
+    dst_slot[tid] = p.slot;
+  }
+  __syncthreads();
+
+  if (kind == 1) {
+    if (mine) {
+      float x[G][8];
+      float hi = -__builtin_inff(), lo = __builtin_inff();
+      const T* row = v + (size_t)t * v_stride + (size_t)head * D + 8 * j;
+#pragma unroll
+      for (int g = 0; g < G; ++g) load8(row + 32 * g, v_aligned, x[g]);
+#pragma unroll
+      for (int g = 0; g < G; ++g) extremes(x[g], hi, lo);
+      over_lanes(hi, lo);
+      const uint32_t word = group_word<BITS>(hi, lo);
+      const float s = word_step(word), z = word_offset(word), inv = 1.f / s;
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; e += BITS == 4 ? 2 : 1) {
+          const int d = 32 * g + 8 * j + e;
+          const int c = code_of<BITS>(x[g][e], s, inv, z);
+          if constexpr (BITS == 4)
+            block_codes[head_in_block][d / 2][tk] = (uint8_t)(c | (code_of<BITS>(x[g][e + 1], s, inv, z) << 4));
+          else
+            block_codes[head_in_block][d][tk] = (uint8_t)c;
+        }
+      if (j == 0 && dst_page[tk]) *(uint32_t*)(dst_page[tk] + (size_t)head * at.bytes + at.value_words + (size_t)dst_slot[tk] * 4) = word;
+    }
+    __syncthreads();
+    // Eight tokens that fill a value block are stored eight bytes at a time; tokens that do not follow one another, or that
+    // begin inside a block, byte by byte.
+    bool whole = dst_page[0] != nullptr && (dst_slot[0] & 7) == 0;
+    for (int i = 1; i < CHUNK; ++i) whole = whole && dst_page[i] == dst_page[0] && dst_slot[i] == dst_slot[0] + i;
+    const int units = min(HEADS_A_BLOCK, n_kv_heads - head0) * UNITS;
+    if (whole) {
+      uint8_t* block = dst_page[0] + (size_t)head0 * at.bytes + at.values + (size_t)(dst_slot[0] >> 3) * UNITS * 8;
+      for (int i = tid; i < units; i += blockDim.x) {
+        const int hb = i / UNITS, u = i - hb * UNITS;
+        uint2 w = *(const uint2*)block_codes[hb][u];
+        if constexpr (BITS == 4) w.x = __builtin_amdgcn_perm(w.x, w.x, 0x03010200u), w.y = __builtin_amdgcn_perm(w.y, w.y, 0x03010200u);
+        *(uint2*)(block + (size_t)hb * at.bytes + u * 8) = w;
+      }
+    } else {
+      for (int i = tid; i < units; i += blockDim.x) {
+        const int hb = i / UNITS, u = i - hb * UNITS;
+        const uint2 w = *(const uint2*)block_codes[hb][u];
+#pragma unroll
+        for (int e = 0; e < CHUNK; ++e) {
+          uint8_t* page = dst_page[e];
+          if (!page) continue;
+          const int slot = dst_slot[e], place = BITS == 4 ? quant_place(slot & 7) : slot & 7;
+          page[(size_t)(head0 + hb) * at.bytes + at.values + ((size_t)(slot >> 3) * UNITS + u) * 8 + place] = (uint8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
+        }
+      }
+    }
+    return;
+  }
+
+  if (!mine) return;
+  const bool is_key = kind == 0;
+  const T* row = (is_key ? k + (size_t)t * k_stride : q + (size_t)t * q_stride) + (size_t)head * D + 8 * j;
+  const bool aligned = is_key ? k_aligned : q_aligned;
+  float x[G][8];
+#pragma unroll
+  for (int g = 0; g < G; ++g) load8(row + 32 * g, aligned, x[g]);
+  if (inv_freq) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const int f = 16 * g + 4 * j + e / 2;
+        const double re = x[g][e], im = x[g][e + 1], c = turn_c[tk][f], s = turn_s[tk][f];
+        x[g][e] = as_stored<T>(to_float(re * c - im * s));
+        x[g][e + 1] = as_stored<T>(to_float(im * c + re * s));
+      }
+  }
+  if (!is_key) {
+    T* out = q + (size_t)t * q_stride + (size_t)head * D + 8 * j;
+#pragma unroll
+    for (int g = 0; g < G; ++g) store8(out + 32 * g, aligned, x[g]);
+    return;
+  }
+  constexpr int WORDS = BITS / 4;  // of a group's eight codes
+  uint32_t codes[G * WORDS], words[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    float hi = -__builtin_inff(), lo = __builtin_inff();
+    extremes(x[g], hi, lo);
+    over_lanes(hi, lo);
+    words[g] = group_word<BITS>(hi, lo);
+    const float s = word_step(words[g]), z = word_offset(words[g]), inv = 1.f / s;
+    int c[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = code_of<BITS>(x[g][e], s, inv, z);
+    if constexpr (BITS == 4) {
+      codes[g] = c[0] | (c[2] << 4) | (c[4] << 8) | (c[6] << 12) | (c[1] << 16) | (c[3] << 20) | (c[5] << 24) | ((uint32_t)c[7] << 28);
+    } else {
+      codes[2 * g] = c[0] | (c[1] << 8) | (c[2] << 16) | ((uint32_t)c[3] << 24);
+      codes[2 * g + 1] = c[4] | (c[5] << 8) | (c[6] << 16) | ((uint32_t)c[7] << 24);
+    }
+  }
+  const Place p = place_of(cache, at.bytes * n_kv_heads, positions[t], seq_of_token[t], block_table, n_seqs, table_width, page_size, num_pages);
+  if (!p.page) return;
+  uint8_t* to = p.page + (size_t)head * at.bytes;
+  put_words<G * WORDS>((uint32_t*)to + ((size_t)p.slot * 4 + j) * G * WORDS, codes);
+  if (j == 0) put_words<G>((uint32_t*)(to + at.key_words) + (size_t)p.slot * G, words);
+}
+
+// Reads the tokens of a list: grid (chunks of eight tokens, groups of eight heads: keys, then values), blocks as above.
+template <typename T, int G, int BITS>
+__global__ void __launch_bounds__(256)
+quant_kv_read_kernel(T* __restrict__ k, T* __restrict__ v, const int* __restrict__ positions, const int* __restrict__ seq_of_token,
+                     const uint8_t* __restrict__ cache, const int* __restrict__ block_table, int n_seqs, int table_width, int page_size,
+                     int num_pages, int n_tokens, int n_kv_heads, int kv_groups) {
+  constexpr int D = 32 * G;
+  constexpr int UNITS = BITS == 4 ? D / 2 : D;
+  constexpr int H = 1 << (BITS - 1);
+  constexpr int WORDS = BITS / 4;
+  const int t0 = blockIdx.x * CHUNK;
+  const bool values = blockIdx.y >= kv_groups;
+  const int head0 = (blockIdx.y - (values ? kv_groups : 0)) * HEADS_A_BLOCK;
+  const int tid = threadIdx.x;
+  const QuantHead at = quant_head(page_size, D, BITS);
+
+  if (!values) {
+    const int t = t0 + ((tid >> 2) & 7), j = tid & 3, head = head0 + (tid >> 5);
+    if (t >= n_tokens || head >= n_kv_heads) return;
+    const Place p = place_of((uint8_t*)cache, at.bytes * n_kv_heads, positions[t], seq_of_token[t], block_table, n_seqs, table_width, page_size, num_pages);
+    uint32_t codes[G * WORDS] = {}, words[G] = {};  // a token without a page reads as zeros
+    if (p.page) {
+      const uint8_t* from = p.page + (size_t)head * at.bytes;
+      get_words<G * WORDS>((const uint32_t*)from + ((size_t)p.slot * 4 + j) * G * WORDS, codes);
+      get_words<G>((const uint32_t*)(from + at.key_words) + (size_t)p.slot * G, words);
+    }
+    T* out = k + ((size_t)t * n_kv_heads + head) * D + 8 * j;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float s = word_step(words[g]), z = word_offset(words[g]);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = BITS == 4 ? (codes[g] >> (4 * (e / 2 + 4 * (e % 2)))) & 15 : (codes[(2 * g + e / 4) % (G * WORDS)] >> (8 * (e & 3))) & 255;
+        x[e] = fmaf(s, (float)(c - H), z);
+      }
+      store8(out + 32 * g, true, x);
+    }
+    return;
+  }
+
+  __shared__ const uint8_t* src_page[CHUNK];
+  __shared__ int src_slot[CHUNK];
+  if (tid < CHUNK) {
+    Place p = {nullptr, 0};
+    if (t0 + tid < n_tokens)
+      p = place_of((uint8_t*)cache, at.bytes * n_kv_heads, positions[t0 + tid], seq_of_token[t0 + tid], block_table, n_seqs, table_width, page_size, num_pages);
+    src_page[tid] = p.page;
+    src_slot[tid] = p.slot;
+  }
+  __syncthreads();
+  // Tokens that follow one another lie in at most two value blocks, of which a thread reads its eight bytes each.
+  const int lead = src_slot[0] & 7, last = min(CHUNK, n_tokens - t0) - 1, second = min(8 - lead, last);
+  bool run = src_page[0] != nullptr && src_page[second] != nullptr;
+  for (int i = 1; i <= last; ++i) {
+    const int first = i < 8 - lead ? 0 : second;
+    run = run && src_page[i] == src_page[first] && src_slot[i] == src_slot[first] + i - first;
+  }
+  run = run && (second < 8 - lead || (src_slot[second] & 7) == 0);
+  const int units = min(HEADS_A_BLOCK, n_kv_heads - head0) * UNITS;
+  for (int i = tid; i < units; i += blockDim.x) {
+    const int hb = i / UNITS, u = i - hb * UNITS, head = head0 + hb;
+    const size_t unit = (size_t)head * at.bytes + at.values + (size_t)u * 8;
+    unsigned long long a = 0, b = 0;
+    if (run) {
+      a = *(const unsigned long long*)(src_page[0] + unit + (size_t)(src_slot[0] >> 3) * UNITS * 8);
+      b = *(const unsigned long long*)(src_page[second] + unit + (size_t)(src_slot[second] >> 3) * UNITS * 8);
+    }
+#pragma unroll
+    for (int e = 0; e < CHUNK; ++e) {
+      if (e > last) break;
+      const uint8_t* page = src_page[e];
+      const int slot = src_slot[e], place = BITS == 4 ? quant_place(slot & 7) : slot & 7;
+      uint32_t byte = 0, word = 0;
+      if (page) {
+        byte = run ? (uint32_t)((e < 8 - lead ? a : b) >> (8 * place)) & 255u : page[unit + (size_t)(slot >> 3) * UNITS * 8 + place];
+        word = *(const uint32_t*)(page + (size_t)head * at.bytes + at.value_words + (size_t)slot * 4);
+      }
+      const float s = word_step(word), z = word_offset(word);
+      T* out = v + ((size_t)(t0 + e) * n_kv_heads + head) * D;
+      if constexpr (BITS == 4) {
+        const float x0 = fmaf(s, (float)((int)(byte & 15) - H), z), x1 = fmaf(s, (float)((int)(byte >> 4) - H), z);
+        if constexpr (sizeof(T) == 2)
+          *(uint32_t*)(out + 2 * u) = pack2_bf16(x0, x1);
+        else
+          *(float2*)(out + 2 * u) = make_float2(x0, x1);
+      } else {
+        Elem<T>::store(out + u, fmaf(s, (float)((int)byte - H), z));
+      }
+    }
+  }
+}
+
+// ---- entry points ------------------------------------------------------------------------ //
+#define FOR_GROUPS(CALL, BITS)                                    switch (head_dim / 32) {                                          case 1: CALL(1, BITS); break;                                   case 2: CALL(2, BITS); break;                                   case 3: CALL(3, BITS); break;                                   case 4: CALL(4, BITS); break;                                   case 5: CALL(5, BITS); break;                                   case 6: CALL(6, BITS); break;                                   case 7: CALL(7, BITS); break;                                   default: CALL(8, BITS); break;                                }
+
+extern "C" int cwm_quant_kv_write(const void* k, long k_stride, const void* v, long v_stride, void* q, long q_stride, int dtype, const int* positions,
+                                  const int* seq_of_token, const float* inv_freq, void* cache, const int* block_table, int n_seqs, int table_width,
+                                  int page_size, int num_pages, int n_tokens, int n_kv_heads, int n_q_heads, int head_dim, int bits,
+                                  hipStream_t stream) {
+  QUANT_REQUIRE_SIZES("quant_kv_write");
+  CWM_REQUIRE(n_tokens >= 0 && n_q_heads >= 0 && n_seqs >= 0, "quant_kv_write: negative sizes");
+  if (n_tokens == 0) return 0;
+  CWM_REQUIRE(k && v && cache && block_table && positions && seq_of_token, "quant_kv_write: a tensor is missing");
+  CWM_REQUIRE(q || n_q_heads == 0, "quant_kv_write: queries missing");
+  CWM_REQUIRE(((uintptr_t)cache % 16) == 0, "quant_kv_write: the cache must be 16-byte aligned");
+  const int kv_groups = (n_kv_heads + HEADS_A_BLOCK - 1) / HEADS_A_BLOCK;
+  const int q_groups = q && inv_freq ? (n_q_heads + HEADS_A_BLOCK - 1) / HEADS_A_BLOCK : 0;
+  CWM_REQUIRE(2 * kv_groups + q_groups <= 65535, "quant_kv_write: too many heads");
+  const int most_heads = q_groups ? HEADS_A_BLOCK : (n_kv_heads < HEADS_A_BLOCK ? n_kv_heads : HEADS_A_BLOCK);
+  const dim3 grid((n_tokens + CHUNK - 1) / CHUNK, 2 * kv_groups + q_groups), block(64 * ((most_heads + 1) / 2));
+  const int piece = dtype == CWM_BF16 ? 8 : 4;
+  const bool ka = k_stride % piece == 0 && (uintptr_t)k % 16 == 0, va = v_stride % piece == 0 && (uintptr_t)v % 16 == 0;
+  const bool qa = q_stride % piece == 0 && (uintptr_t)q % 16 == 0;
+#define CALL_WRITE(G, BITS)                                                                                                                       if (dtype == CWM_BF16)                                                                                                                            hipLaunchKernelGGL((quant_kv_write_kernel<bf16_t, G, BITS>), grid, block, 0, stream, (const bf16_t*)k, k_stride, (const bf16_t*)v, v_stride,                        (bf16_t*)q, q_stride, positions, seq_of_token, inv_freq, (uint8_t*)cache, block_table, n_seqs, table_width, page_size,                          num_pages, n_tokens, n_kv_heads, n_q_heads, kv_groups, ka, va, qa);                                                        else                                                                                                                                              hipLaunchKernelGGL((quant_kv_write_kernel<float, G, BITS>), grid, block, 0, stream, (const float*)k, k_stride, (const float*)v, v_stride,                          (float*)q, q_stride, positions, seq_of_token, inv_freq, (uint8_t*)cache, block_table, n_seqs, table_width, page_size,                           num_pages, n_tokens, n_kv_heads, n_q_heads, kv_groups, ka, va, qa)
+  if (bits == 4) {
+    FOR_GROUPS(CALL_WRITE, 4)
+  } else {
+    FOR_GROUPS(CALL_WRITE, 8)
+  }
+  return cwm_launch_status("quant_kv_write");
+}
+
+extern "C" int cwm_quant_kv_read(void* k, void* v, int dtype, const int* positions, const int* seq_of_token, const void* cache, const int* block_table,
+                                 int n_seqs, int table_width, int page_size, int num_pages, int n_tokens, int n_kv_heads, int head_dim, int bits,
+                                 hipStream_t stream) {
+  QUANT_REQUIRE_SIZES("quant_kv_read");
+  CWM_REQUIRE(n_tokens >= 0 && n_seqs >= 0, "quant_kv_read: negative sizes");
+  if (n_tokens == 0) return 0;
+  CWM_REQUIRE(k && v && cache && block_table && positions && seq_of_token, "quant_kv_read: a tensor is missing");
+  CWM_REQUIRE(((uintptr_t)cache % 16) == 0 && ((uintptr_t)k % 16) == 0 && ((uintptr_t)v % 16) == 0, "quant_kv_read: tensors must be 16-byte aligned");
+  const int kv_groups = (n_kv_heads + HEADS_A_BLOCK - 1) / HEADS_A_BLOCK;
+  CWM_REQUIRE(2 * kv_groups <= 65535, "quant_kv_read: too many heads");
+  const dim3 grid((n_tokens + CHUNK - 1) / CHUNK, 2 * kv_groups), block(64 * (((n_kv_heads < HEADS_A_BLOCK ? n_kv_heads : HEADS_A_BLOCK) + 1) / 2));
+#define CALL_READ(G, BITS)                                                                                                                         if (dtype == CWM_BF16)                                                                                                                             hipLaunchKernelGGL((quant_kv_read_kernel<bf16_t, G, BITS>), grid, block, 0, stream, (bf16_t*)k, (bf16_t*)v, positions, seq_of_token,                                 (const uint8_t*)cache, block_table, n_seqs, table_width, page_size, num_pages, n_tokens, n_kv_heads, kv_groups);            else                                                                                                                                               hipLaunchKernelGGL((quant_kv_read_kernel<float, G, BITS>), grid, block, 0, stream, (float*)k, (float*)v, positions, seq_of_token,                                    (const uint8_t*)cache, block_table, n_seqs, table_width, page_size, num_pages, n_tokens, n_kv_heads, kv_groups)
+  if (bits == 4) {
+    FOR_GROUPS(CALL_READ, 4)
+  } else {
+    FOR_GROUPS(CALL_READ, 8)
+  }
+  return cwm_launch_status("quant_kv_read");
+}

@@ -1,0 +1,318 @@
+"""The quantised cache on the GPU: bytes as the layout says, what is read back, and attention over it."""
+
+import math
+
+import pytest
+import torch
+
+from cwm_amd import ops
+from helpers import quantised as held
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _inv_freq(dim):
+    return 1.0 / (500000.0 ** (torch.arange(0, dim, 2).float() / dim))
+
+
+def _garbage(shape, seed):
+    """Bytes of every kind: words that are NaN, infinite and subnormal among them."""
+    return torch.randint(0, 256, shape, dtype=torch.uint8, generator=torch.Generator().manual_seed(seed))
+
+
+def _joined(tokens, q_heads, heads, dim, dtype, seed):
+    """Keys and values as views of a joined projection's rows."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(tokens, (q_heads + 2 * heads) * dim, generator=g)
+    x[:, q_heads * dim : (q_heads + heads) * dim] += 3 * torch.randn(heads * dim, generator=g) * (torch.rand(heads * dim, generator=g) < 0.1)
+    x = x.to(dtype)
+    return x, x[:, : q_heads * dim].unflatten(1, (q_heads, dim)), x[:, q_heads * dim : -heads * dim].unflatten(1, (heads, dim)), x[:, -heads * dim :].unflatten(1, (heads, dim))
+
+
+def _views(x, q_heads, heads, dim):
+    return x[:, : q_heads * dim].unflatten(1, (q_heads, dim)), x[:, q_heads * dim : -heads * dim].unflatten(1, (heads, dim)), x[:, -heads * dim :].unflatten(1, (heads, dim))
+
+
+WRITES = [  # new tokens, lengths, page, heads
+    ([1], [1], 8, 1),
+    ([1, 1, 1], [9, 40, 17], 16, 2),
+    ([8], [16], 8, 3),
+    ([37], [37], 32, 8),
+    ([5, 1, 30], [25, 40, 31], 24, 9),
+    ([64, 3], [64, 70], 256, 17),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_written_bytes(dim, bits, dtype):
+    for i, (new, kv, page, heads) in enumerate(WRITES):
+        step = held.Step(new, kv, page, seed=i)
+        x, _, k, v = _joined(sum(new), 2, heads, dim, dtype, seed=10 + i)
+        before = _garbage((step.pool, *ops.quant_page_shape(heads, dim, page, bits)), i)
+        turned = held.turn(k, step.positions, _inv_freq(dim))
+        want = before.clone()
+        at = step.positions.long()
+        held.put_tokens(want, step.table[step.seq.long(), at // page].long(), at % page, turned, v, bits)
+        cache, xd = before.to(DEV), x.to(DEV)
+        q_d, k_d, v_d = _views(xd, 2, heads, dim)
+        table, positions, seq = step.table.to(DEV), step.positions.to(DEV), step.seq.to(DEV)
+        ops.quant_kv_write(k_d, v_d, positions, _inv_freq(dim).to(DEV), cache, table, seq, bits, q=q_d)
+        off = int((cache.cpu() != want).sum())
+        assert off == 0, (off, new, kv, page, heads)
+        q_want = held.turn(x[:, : 2 * dim].unflatten(1, (2, dim)), step.positions, _inv_freq(dim))
+        assert torch.equal(q_d.cpu(), q_want)
+        assert torch.equal(xd[:, 2 * dim :].cpu(), x[:, 2 * dim :])  # keys and values stay as they are
+        # what is held, read back token by token in another order
+        order = torch.randperm(sum(new), generator=torch.Generator().manual_seed(i))
+        for places in (torch.arange(sum(new)), order):
+            k_r, v_r = ops.quant_kv_read(cache, table, positions[places.to(DEV)], seq[places.to(DEV)], dim, bits, dtype)
+            kc = held.stands_for(*held.hold(turned.reshape(-1, heads, dim // 32, 32), bits), bits).flatten(2)
+            vc = held.stands_for(*held.hold(v, bits), bits)
+            # z + s (c - H) in one fused float32 rounding, then to the type: the float64 value rounded twice
+            assert torch.equal(k_r.cpu(), kc[places].float().to(dtype))
+            assert torch.equal(v_r.cpu(), vc[places].float().to(dtype))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_writing_without_rotation_and_with_loose_rows(bits):
+    """Rows that no vector load can take (an odd token stride, an odd first element), and no table of angles."""
+    dim, heads, page, n = 64, 2, 16, 21
+    step = held.Step([n], [n + 3], page)
+    g = torch.Generator().manual_seed(3)
+    wide = torch.randn(n, 2 * heads * dim + 5, generator=g).bfloat16()
+    for offset in (1, 2, 4):
+        def views(t):
+            return t[:, offset : offset + heads * dim].unflatten(1, (heads, dim)), t[:, offset + heads * dim : offset + 2 * heads * dim].unflatten(1, (heads, dim))
+
+        (k, v), (kd, vd) = views(wide), views(wide.to(DEV))
+        cache = torch.zeros((step.pool, *ops.quant_page_shape(heads, dim, page, bits)), dtype=torch.uint8)
+        want, at = cache.clone(), step.positions.long()
+        held.put_tokens(want, step.table[0, at // page].long(), at % page, k, v, bits)
+        cache = cache.to(DEV)
+        ops.quant_kv_write(kd, vd, step.positions.to(DEV), None, cache, step.table.to(DEV), step.seq.to(DEV), bits)
+        assert torch.equal(cache.cpu(), want)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_writing_values_of_every_kind(bits, dtype):
+    """Equal values, zeros, far ends of the range, subnormal numbers, infinities and NaN."""
+    dim, heads, page, n = 64, 1, 16, 16
+    step = held.Step([n], [n], page)
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(n, heads, dim, generator=g)
+    x[0] = 0.0
+    x[1] = 3.7
+    x[2] *= 1e36
+    x[3] *= 1e-36
+    x[4, 0, 5] = math.inf
+    x[5, 0, 40] = -math.inf
+    x[6, 0, 31] = math.nan
+    x[7, 0, 32:] = 1e-40
+    x[8, 0, 3] = 1e30
+    x[9] = 100.0 + 1e-3 * torch.randn(heads, dim, generator=g)
+    x[10] = torch.where(torch.rand(heads, dim, generator=g) < 0.5, 3.3e38, -3.3e38)
+    x = x.to(dtype)
+    want = torch.zeros((step.pool, *ops.quant_page_shape(heads, dim, page, bits)), dtype=torch.uint8)
+    cache = want.to(DEV)
+    at = step.positions.long()
+    held.put_tokens(want, step.table[0, at // page].long(), at % page, x, x, bits)
+    ops.quant_kv_write(x.to(DEV), x.to(DEV), step.positions.to(DEV), None, cache, step.table.to(DEV), step.seq.to(DEV), bits)
+    assert torch.equal(cache.cpu(), want)
+    k, v = ops.quant_kv_read(cache, step.table.to(DEV), step.positions.to(DEV), step.seq.to(DEV), dim, bits, torch.float32)
+    assert torch.isnan(k[4, 0, :32]).all() and not torch.isnan(k[4, 0, 32:]).any() and torch.isnan(v[4]).all()
+    assert torch.isnan(k[5, 0, 32:]).all() and torch.isnan(v[6]).all() and torch.isfinite(v[:4]).all()
+
+
+def test_tokens_without_a_page():
+    """A token whose page is not held, or lies outside the pool or the table, is not written, and reads as zeros."""
+    dim, heads, page, bits = 32, 2, 8, 4
+    g = torch.Generator().manual_seed(5)
+    k, v = torch.randn(6, heads, dim, generator=g), torch.randn(6, heads, dim, generator=g)
+    table = torch.tensor([[1, -1, 7]], dtype=torch.int32)  # a pool of three pages
+    positions, seq = torch.tensor([0, 8, 16, 24, 7, 2], dtype=torch.int32), torch.tensor([0, 0, 0, 0, 0, 1], dtype=torch.int32)
+    before = _garbage((3, *ops.quant_page_shape(heads, dim, page, bits)), 1)
+    want = before.clone()
+    held.put_tokens(want, torch.tensor([1, 1]), torch.tensor([0, 7]), k[[0, 4]], v[[0, 4]], bits)
+    cache = before.to(DEV)
+    args = positions.to(DEV), seq.to(DEV)
+    ops.quant_kv_write(k.to(DEV), v.to(DEV), args[0], None, cache, table.to(DEV), args[1], bits)
+    assert torch.equal(cache.cpu(), want)
+    kr, vr = ops.quant_kv_read(cache, table.to(DEV), *args, dim, bits, torch.float32)
+    assert not kr[[1, 2, 3, 5]].any() and not vr[[1, 2, 3, 5]].any()
+    assert torch.equal(vr[[0, 4]].cpu(), held.stands_for(*held.hold(v[[0, 4]], bits), bits).float())
+
+
+def test_no_tokens():
+    cache = _garbage((1, *ops.quant_page_shape(1, 32, 8, 4)), 2).to(DEV)
+    none, table = torch.zeros(0, dtype=torch.int32, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    before = cache.clone()
+    ops.quant_kv_write(torch.zeros(0, 1, 32, device=DEV), torch.zeros(0, 1, 32, device=DEV), none, None, cache, table, none, 4)
+    k, v = ops.quant_kv_read(cache, table, none, none, 32, 4, torch.bfloat16)
+    assert torch.equal(cache, before) and k.shape == v.shape == (0, 1, 32)
+
+
+def _case(new, kv, page, q_heads, heads, dim, bits, dtype, window, seed, sharpen=1.5):
+    """The operands of an attention step over a cache that is garbage wherever no key is, and the float64 result."""
+    step = held.Step(new, kv, page, seed=seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    centre = 3 * torch.randn(heads, dim, generator=g) * (torch.rand(heads, dim, generator=g) < 0.1)
+    keys = [(torch.randn(n, heads, dim, generator=g) + centre).to(dtype) for n in kv]
+    values = [(torch.randn(n, heads, dim, generator=g) + 0.5).to(dtype) for n in kv]
+    cache = _garbage((step.pool, *ops.quant_page_shape(heads, dim, page, bits)), seed)
+    held.put_all(cache, step.table, kv, keys, values, bits)
+    q = (sharpen * torch.randn(sum(new), q_heads, dim, generator=g)).to(dtype)
+    return step, cache, q, keys, values
+
+
+def _attend(step, cache, q, bits, window, scale):
+    return ops.quant_paged_attention(q.to(DEV), cache.to(DEV), step.table.to(DEV), step.batch(DEV), window, scale, bits)
+
+
+def _close(got, step, q, keys, values, bits, window, scale):
+    want, limit = held.attention(step, q, keys, values, bits, window, scale)
+    off = (got.cpu().double() - want).abs()
+    assert torch.isfinite(got).all()
+    worst = float((off / limit).max())
+    assert worst <= 1, f"{worst} of the limit, {float(off.max())} off"
+
+
+STEPS = [  # new tokens, lengths, page, query heads, key/value heads, window
+    ([1], [1], 8, 1, 1, None),
+    ([1], [33], 32, 6, 1, None),
+    ([1, 1, 1], [7, 100, 64], 16, 8, 2, None),
+    ([1, 1], [300, 45], 24, 16, 1, 40),
+    ([1, 9, 1, 20], [61, 9, 500, 33], 64, 6, 2, None),
+    ([13], [200], 8, 3, 3, 17),
+    ([1, 1], [2300, 2049], 256, 5, 1, None),  # longer than a block takes: cut and joined
+    ([70], [70], 32, 8, 2, None),  # 280 rows: blocks of 128
+    ([150, 1, 50], [190, 70, 50], 40, 3, 1, 64),
+    ([1], [77], 96, 20, 1, 1),  # more than 16 query heads to a key/value head
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_attention(dim, bits, dtype):
+    for i, (new, kv, page, q_heads, heads, window) in enumerate(STEPS):
+        step, cache, q, keys, values = _case(new, kv, page, q_heads, heads, dim, bits, dtype, window, 100 + i)
+        scale = dim ** -0.5
+        got = _attend(step, cache, q, bits, window, scale)
+        print(dim, bits, dtype, new, kv, page, q_heads, heads, window, flush=True)
+        _close(got, step, q, keys, values, bits, window, scale)
+
+
+@pytest.mark.parametrize("bits,dtype", [(4, torch.bfloat16), (8, torch.bfloat16), (4, torch.float32)])
+def test_long_contexts(bits, dtype):
+    for new, kv, heads, window in [([1], [9001], 2, None), ([1, 1], [70003, 12], 1, None), ([2], [20000], 1, 8195), ([60], [5003], 1, None)]:
+        step, cache, q, keys, values = _case(new, kv, 64, 3 * heads, heads, 64, bits, dtype, window, 7)
+        _close(_attend(step, cache, q, bits, window, 0.125), step, q, keys, values, bits, window, 0.125)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_scores_that_outgrow_their_reference(bits):
+    """Scores that climb by far more than 256 from tile to tile, and fall again."""
+    new, kv, dim = [1, 40], [700, 300], 64
+    step, cache, q, keys, values = _case(new, kv, 32, 4, 1, dim, bits, torch.bfloat16, None, 9)
+    for k in keys:
+        n = k.shape[0]
+        k *= (1 + 3 * torch.sin(torch.arange(n) * 6.0 / n))[:, None, None].to(k.dtype)
+    held.put_all(cache, step.table, kv, keys, values, bits)
+    q *= 8
+    _close(_attend(step, cache, q, bits, None, 0.125), step, q, keys, values, bits, None, 0.125)
+
+
+def test_a_key_that_is_not_finite_reaches_its_readers_only():
+    new, kv, dim, bits = [12, 1], [60, 300], 64, 4
+    step, cache, q, keys, values = _case(new, kv, 16, 4, 2, dim, bits, torch.bfloat16, 20, 11)
+    values[0][55, 1, 3] = math.nan  # head 1: read by the queries at 55 .. 59 (tokens 7 .. 11)
+    keys[1][100, 0, 0] = math.inf  # outside the window of the token at 299
+    held.put_all(cache, step.table, kv, keys, values, bits)
+    got = _attend(step, cache, q, bits, 20, 0.125).reshape(13, 4, dim)
+    bad = torch.isnan(got).all(-1).cpu()
+    want = torch.zeros(13, 4, dtype=torch.bool)
+    want[7:12, 2:] = True
+    assert torch.equal(bad, want) and torch.isfinite(got[~want.to(DEV)]).all()
+
+
+def test_a_missing_page_is_seen():
+    new, kv, dim, bits = [1, 1], [60, 60], 64, 4
+    step, cache, q, keys, values = _case(new, kv, 16, 4, 2, dim, bits, torch.bfloat16, 20, 12)
+    step.table[0, 0] = -1  # given back: the window has passed it
+    step.table[1, 3] = 99
+    got = _attend(step, cache, q, bits, 20, 0.125)
+    assert torch.isfinite(got[0]).all() and torch.isnan(got[1]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_row_does_not_depend_on_its_batch(dtype):
+    dim, bits = 128, 4
+    new, kv = [1, 1, 40, 1], [3000, 77, 40, 513]
+    step, cache, q, keys, values = _case(new, kv, 32, 16, 2, dim, bits, dtype, None, 13)
+    together = _attend(step, cache, q, bits, None, dim ** -0.5)
+    t0 = 0
+    for b, m in enumerate(new):
+        alone = held.Step([m], [kv[b]], 32)
+        alone.table = step.table[b : b + 1].contiguous()
+        got = _attend(alone, cache, q[t0 : t0 + m], bits, None, dim ** -0.5)
+        assert torch.equal(got, together[t0 : t0 + m])
+        t0 += m
+    assert torch.equal(together, _attend(step, cache, q, bits, None, dim ** -0.5))
+
+
+def test_written_then_attended_in_one_stream_of_steps():
+    """A prompt in portions and decoded tokens, as a model's layer runs them: each step writes, then reads."""
+    dim, heads, q_heads, page, bits = 64, 2, 8, 16, 4
+    total, cuts = 75, [0, 30, 31, 62, 63, 64, 75]
+    g = torch.Generator().manual_seed(21)
+    x = torch.randn(total, (q_heads + 2 * heads) * dim, generator=g).bfloat16()
+    full = held.Step([total], [total], page)
+    cache = _garbage((full.pool, *ops.quant_page_shape(heads, dim, page, bits)), 3).to(DEV)
+    got = []
+    for a, b in zip(cuts, cuts[1:]):
+        step = held.Step([b - a], [b], page)
+        step.table = full.table
+        q, k, v = _views(x[a:b].to(DEV), q_heads, heads, dim)
+        batch = step.batch(DEV)
+        ops.quant_kv_write(k, v, batch.positions, _inv_freq(dim).to(DEV), cache, full.table.to(DEV), batch.seq_of_token, bits, q=q)
+        got.append(ops.quant_paged_attention(q, cache, full.table.to(DEV), batch, None, 0.125, bits))
+    q, k, v = _views(x, q_heads, heads, dim)
+    turned = [held.turn(t, full.positions, _inv_freq(dim)) for t in (q, k)]
+    _close(torch.cat(got), full, turned[0], [turned[1]], [v], bits, None, 0.125)
+
+
+def test_on_a_stream_of_its_own_and_captured():
+    dim, bits = 64, 4
+    new, kv = [1, 1], [40, 300]
+    step, cache, q, keys, values = _case(new, kv, 32, 8, 2, dim, bits, torch.bfloat16, None, 17)
+    cache, table, batch = cache.to(DEV), step.table.to(DEV), step.batch(DEV)
+    k, v = torch.randn(2, 2, dim, device=DEV).bfloat16(), torch.randn(2, 2, dim, device=DEV).bfloat16()
+    k2, v2 = torch.randn(2, 2, dim, device=DEV).bfloat16(), torch.randn(2, 2, dim, device=DEV).bfloat16()
+    qd = q.to(DEV)
+    kin, vin = k.clone(), v.clone()
+
+    def layer():
+        ops.quant_kv_write(kin, vin, batch.positions, None, cache, table, batch.seq_of_token, bits)
+        read = ops.quant_kv_read(cache, table, batch.positions, batch.seq_of_token, dim, bits, torch.bfloat16)
+        return (ops.quant_paged_attention(qd, cache, table, batch, None, 0.125, bits), *read)
+
+    want = [t.clone() for t in layer()]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = layer()
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer()
+    for kk, vv in ((k2, v2), (k, v), (k2, v2)):
+        kin.copy_(kk), vin.copy_(vv)
+        graph.replay()
+        replayed = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(replayed, layer()))
