@@ -1,6 +1,7 @@
 // The loop of a matrix product whose operands both pass through LDS: C[m, n] = sum over k of A[m, k] * W[n, k],
-// bfloat16 operands, float32 sums.  Shared by the plain product of many rows (gemm_bf16_wide.hip) and the routed
-// experts' (routed.hip), which differ in where a tile's rows lie and in what becomes of its sums.
+// bfloat16 operands and float32 sums, or 8-bit integers and 32-bit sums.  Shared by the plain product of many rows
+// (gemm_bf16_wide.hip), the routed experts' (routed.hip) and that of integers (gemm_int8.hip), which differ in where a tile's rows
+// lie and in what becomes of its sums.
 //
 // Persistent blocks of eight wavefronts, two along the rows and four along the columns; a wavefront holds WM x WN tiles
 // of 16 x 16 sums.  K goes in steps of 64.  A step's rows of A and W (BM + BN rows of 128 bytes, a cache line each) reach
@@ -42,6 +43,20 @@ struct WideShape {
   static_assert(S >= 3, "a tile needs three buffers");
 };
 
+// The matrix instruction: its operands are 16 bytes of a lane whatever their type.  A loop of another type's operands counts its
+// rows in pairs of bytes as if they were bfloat16 (K and the row strides in units of two bytes).
+struct WideBf16 {
+  typedef float4v Sums;
+  static __device__ __forceinline__ Sums run(const Frag8& w, const Frag8& a, const Sums& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v, a.v, c, 0, 0, 0); }
+};
+typedef int int4v __attribute__((ext_vector_type(4)));
+struct WideInt8 {  // K goes in steps of 128
+  typedef int4v Sums;
+  static __device__ __forceinline__ Sums run(const Frag8& w, const Frag8& a, const Sums& c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4v, w.u), __builtin_bit_cast(int4v, a.u), c, 0, 0, 0);
+  }
+};
+
 template <int WN>
 __device__ __forceinline__ int wide_w_key(int row) {  // of a row of W within the tile (a wavefront's rows are 16 WN in turn)
   return ((row >> 1) & 1) | (((row / (4 * WN)) & 3) << 1);
@@ -50,7 +65,7 @@ __device__ __forceinline__ int wide_w_key(int row) {  // of a row of W within th
 // SOURCE: enter(tile) sets what base(p) answers, where piece p of a step lies (a uniform pointer; pieces p < BM / 8 are A's rows
 // 8 p .., the others eight rows of W, or an operand of half a step), and `off[ND]`, this lane's byte offsets of its loads from there.  SINK: store(tile, acc) writes
 // the sums, with exactly STORES store instructions if it answers true.
-template <int WM, int WN, int STORES, typename SOURCE, typename SINK>
+template <int WM, int WN, int STORES, typename MMA = WideBf16, typename SOURCE, typename SINK>
 __device__ __forceinline__ void wide_loop(unsigned char* lds, SOURCE& src, SINK& sink, int tile, int tile_stride, int n_tiles, int steps) {
   typedef WideShape<WM, WN> Shape;
   constexpr int BM = Shape::BM, ND = Shape::ND, STAGE = Shape::STAGE, S = Shape::S, PIECES = Shape::PIECES;
@@ -88,12 +103,12 @@ __device__ __forceinline__ void wide_loop(unsigned char* lds, SOURCE& src, SINK&
   for (int b = 0; b < WN; ++b) w_piece[b] = SOURCE::W_TILES ? b * 2048 : b * 512 + ((j ^ wide_w_key<WN>(wn * WN * 16 + w_row + 4 * b)) * 16);
   const int a_piece = (j ^ a_key) * 16;
 
-  float4v acc[WM][WN];
+  typename MMA::Sums acc[WM][WN];
   Frag8 a0[WM], b0[WN], a1[WM], b1[WN];
 #define WIDE_READ_A(FA, ST, HALF, i) FA[i].u = *(const uint4*)(a_base + (ST) + (i) * 2048 + (a_piece ^ ((HALF) * 64)))
 #define WIDE_READ_W(FB, ST, HALF, i) FB[i].u = *(const uint4*)(w_base + (ST) + (w_piece[i] ^ ((HALF) * (SOURCE::W_TILES ? 1024 : 64))))
 #define WIDE_ROW(FA, FB, i) \
-  _Pragma("unroll") for (int b = 0; b < WN; ++b) acc[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(FB[b].v, FA[i].v, acc[i][b], 0, 0, 0);
+  _Pragma("unroll") for (int b = 0; b < WN; ++b) acc[i][b] = MMA::run(FB[b], FA[i], acc[i][b]);
   constexpr int READS = (WN + WM + WM - 2) / (WM - 1);  // after a row of matrix instructions, so that none follow the last
 #define WIDE_READS(FA, FB, ST, HALF, i)                                           \
   _Pragma("unroll") for (int q = (i) * READS; q < (i) * READS + READS; ++q) {     \
@@ -119,7 +134,7 @@ __device__ __forceinline__ void wide_loop(unsigned char* lds, SOURCE& src, SINK&
 #pragma unroll
     for (int a = 0; a < WM; ++a)
 #pragma unroll
-      for (int b = 0; b < WN; ++b) acc[a][b] = (float4v){0.f, 0.f, 0.f, 0.f};
+      for (int b = 0; b < WN; ++b) acc[a][b] = (typename MMA::Sums){0, 0, 0, 0};
     for (int k = 0; k < steps; ++k) {
       const int nxt = cur + STAGE == S * STAGE ? 0 : cur + STAGE;
 #pragma unroll

@@ -1,6 +1,7 @@
 """Entry points of the kernels that serve in fewer bits: the paged cache of keys and values in 4 or 8 bits
-(`csrc/quant_cache.hip`, `csrc/attention_quant.hip`; layout and formulas in `csrc/quant_cache.h`).  Shapes, types and devices
-are checked on the host; there is no CPU path."""
+(`csrc/quant_cache.hip`, `csrc/attention_quant.hip`; layout and formulas in `csrc/quant_cache.h`), and the product of 8-bit
+integers with a scale for every token and output channel (`csrc/gemm_int8.hip`).  Shapes, types and devices are checked on the
+host; there is no CPU path."""
 
 from __future__ import annotations
 
@@ -214,3 +215,92 @@ def quant_paged_attention(
         ),
     )
     return out
+
+
+# --------------------------------------------------------------------------- #
+INT8_MAX_K = 131072  # csrc/gemm_int8.hip: 127^2 K fits the 32 bits of a sum
+INT8_FEW_ROWS = 64
+_INT8_TILES = {1: (256, 128), 2: (128, 256), 3: (64, 128), 4: (128, 128)}
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """`x` [M, K] (float32 or bfloat16) as int8 [M, K] and a float32 scale a row [M]: the scale is the row's largest magnitude over
+    127, the integers x / scale rounded, ties to even.  A row of zeros has a scale of 0; one with an infinity or a NaN has a NaN
+    for its scale.  The integers are a view of rows padded with zeros to a multiple of 128, which `linear_int8` likes best for
+    its weights."""
+    KernelError, _check, _code, _i32, _need_gpu, _ptr, _stream = _base()
+    _need_gpu(x)
+    _check_device(x)
+    if x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise KernelError("rows to quantise must be [M, K] with contiguous rows")
+    code = _code(x.dtype)
+    m, k = x.shape
+    padded = -(-k // 128) * 128
+    codes = torch.empty((m, padded), dtype=torch.int8, device=x.device)
+    scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    lib = _build.load("gemm_int8")
+    _check(lib, lib.cwm_quantize_rows(_ptr(x), ctypes.c_long(x.stride(0)), code, _ptr(codes), ctypes.c_long(padded), _ptr(scale), m, k, padded, _stream()))
+    return codes[:, :k], scale
+
+
+def int8_limits(n: int, k: int) -> Optional[str]:
+    """Why a weight [n, k] cannot be one of `linear_int8`, or None if it can."""
+    if n < 1 or k < 1 or k % 16 != 0 or k > INT8_MAX_K:
+        return f"the product of 8-bit integers takes rows of a multiple of 16 columns up to {INT8_MAX_K}, not {k}"
+    return None
+
+
+def linear_int8(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    weight_scale: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    out_dtype: Optional[torch.dtype] = None,
+    tile: Optional[int] = None,
+) -> torch.Tensor:
+    """y = x W^T (+ bias) in 8-bit integers: the rows of `x` [M, K] (float32 or bfloat16) are quantised as by `quantize_rows`,
+    multiplied with the int8 `weight` [N, K] with exact 32-bit sums, and scaled by the rows' scales and the float32
+    `weight_scale` [N] (`quantize_rows` of the weight); `bias` float32 [N].  K a multiple of 16, rows of the weight 16-byte
+    aligned.  Returns [M, N] in `out_dtype` (default: x's).  `tile` (tests) names one of the kernels."""
+    KernelError, _check, _code, _i32, _need_gpu, _ptr, _stream = _base()
+    from . import _compute_units
+
+    _need_gpu(x, weight, weight_scale, bias)
+    _check_device(x, weight, weight_scale, bias)
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
+        raise KernelError(f"linear_int8: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
+    m, k = x.shape
+    n = weight.shape[0]
+    why = int8_limits(n, k)
+    if why is not None:
+        raise KernelError(why)
+    if weight.dtype != torch.int8 or weight.stride(1) != 1 or weight.data_ptr() % 16 != 0 or (n > 1 and (weight.stride(0) % 16 != 0 or weight.stride(0) < k)):
+        raise KernelError(f"the weight must be int8 with 16-byte aligned rows, found {weight.dtype} with strides {weight.stride()}")
+    if weight_scale.dtype != torch.float32 or weight_scale.shape != (n,) or not weight_scale.is_contiguous():
+        raise KernelError(f"the weight's scales must be a contiguous float32 [{n}] tensor")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise KernelError(f"linear_int8: the bias must be a contiguous float32 [{n}] tensor")
+    y = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
+    code = _code(y.dtype)
+    if m == 0:
+        _code(x.dtype)
+        return y
+    codes, scale = quantize_rows(x)
+    if tile is None:
+        tile = _int8_tile(m, n, k)
+    lib = _build.load("gemm_int8")
+    _check(
+        lib,
+        lib.cwm_gemm_int8(
+            _ptr(codes), ctypes.c_long(codes.stride(0)), _ptr(scale), _ptr(weight), ctypes.c_long(weight.stride(0) if n > 1 else max(k, weight.stride(0))),
+            _ptr(weight_scale), _ptr(bias), _ptr(y), code, ctypes.c_long(n), m, n, k, _compute_units(x.device), tile, _stream(),
+        ),
+    )
+    return y
+
+
+def _int8_tile(m: int, n: int, k: int) -> int:
+    """The kernel for a product's sizes."""
+    if m <= INT8_FEW_ROWS or k % 128 != 0:
+        return 0
+    return 1

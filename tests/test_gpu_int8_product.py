@@ -1,0 +1,154 @@
+"""The product of 8-bit integers: the integers of a row, every kernel at sizes that end inside its tiles, and the whole call."""
+
+import math
+
+import pytest
+import torch
+
+from cwm_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _rows(m, k, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(m, k, generator=g) * torch.exp(torch.randn(1, k, generator=g))).to(dtype)
+
+
+def _quantised(x):
+    """The definition: float32 scale, true quotients, ties to even."""
+    x = x.float()
+    top = x.abs().amax(1)
+    a = top / torch.full_like(top, 127)
+    c = torch.where(a[:, None] > 0, torch.round(x / a[:, None]), torch.zeros_like(x))
+    return c.to(torch.int8), a
+
+
+def _weight(n, k, seed, stride=None):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randint(-127, 128, (n, stride or k), generator=g).to(torch.int8)
+    return w[:, :k], torch.rand(n, generator=g) * 0.01 + 1e-4
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", [(1, 16), (3, 100), (7, 1), (2, 129), (5, 4096), (300, 2056)])
+def test_integers_of_rows(m, k, dtype):
+    x = _rows(m, k, dtype, m + k)
+    x[0] *= 0
+    codes, scale = ops.quantize_rows(x.to(DEV))
+    want, a = _quantised(x)
+    assert codes.shape == (m, k) and torch.equal(codes.cpu(), want) and torch.equal(scale.cpu(), a)
+    assert codes.stride(0) % 128 == 0 and not codes._base[:, k:].any()
+    wide = torch.cat([x, x[:, :3]], 1).to(DEV)[:, 1 : 1 + k] if k > 1 else x.to(DEV)  # rows that no vector load takes
+    codes, scale = ops.quantize_rows(wide)
+    want, a = _quantised(wide.cpu())
+    assert torch.equal(codes.cpu(), want) and torch.equal(scale.cpu(), a)
+
+
+def test_rows_that_are_not_finite():
+    x = _rows(5, 64, torch.float32, 1)
+    x[1, 3], x[2, 60], x[3, 0] = math.nan, math.inf, -math.inf
+    codes, scale = ops.quantize_rows(x.to(DEV))
+    assert torch.isnan(scale[1:4]).all() and torch.isfinite(scale[[0, 4]]).all() and not codes[1:4].any()
+    w, s = _weight(40, 64, 2)
+    y = ops.linear_int8(x.to(DEV), w.to(DEV), s.to(DEV))
+    assert torch.isnan(y[1:4]).all() and torch.isfinite(y[[0, 4]]).all()
+
+
+def _check(x, w, s, bias, out_dtype, tile=None):
+    y = ops.linear_int8(x.to(DEV), w.to(DEV), s.to(DEV), None if bias is None else bias.to(DEV), out_dtype, tile)
+    codes, a = _quantised(x)
+    exact = (codes.double() @ w.double().t()) * a.double()[:, None] * s.double()
+    # the sum's conversion, two products and the bias's sum, 2^-24 of themselves each, and the result's own rounding
+    limit = 3.01 * 2.0 ** -24 * exact.abs()
+    if bias is not None:
+        exact = exact + bias.double()
+        limit = limit + 2.0 ** -24 * (exact.abs() + limit)
+    limit = limit + (2.0 ** -8 if out_dtype == torch.bfloat16 else 0) * (exact.abs() + limit) + 1e-44
+    assert y.dtype == out_dtype and y.shape == exact.shape
+    off = (y.cpu().double() - exact).abs()
+    assert (off <= limit).all(), (x.shape, w.shape, tile, float((off / limit).max()))
+
+
+SIZES = [  # rows, columns, K
+    (1, 1, 16), (1, 100, 48), (3, 16, 128), (16, 33, 144), (17, 64, 256), (33, 31, 1040), (64, 130, 384), (70, 48, 112), (129, 70, 272),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_products_of_few_rows(dtype):
+    for i, (m, n, k) in enumerate(SIZES):
+        x = _rows(m, k, dtype, i)
+        w, s = _weight(n, k, i)
+        _check(x, w, s, torch.randn(n) if i % 2 else None, dtype, 0)
+        w, s = _weight(n, k, i, stride=k + 16)
+        _check(x, w, s, None, torch.float32, 0)
+
+
+@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+def test_products_of_many_rows(tile):
+    for i, (m, n, k) in enumerate([(1, 1, 128), (65, 100, 256), (300, 130, 384), (257, 513, 1024), (1000, 2000, 512), (513, 1027, 128)]):
+        x = _rows(m, k, torch.bfloat16, i)
+        w, s = _weight(n, k, i, stride=k + 128 * (i % 2))
+        _check(x, w, s, torch.randn(n) if i % 2 else None, torch.bfloat16 if i % 3 else torch.float32, tile)
+
+
+def test_sums_at_the_end_of_their_range():
+    """All integers 127 at the largest K: the sum is 32 bits to the last one."""
+    k = ops.INT8_MAX_K
+    for m, tile in ((2, 0), (70, 3)):
+        x, w = torch.ones(m, k), torch.full((20, k), 127, dtype=torch.int8)
+        _check(x, w, torch.ones(20), None, torch.float32, tile)
+        _check(-x, w, torch.ones(20), None, torch.float32, tile)
+
+
+def test_the_call_chooses_among_its_kernels():
+    for m, n, k in [(1, 2048, 2048), (5, 512, 8192), (40, 4096, 512), (100, 1024, 1024), (600, 1536, 640), (200, 256, 2064)]:
+        x = _rows(m, k, torch.bfloat16, m)
+        w, s = _weight(n, k, m)
+        _check(x, w, s, None, torch.bfloat16)
+
+
+def test_no_rows_and_weights_of_its_own_making():
+    w = torch.randn(48, 200, device=DEV)
+    codes, scale = ops.quantize_rows(w)
+    x = torch.randn(9, 208, device=DEV)
+    with pytest.raises(ops.KernelError, match="multiple of 16"):
+        ops.linear_int8(x[:, :200], codes, scale)
+    codes, scale = ops.quantize_rows(torch.randn(48, 208, device=DEV))
+    _check(x.cpu(), codes.cpu(), scale.cpu(), None, torch.float32)
+    assert ops.linear_int8(x[:0], codes, scale).shape == (0, 48)
+    assert torch.equal(ops.linear_int8(x, codes, scale), ops.linear_int8(x, codes.contiguous(), scale))
+
+
+def test_a_row_does_not_depend_on_its_batch():
+    x = _rows(500, 1024, torch.bfloat16, 3).to(DEV)
+    w, s = (t.to(DEV) for t in _weight(700, 1024, 4))
+    whole = ops.linear_int8(x, w, s)
+    for a, b in ((0, 1), (3, 20), (100, 163), (7, 200), (0, 400)):
+        assert torch.equal(ops.linear_int8(x[a:b], w, s), whole[a:b])
+
+
+def test_on_a_stream_of_its_own_and_captured():
+    x = [_rows(m, 512, torch.bfloat16, m).to(DEV) for m in (3, 200)]
+    other = [t.flip(0) * 2 for t in x]
+    w, s = (t.to(DEV) for t in _weight(300, 512, 5))
+    want = [ops.linear_int8(t, w, s) for t in x]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = [ops.linear_int8(t, w, s) for t in x]
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    held = [t.clone() for t in x]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [ops.linear_int8(t, w, s) for t in held]
+    for source in (other, x, other):
+        for h, t in zip(held, source):
+            h.copy_(t)
+        graph.replay()
+        replayed = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, ops.linear_int8(t, w, s)) for a, t in zip(replayed, source))

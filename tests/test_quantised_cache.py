@@ -145,3 +145,37 @@ def test_attention_that_is_refused(no_device, changed, why):
                 batch=held.Step([3], [5], 16).batch("cpu"), window=None, scale=0.125, bits=4)
     with pytest.raises(ops.KernelError, match=why):
         ops.quant_paged_attention(**{**args, **changed})
+
+
+def _product_args(**changed):
+    a = dict(x=torch.zeros(3, 64), weight=torch.zeros(5, 64, dtype=torch.int8), weight_scale=torch.ones(5), bias=None, out_dtype=None)
+    return {**a, **changed}
+
+
+@pytest.mark.parametrize("changed,why", [
+    (dict(x=torch.zeros(3, 48)), "do not fit"),
+    (dict(x=torch.zeros(64)), "do not fit"),
+    (dict(x=torch.zeros(3, 40), weight=torch.zeros(5, 40, dtype=torch.int8)), "multiple of 16"),
+    (dict(x=torch.zeros(1, 131088), weight=torch.zeros(1, 131088, dtype=torch.int8), weight_scale=torch.ones(1)), "131072"),
+    (dict(weight=torch.zeros(5, 64)), "int8"),
+    (dict(weight=torch.zeros(64, 5, dtype=torch.int8).t()), "int8"),
+    (dict(weight=torch.zeros(5, 72, dtype=torch.int8)[:, :64]), "aligned"),
+    (dict(weight=torch.zeros(1, 64, dtype=torch.int8).expand(5, 64)), "aligned"),
+    (dict(weight_scale=torch.ones(4)), "scales"),
+    (dict(weight_scale=torch.ones(5, dtype=torch.bfloat16)), "scales"),
+    (dict(bias=torch.ones(4)), "bias"),
+    (dict(bias=torch.ones(5, dtype=torch.bfloat16)), "bias"),
+    (dict(out_dtype=torch.float16), "float32 and bfloat16"),
+    (dict(x=torch.zeros(3, 64, dtype=torch.float16), out_dtype=torch.float32), "float32 and bfloat16"),
+    (dict(x=torch.zeros(64, 3).t()), "contiguous rows"),
+])
+def test_products_that_are_refused(no_device, changed, why):
+    with pytest.raises(ops.KernelError, match=why):
+        ops.linear_int8(**_product_args(**changed))
+
+
+def test_the_product_has_no_cpu_path():
+    with pytest.raises(ops.KernelError, match="HIP device"):
+        ops.linear_int8(**_product_args())
+    with pytest.raises(ops.KernelError, match="HIP device"):
+        ops.quantize_rows(torch.zeros(2, 16))
