@@ -53,7 +53,7 @@ class CacheStorage:
         for cid, spec in enumerate(manager.specs):
             if isinstance(spec, PagedKVSpec):
                 pool = manager.groups[manager.group_of_cache[cid]].pool
-                self.paged[cid] = torch.zeros((pool.num_pages, *spec.page_shape(manager.page_size)), dtype=dtype, device=device)
+                self.paged[cid] = torch.zeros((pool.num_pages, *spec.page_shape(manager.page_size)), dtype=spec.element_type(dtype), device=device)
             elif isinstance(spec, StateSpec):
                 self.state[cid] = torch.zeros((manager.max_requests, *spec.shape), dtype=spec.dtype, device=device)
 
@@ -66,12 +66,13 @@ class CacheStorage:
             t[slot].zero_()
 
     def fill_pages(self, group: int, pages: Sequence[int], value: float) -> None:
-        """Overwrite given-back pages (tests poison them to show stale reads)."""
+        """Overwrite given-back pages (tests poison them to show stale reads; pages of bytes with bytes of 255, whose steps
+        and offsets are NaN)."""
         if not pages:
             return
         idx = torch.as_tensor(list(pages), dtype=torch.long, device=self.device)
         for cid in self.manager.groups[group].cache_ids:
-            self.paged[cid][idx] = value
+            self.paged[cid][idx] = value if self.paged[cid].dtype.is_floating_point else 255
 
     def view(self, cache_id: int, batch) -> object:
         spec = self.manager.specs[cache_id]

@@ -35,6 +35,9 @@ class GenArgs:
     min_prefill: int = 512  # reference batching threshold: not needed with mixed steps, ignored
     min_prefill_batch: int = 8  # likewise ignored
 
+    cache_bits: Optional[int] = None  # not in the reference: 4 or 8 to cache keys and values in so many bits (dense decoder only)
+    weight_bits: Optional[int] = None  # not in the reference: 8 to hold the layers' matrices as 8-bit integers with a scale an
+    # output channel and quantise the activations token by token (dense decoder only; embedding and head stay as they are)
     expected_seq: int = -1  # not in the reference: tokens a typical request holds; how free memory is split between
     # layer groups when max_seq is negative (negative: the context length the model's configuration names)
     prefill_gb: float = 2  # memory kept free for activations when max_seq is negative
@@ -47,6 +50,10 @@ class GenArgs:
     def __post_init__(self) -> None:
         if self.host_cache_gb != 0:
             raise ValueError("host_cache_gb: the host prefix cache is not part of this engine, set it to 0")
+        if self.cache_bits not in (None, 4, 8):
+            raise ValueError(f"cache_bits must be 4 or 8 (or left out), found {self.cache_bits}")
+        if self.weight_bits not in (None, 8):
+            raise ValueError(f"weight_bits must be 8 (or left out), found {self.weight_bits}")
         if self.max_batch <= 0:
             raise ValueError("max_batch must be positive")
         if self.cache_block <= 0:

@@ -131,6 +131,9 @@ class Engine:
     ) -> None:
         if model.runtime is None:
             raise RuntimeError("the model has no weights yet")
+        for name, asked, has in (("cache_bits", args.cache_bits, model.cache_bits), ("weight_bits", args.weight_bits, model.runtime.weight_bits)):
+            if asked is not None and asked != has:
+                raise ValueError(f"{name}={asked} is asked for, the model was built with {has}")
         self.args = args
         self.model = model
         self.device = model.runtime.device
@@ -185,8 +188,9 @@ class Engine:
         stop_tokens: Iterable[int] = (),
         seed: int = 17,
     ) -> "Engine":
-        model, _config = load_model(checkpoint_dir, dtype, device)
-        return cls(args or GenArgs(), model, stop_tokens, seed)
+        args = args or GenArgs()
+        model, _config = load_model(checkpoint_dir, dtype, device, cache_bits=args.cache_bits, weight_bits=args.weight_bits)
+        return cls(args, model, stop_tokens, seed)
 
     @classmethod
     def from_random(
@@ -200,8 +204,9 @@ class Engine:
         seed: int = 17,
         std: float = 0.02,
     ) -> "Engine":
-        model, _config = random_model(config, weight_seed, dtype, device, std=std)
-        return cls(args or GenArgs(), model, stop_tokens, seed)
+        args = args or GenArgs()
+        model, _config = random_model(config, weight_seed, dtype, device, std=std, cache_bits=args.cache_bits, weight_bits=args.weight_bits)
+        return cls(args, model, stop_tokens, seed)
 
     # ---- requests ----------------------------------------------------------------- #
     def submit(self, packet: Packet) -> None:

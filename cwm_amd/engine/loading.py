@@ -58,17 +58,19 @@ def wants_stream_copies(model: Model, act_dtype: torch.dtype, device: torch.devi
 
 def load_model(
     folder: str, dtype: Union[str, torch.dtype], device: Union[str, torch.device], keep_float32: bool = False,
-    stream_copies: Optional[bool] = None,
+    stream_copies: Optional[bool] = None, cache_bits: Optional[int] = None, weight_bits: Optional[int] = None,
 ) -> Tuple[Model, Any]:
     """The model that `folder/config.json` names, with the folder's tensors.  In bfloat16 mode
     matrices stored in 32 bits are cast to bfloat16 unless `keep_float32`.  `stream_copies`: see
-    `wants_stream_copies` (None: by the memory there is)."""
+    `wants_stream_copies` (None: by the memory there is).  `cache_bits` (4 or 8) and `weight_bits` (8): see
+    `GenArgs`; None keeps the activations' type."""
     device = torch.device(device)
     act_dtype = parse_dtype(dtype)
     arch, config = load_config(folder)
-    model = Model(arch.build_plan(config))
+    model = Model(arch.build_plan(config), cache_bits)
     tensors = load_tensors(folder, model.tensor_specs(), act_dtype, device, keep_float32)
-    model.bind(tensors, Runtime(device=device, act_dtype=act_dtype, stream_copies=wants_stream_copies(model, act_dtype, device, stream_copies)))
+    copies = wants_stream_copies(model, act_dtype, device, stream_copies)
+    model.bind(tensors, Runtime(device=device, act_dtype=act_dtype, stream_copies=copies, weight_bits=weight_bits))
     return model, config
 
 
@@ -80,16 +82,19 @@ def random_model(
     std: float = 0.02,
     norm_init: str = "ones",
     stream_copies: Optional[bool] = None,
+    cache_bits: Optional[int] = None,
+    weight_bits: Optional[int] = None,
 ) -> Tuple[Model, Any]:
     """A model with random weights drawn on the device, without a folder in between
     (for shapes whose weights would not pass through host memory quickly)."""
     device = torch.device(device)
     act_dtype = parse_dtype(dtype)
     arch, typed = parse_config(config)
-    model = Model(arch.build_plan(typed))
+    model = Model(arch.build_plan(typed), cache_bits)
     tensors = {
         name: random_tensor(name, spec, seed, std, norm_init, act_dtype, device)
         for name, spec in model.tensor_specs().items()
     }
-    model.bind(tensors, Runtime(device=device, act_dtype=act_dtype, stream_copies=wants_stream_copies(model, act_dtype, device, stream_copies)))
+    copies = wants_stream_copies(model, act_dtype, device, stream_copies)
+    model.bind(tensors, Runtime(device=device, act_dtype=act_dtype, stream_copies=copies, weight_bits=weight_bits))
     return model, typed

@@ -7,12 +7,16 @@ from typing import Dict, List, Mapping, Optional, Set, Tuple
 
 import torch
 
-from ..parts.base import BLOCKS, Block, CacheSpec, Embedding, Head, LayerCall, ModelPlan, Norm, Part, Runtime, TensorSpec, is_absolute
+from ..parts.base import (
+    BLOCKS, Block, CacheSpec, Embedding, FeedForward, Head, LayerCall, Mixer, ModelPlan, Norm, Part, Runtime, TensorSpec, is_absolute,
+)
 
 
 class Model:
-    def __init__(self, plan: ModelPlan) -> None:
+    def __init__(self, plan: ModelPlan, cache_bits: Optional[int] = None) -> None:
+        """`cache_bits`: 4 or 8 for keys and values cached in so many bits; a mixer that cannot refuses."""
         self.plan = plan
+        self.cache_bits = cache_bits
         self.vocab_size = plan.vocab_size
         self.dim = plan.dim
         self.blocks: List[Block] = []
@@ -22,6 +26,10 @@ class Model:
             built = {role: slot.build() for role, slot in layer.parts.items()}
             names = {role: slot.prefix for role, slot in layer.parts.items()}
             self.blocks.append(BLOCKS[layer.block](names=names, **built))
+        if cache_bits is not None:
+            for block in self.blocks:
+                for mixer in block.mixers():
+                    mixer.set_cache_bits(cache_bits)
         self.embedding: Embedding = plan.embedding.build()  # type: ignore[assignment]
         self.final_norm: Norm = plan.final_norm.build()  # type: ignore[assignment]
         self.head: Head = plan.head.build()  # type: ignore[assignment]
@@ -119,7 +127,17 @@ class Model:
                 return {prefix + name for name in part.tensor_specs()}
         raise KeyError(f"the model's own parts are embedding, final_norm and head, not {role!r}")
 
+    def _check_weight_bits(self, bits: int) -> None:
+        if bits != 8:
+            raise ValueError(f"matrices are held in 8 bits or in the activations' type, not in {bits} bits")
+        for block in self.blocks:
+            for part in getattr(block, "parts", {}).values():
+                if isinstance(part, (Mixer, FeedForward)) and not part.takes_weight_bits:
+                    raise ValueError(f"{type(part).__name__} holds its matrices in the activations' type only, not in {bits} bits")
+
     def bind(self, tensors: Mapping[str, torch.Tensor], runtime: Runtime) -> None:
+        if runtime.weight_bits is not None:
+            self._check_weight_bits(runtime.weight_bits)
         self.runtime = runtime
         for layer, block in zip(self.plan.layers, self.blocks):
             prefix = layer.prefix

@@ -25,6 +25,7 @@ from .base import (
     PartChoice,
     PartSlot,
     PositionEncoding,
+    QuantKVSpec,
     Runtime,
     StateSpec,
     TensorSpec,

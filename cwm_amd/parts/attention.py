@@ -8,7 +8,7 @@ import torch
 
 from .. import ops
 from .base import (
-    CacheSpec, ChunkedKVSpec, KeptFirstKVSpec, Mixer, PagedKVSpec, PartChoice, PositionEncoding, Runtime, StateSpec, TensorSpec, register_part,
+    CacheSpec, ChunkedKVSpec, KeptFirstKVSpec, Mixer, PagedKVSpec, QuantKVSpec, PartChoice, PositionEncoding, Runtime, StateSpec, TensorSpec, register_part,
 )
 from .linear import LinearWeights
 
@@ -27,8 +27,11 @@ class PagedAttention(Mixer):
     the output projection.  Every constant is an argument: sizes, `scale`
     (the reference fixes head_dim ** -0.5 at forward.py:651), `window` (keys read
     per query, own included; None for all), `bias` on the three input projections
-    (cwm/model/transformer.py:173-187) and the position encoding.
+    (cwm/model/transformer.py:173-187) and the position encoding.  With `cache_bits`
+    4 or 8 (`set_cache_bits`) keys and values are cached in so many bits.
     """
+
+    takes_weight_bits = True
 
     def __init__(
         self,
@@ -57,7 +60,15 @@ class PagedAttention(Mixer):
         )
 
     def cache_spec(self) -> PagedKVSpec:
+        if self.cache_bits is not None:
+            return QuantKVSpec(n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, window=self.window, bits=self.cache_bits)
         return PagedKVSpec(n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, window=self.window)
+
+    def set_cache_bits(self, bits: int) -> None:
+        why = ops.quant_cache_limits(self.head_dim, 8, bits)
+        if why is not None:
+            raise ValueError(why)
+        self.cache_bits = bits
 
     def tensor_specs(self) -> Dict[str, TensorSpec]:
         q_out = self.n_heads * self.head_dim
@@ -97,10 +108,15 @@ class PagedAttention(Mixer):
                     biases[n] = biases[n][rows]
         elif pairing != "adjacent":
             raise ValueError(f"rotary pairing {pairing!r}: 'adjacent' and 'halves' are known")
-        self.qkv = LinearWeights.joined([weights[n] for n in names], [biases[n] for n in names], stream_copy=runtime.stream_copies)
-        self.wo = LinearWeights(tensors["wo.weight"], stream_copy=runtime.stream_copies)
-        # a subclass that changes queries and keys between projection and rotation cannot use the fused product
-        self._plain_projection = type(self).transform_qk is not PagedAttention.transform_qk
+        self.qkv = LinearWeights.joined(
+            [weights[n] for n in names], [biases[n] for n in names], stream_copy=runtime.stream_copies, bits=runtime.weight_bits
+        )
+        self.wo = LinearWeights(tensors["wo.weight"], stream_copy=runtime.stream_copies, bits=runtime.weight_bits)
+        # a subclass that changes queries and keys between projection and rotation cannot use the fused product, nor can
+        # matrices or a cache of fewer bits
+        self._plain_projection = (
+            type(self).transform_qk is not PagedAttention.transform_qk or self.qkv.codes is not None or self.cache_bits is not None
+        )
 
     def transform_qk(self, q: torch.Tensor, k: Optional[torch.Tensor], batch: Any) -> None:
         """The seam between projection and rotation: a subclass may change the projected queries
@@ -140,13 +156,19 @@ class PagedAttention(Mixer):
                 k = qkv[:, q_out : q_out + kv_out].unflatten(1, (self.n_kv_heads, hd))
                 v = qkv[:, q_out + kv_out :].unflatten(1, (self.n_kv_heads, hd))
                 self.transform_qk(q, k, batch)
-                ops.rope_kv_write(q, k, v, batch.positions, table, cache.cache, cache.block_table, batch.seq_of_token)
+                if self.cache_bits is not None:
+                    ops.quant_kv_write(k, v, batch.positions, table, cache.cache, cache.block_table, batch.seq_of_token, self.cache_bits, q=q)
+                else:
+                    ops.rope_kv_write(q, k, v, batch.positions, table, cache.cache, cache.block_table, batch.seq_of_token)
             else:
                 # reads a cache that another layer wrote in this step: only the queries are needed
                 self.transform_qk(q, None, batch)
                 if table is not None:
                     ops.rope_kv_write(q, None, None, batch.positions, table)
-        attn = ops.paged_attention(q, cache.cache, cache.block_table, batch, self.window, self.scale)
+        if self.cache_bits is not None:
+            attn = ops.quant_paged_attention(q, cache.cache, cache.block_table, batch, self.window, self.scale, self.cache_bits)
+        else:
+            attn = ops.paged_attention(q, cache.cache, cache.block_table, batch, self.window, self.scale)
         return self.wo(attn, partials_ok=True)  # added into the residual by the next norm
 
 

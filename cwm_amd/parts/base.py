@@ -27,6 +27,8 @@ from typing import Any, Callable, Dict, Hashable, List, Mapping, Optional, Tuple
 
 import torch
 
+from .. import ops
+
 
 # --------------------------------------------------------------------------- #
 # tensors a part needs
@@ -110,6 +112,30 @@ class PagedKVSpec:
             count *= n
         return count * element_size
 
+    def element_type(self, act_dtype: torch.dtype) -> torch.dtype:
+        """Type of the storage's elements in a model whose activations are of `act_dtype`."""
+        return act_dtype
+
+
+@dataclass(frozen=True)
+class QuantKVSpec(PagedKVSpec):
+    """Keys and values in pages of 4 or 8 bits a value (`ops.quant_kv_write`); the pages are bytes."""
+
+    bits: int = 8
+
+    def page_shape(self, page_size: int) -> Tuple[int, ...]:
+        why = ops.quant_cache_limits(self.head_dim, page_size, self.bits)
+        if why is not None:
+            raise ValueError(why)
+        return ops.quant_page_shape(self.n_kv_heads, self.head_dim, page_size, self.bits)
+
+    def bytes_per_token(self, element_size: int) -> int:
+        heads, size = ops.quant_page_shape(self.n_kv_heads, self.head_dim, 1, self.bits)
+        return heads * size
+
+    def element_type(self, act_dtype: torch.dtype) -> torch.dtype:
+        return torch.uint8
+
 
 @dataclass(frozen=True)
 class ChunkedKVSpec(PagedKVSpec):
@@ -176,6 +202,9 @@ class Runtime:
     # for the weight-streaming product of a decode step (`ops.stream_layout`): twice the memory for the matrices,
     # about a tenth less time to stream them.  Whoever loads the model decides, from the memory there is.
     stream_copies: bool = False
+    # 8: the matrices of the layers are held as 8-bit integers with a scale an output channel, and their products quantise
+    # the activations row by row (`ops.linear_int8`); None: in the activations' type
+    weight_bits: Optional[int] = None
 
 
 class Part:
@@ -187,6 +216,9 @@ class Part:
     # nothing goes between host and device in it.  A part that does not say so keeps its model on the path
     # that launches every step kernel by kernel.
     replayable = False
+    # Whether the part holds its matrices in `Runtime.weight_bits`; a model is refused other than that by its first mixer
+    # or feed-forward that does not.
+    takes_weight_bits = False
 
     def tensor_specs(self) -> Dict[str, TensorSpec]:
         return {}
@@ -232,8 +264,16 @@ class Mixer(Part):
     """A mixer that needs several caches or states (several mixers side by side; pages and a state beside them) lists one
     mixer a need as `children()`; its `forward` then gets a tuple of views in that order."""
 
+    cache_bits: Optional[int] = None  # 4 or 8: keys and values are cached in so many bits
+
     def cache_spec(self) -> CacheSpec:
         return None
+
+    def set_cache_bits(self, bits: int) -> None:
+        """Cache keys and values in 4 or 8 bits (before `cache_spec` is asked).  A mixer that keeps none ignores it; one whose
+        kernels read them in the activations' type only refuses."""
+        if isinstance(self.cache_spec(), PagedKVSpec):
+            raise ValueError(f"{type(self).__name__} caches keys and values in the activations' type only, not in {bits} bits")
 
     def forward(self, x: torch.Tensor, batch: Any, cache: Any, write_cache: bool = True) -> torch.Tensor:
         """x: normalised activations [T, D] -> [T, D] to be added to the residual (or

@@ -18,6 +18,7 @@ class SwiGLU(FeedForward):
     rounded once."""
 
     replayable = True
+    takes_weight_bits = True
 
     def __init__(self, dim: int, hidden_dim: int) -> None:
         self.dim = dim
@@ -37,14 +38,16 @@ class SwiGLU(FeedForward):
         self.grouped = self.hidden_dim % 8 == 0
         self.gate_up = LinearWeights.joined(
             [tensors["w1.weight"], tensors["w3.weight"]], [None, None], group=8 if self.grouped else None,
-            stream_copy=runtime.stream_copies,
+            stream_copy=runtime.stream_copies, bits=runtime.weight_bits,
         )
-        self.down = LinearWeights(tensors["w2.weight"], stream_copy=runtime.stream_copies)
+        self.down = LinearWeights(tensors["w2.weight"], stream_copy=runtime.stream_copies, bits=runtime.weight_bits)
 
     def forward(self, x: torch.Tensor, batch: Any) -> torch.Tensor:
         # the result (or partial sums of it) is added into the residual by the next norm.  (Forming
         # silu(gate) * up inside the down product was tried: every block recomputes it, which costs
         # more than the kernel it saves.)
+        if self.gate_up.codes is not None:
+            return self.down(ops.silu_mul(self.gate_up(x), grouped=self.grouped), partials_ok=True)
         hidden = ops.gate_up_silu(x, self.gate_up.weight, self.gate_up.bias, self.grouped, streamed=self.gate_up.streamed)
         return self.down(hidden, partials_ok=True)
 

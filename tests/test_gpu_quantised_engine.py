@@ -1,0 +1,151 @@
+"""Models with a cache in 4 or 8 bits and matrices in 8, through the engine: against the plain decoder with the same values
+held, over steps cut anywhere, replayed as graphs, preempted, and from the command line."""
+
+import json
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from cwm_amd import ops
+from cwm_amd.cache import CacheManager, CacheStorage
+from cwm_amd.engine import Engine, GenArgs, ModelRunner, Portion, load_model
+from helpers import configs, models, quantised as held, traces
+from plain import llama3_plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _held(x, bits):
+    """What a cache of float32 keys (groups of 32) or values (whole heads) holds of them."""
+    x = x.float()
+    return held.stands_for(*held.hold(x, bits), bits)
+
+
+def _plain(monkeypatch, folder, tokens, cache_bits, weight_bits):
+    """The plain decoder's float64 logits with keys and values, matrices and their inputs replaced by what is held of them."""
+    attention, linear = llama3_plain.attention, llama3_plain.linear
+
+    def quantised_attention(q, k, v, **kw):
+        n, heads, dim = k.shape
+        k, v = _held(k.reshape(n, heads, dim // 32, 32), cache_bits).reshape(n, heads, dim), _held(v, cache_bits)
+        return attention(q, k, v, **kw)
+
+    def rows(x):
+        x = x.float()
+        a = x.abs().amax(1, keepdim=True) / torch.full((x.shape[0], 1), 127.0)
+        return torch.where(a > 0, torch.round(x / a), torch.zeros_like(x)).double() * a.double()
+
+    def quantised_linear(x, weight, bias=None):
+        return linear(rows(x), rows(weight), bias)
+
+    def quantised_swiglu(x, w1, w2, w3, rounding=None):
+        gate, up = rows(x) @ rows(w1).T, rows(x) @ rows(w3).T
+        return rows(gate * torch.sigmoid(gate) * up) @ rows(w2).T
+
+    with monkeypatch.context() as m:
+        if cache_bits:
+            m.setattr(llama3_plain, "attention", quantised_attention)
+        if weight_bits:
+            config, weights = models.read_folder(folder)
+            head = weights["output.weight"].double()
+            m.setattr(llama3_plain, "linear", lambda x, w, bias=None: linear(x, w, bias) if w.shape == head.shape and torch.equal(w, head) else quantised_linear(x, w, bias))
+            m.setattr(llama3_plain, "swiglu", quantised_swiglu)
+        return models.plain_logits(folder, {"a": tokens})["a"]
+
+
+def _logits(model, tokens, cuts, page=16, graphs=0):
+    manager = CacheManager(model.cache_specs, page, -(-len(tokens) // page) + 2, 2)
+    runner = ModelRunner(model, manager, CacheStorage(manager, model.runtime.device, model.runtime.act_dtype), num_graphs=graphs)
+    runner.on_pages_freed = lambda group, pages: runner.storage.fill_pages(group, pages, float("nan"))
+    runner.admit("a")
+    out, at = [], 0
+    for n in cuts:
+        assert manager.extend("a", n)
+        out.append(runner.step([Portion("a", tokens[at : at + n], list(range(n)))]).float().cpu())
+        at += n
+    return torch.cat(out), runner
+
+
+def _cuts(total, sizes):
+    cuts = []
+    while sum(cuts) < total:
+        cuts.append(min(sizes[len(cuts) % len(sizes)], total - sum(cuts)))
+    return cuts
+
+
+@pytest.mark.parametrize("cache_bits,weight_bits", [(4, None), (8, None), (None, 8), (4, 8)])
+@pytest.mark.parametrize("name", ["tiny_b", "tiny_d"])
+def test_logits_are_those_of_the_held_values(tmp_path, monkeypatch, name, cache_bits, weight_bits):
+    """float32: the engine is off the plain decoder with the same values held by a small part of what holding them changes.
+
+    A sum in another order can tip a value next to a border to the neighbouring code.  The cache: of some ten thousand codes each
+    moves the logits by about a hundredth of what all their roundings do, and about one in a hundred thousand is so near.
+    Activations in 8 bits: 608 codes a token and layer, a value of up to 127 steps off by 1e-6 of itself, so one code in ten
+    thousand tips, some ten of a request's 146,000; and a row that has one tipped code differs by a good part of a step wherever
+    it is quantised next, so its later codes are a new draw of the rounding.  Two draws of the activations' rounding
+    differ by sqrt(2) of one, which with the weights' (the same in both) makes up what is changed: off^2 <= 2 changed^2."""
+    folder = models.make_folder(tmp_path, name, seed=3, dtype="float32")
+    tokens = traces.random_tokens(5, 60, configs.get(name)["vocab_size"])
+    model, _ = load_model(folder, "float32", DEV, cache_bits=cache_bits, weight_bits=weight_bits)
+    full = torch.from_numpy(models.plain_logits(folder, {"a": tokens})["a"]).double()
+    want = torch.from_numpy(_plain(monkeypatch, folder, tokens, cache_bits, weight_bits)).double()
+    changed = float((want - full).norm())
+    assert changed > 0
+    for sizes in ([60], [1], [7, 1, 20]):
+        got, _ = _logits(model, tokens, _cuts(60, sizes))
+        off = float((got.double() - want).norm())
+        limit = 0.05 * changed + 3e-5 * float(want.norm()) if weight_bits is None else 2 ** 0.5 * changed
+        assert off <= limit, (sizes, off, changed)
+
+
+@pytest.mark.parametrize("cache_bits,weight_bits", [(4, None), (8, 8)])
+def test_bfloat16_steps_and_their_graphs(tmp_path, cache_bits, weight_bits):
+    """bfloat16: decode steps replayed as graphs have the bits of the launched ones, over cuts of the cache and of the window."""
+    folder = models.make_folder(tmp_path, "tiny_d", seed=4, dtype="bfloat16")
+    tokens = traces.random_tokens(6, 150, configs.get("tiny_d")["vocab_size"])
+    model, _ = load_model(folder, "bfloat16", DEV, cache_bits=cache_bits, weight_bits=weight_bits)
+    cuts = [70] + [1] * 80
+    want, _ = _logits(model, tokens, cuts)
+    got, runner = _logits(model, tokens, cuts, graphs=2)
+    assert runner.n_replays > 50 and torch.isfinite(got).all() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("cache_bits,weight_bits", [(4, 8), (8, None)])
+def test_generation_with_preemption(tmp_path, cache_bits, weight_bits):
+    """Greedy tokens of a cache that holds barely more than one sequence are those of a roomy one."""
+    folder = models.make_folder(tmp_path, "tiny_b", seed=8, dtype="float32")
+    prompts = [traces.random_tokens(i, n, 509) for i, n in enumerate([5, 17, 33, 64])]
+    more = dict(use_sampling=False, max_batch=4, max_prefill=48, cache_bits=cache_bits, weight_bits=weight_bits)
+    engine = Engine.from_folder(folder, GenArgs(max_seq=2048, cache_block=16, **more), dtype="float32")
+    assert all(t.dtype == torch.uint8 for t in engine.storage.paged.values())
+    got = engine.generate_tokens(prompts, max_gen=16)
+    small = Engine.from_folder(folder, GenArgs(max_seq=96, cache_block=8, **more), dtype="float32")
+    again = small.generate_tokens(prompts, max_gen=16)
+    assert any(e.startswith("preempt") for e in small.scheduler.events)
+    assert again == got and all(len(t) == 16 for t in got)
+
+
+def test_a_cache_of_fewer_bits_is_smaller(tmp_path):
+    folder = models.make_folder(tmp_path, "tiny_d", seed=8, dtype="bfloat16")
+    sizes = {}
+    for bits in (None, 8, 4):
+        engine = Engine.from_folder(folder, GenArgs(max_batch=2, max_seq=1024, cache_block=64, cache_bits=bits), dtype="bfloat16")
+        sizes[bits] = engine.storage.bytes()
+    # heads of 64: 256 bytes a token in bfloat16, 128 + 12 and 64 + 12 in codes and words
+    assert sizes[8] * 256 == sizes[None] * 140 and sizes[4] * 256 == sizes[None] * 76
+
+
+def test_the_command_line_takes_the_options(tmp_path):
+    folder = models.make_folder(tmp_path, "tiny_b", seed=8, dtype="bfloat16")
+    out = os.path.join(str(tmp_path), "out.jsonl")
+    cmd = [sys.executable, "-m", "cwm_amd.generate", f"checkpoint_dir={folder}", "prompt=[1,2,3,4,5]", f"out={out}", "gen_args.max_gen=6", "gen_args.max_seq=256",
+           "gen_args.max_batch=2", "gen_args.cache_block=32", "gen_args.cache_bits=4", "gen_args.weight_bits=8"]
+    done = subprocess.run(cmd, cwd=ROOT, capture_output=True, text=True, timeout=110)
+    assert done.returncode == 0, done.stderr[-2000:]
+    with open(out) as fh:
+        assert len(json.loads(fh.readline())["tokens"]) == 6
