@@ -27,12 +27,13 @@ __device__ __forceinline__ int int8_of(float x, float a) {
   return (int)rintf(x / a);  // a true quotient: ties are common among short numbers, and a product with 1 / a would decide them otherwise
 }
 
-// One block a row: the largest magnitude, then the integers, zeros from K to Kp.  A row with a NaN or an infinity in it has a
-// NaN for its scale (and zeros for its integers).
+// One block a row: the largest magnitude, then the integers in a row of Kp.  Zeros fill it up, from K on, or (`shift`, Kp - K) ahead of
+// the integers from the last multiple of 128 on, which then end with the row.  A row with a NaN or an infinity in it has a NaN
+// for its scale (and zeros for its integers).
 template <typename T>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T* __restrict__ x, long x_stride, int8_t* __restrict__ codes, long c_stride, float* __restrict__ scale, int K, int Kp,
-                     bool aligned) {
+                     int shift, bool aligned) {
   __shared__ float scratch[16];
   const T* row = x + (size_t)blockIdx.x * x_stride;
   int8_t* out = codes + (size_t)blockIdx.x * c_stride;
@@ -53,92 +54,206 @@ quantize_rows_kernel(const T* __restrict__ x, long x_stride, int8_t* __restrict_
   const float a = most / 127.f;
   if (threadIdx.x == 0) scale[blockIdx.x] = finite ? a : __uint_as_float(0x7fc00000u);
   const bool none = !finite || a == 0.f;
+  const int tail = shift > 0 ? K / 128 * 128 : Kp;  // where the integers move on by `shift`
   if (aligned) {
-    for (int k = 4 * threadIdx.x; k < Kp; k += 1024) {
+    for (int at = 4 * threadIdx.x; at < Kp; at += 1024) {
+      const int k = at >= tail ? at - shift : at;
       uint32_t w = 0;
-      if (k < K && !none) {
+      if (k < K && (at < tail || k >= tail) && !none) {
         float v[4];
         load4(row + k, v);
 #pragma unroll
         for (int e = 0; e < 4; ++e) w |= ((uint32_t)int8_of(v[e], a) & 255u) << (8 * e);
       }
-      *(uint32_t*)(out + k) = w;
+      *(uint32_t*)(out + at) = w;
     }
   } else {
-    for (int k = threadIdx.x; k < Kp; k += 256) out[k] = k < K && !none ? (int8_t)int8_of(Elem<T>::load(row + k), a) : 0;
+    for (int at = threadIdx.x; at < Kp; at += 256) {
+      const int k = at >= tail ? at - shift : at;
+      out[at] = k < K && (at < tail || k >= tail) && !none ? (int8_t)int8_of(Elem<T>::load(row + k), a) : 0;
+    }
   }
 }
 
-extern "C" int cwm_quantize_rows(const void* x, long x_stride, int dtype, void* codes, long c_stride, float* scale, int M, int K, int Kp,
-                                 hipStream_t stream) {
+static int quantize_rows(const void* x, long x_stride, int dtype, void* codes, long c_stride, float* scale, int M, int K, int Kp, int shift,
+                         hipStream_t stream) {
   CWM_REQUIRE(M >= 0 && K > 0 && Kp >= K && c_stride >= Kp, "quantize_rows: bad sizes M=%d K=%d padded %d", M, K, Kp);
   if (M == 0) return 0;
   CWM_REQUIRE(x && codes && scale, "quantize_rows: a tensor is missing");
   const int size = dtype == CWM_BF16 ? 2 : 4;
   const bool aligned = K % 4 == 0 && Kp % 4 == 0 && x_stride % 4 == 0 && c_stride % 4 == 0 && (uintptr_t)x % (4 * size) == 0 && (uintptr_t)codes % 4 == 0;
   if (dtype == CWM_BF16)
-    hipLaunchKernelGGL(quantize_rows_kernel<bf16_t>, dim3(M), dim3(256), 0, stream, (const bf16_t*)x, x_stride, (int8_t*)codes, c_stride, scale, K, Kp, aligned);
+    hipLaunchKernelGGL(quantize_rows_kernel<bf16_t>, dim3(M), dim3(256), 0, stream, (const bf16_t*)x, x_stride, (int8_t*)codes, c_stride, scale, K, Kp, shift, aligned);
   else
-    hipLaunchKernelGGL(quantize_rows_kernel<float>, dim3(M), dim3(256), 0, stream, (const float*)x, x_stride, (int8_t*)codes, c_stride, scale, K, Kp, aligned);
+    hipLaunchKernelGGL(quantize_rows_kernel<float>, dim3(M), dim3(256), 0, stream, (const float*)x, x_stride, (int8_t*)codes, c_stride, scale, K, Kp, shift, aligned);
   return cwm_launch_status("quantize_rows");
+}
+
+extern "C" int cwm_quantize_rows(const void* x, long x_stride, int dtype, void* codes, long c_stride, float* scale, int M, int K, int Kp,
+                                 hipStream_t stream) {
+  return quantize_rows(x, x_stride, dtype, codes, c_stride, scale, M, K, Kp, 0, stream);
 }
 
 // ---- few rows ------------------------------------------------------------------------------- //
 // A block has 16 rows of W and up to 16 RT rows of X; its wavefronts take pieces of 128 columns in turn, lane 16 j + r the bytes
 // 32 j .. 32 j + 31 of row r, which are two operands of the matrix instruction (the columns of a product may come in any order
-// that both operands keep): a wavefront's load of W is 16 whole cache lines.  X is read from the caches.
-#define FEW_WAVES 4
+// that both operands keep): a wavefront's load of W is 16 whole cache lines.  AHEAD pieces of a wavefront are in flight at a time,
+// where K allows all of them: what the reading takes is then its latency once and the memory's rate.
+// X comes from the caches, or (FUSED, up to FUSED_ROWS rows) every block makes the integers of x itself, in LDS, while its first
+// pieces of W are under way: a second launch would cost more than the few thousand quotients.
+#define FEW_WAVES 8
+#define FUSED_ROWS 4
+#define FUSED_SLOTS 8  // a thread's pieces of four values of x: eight of one row, four of each of two, two of each of four
+#define FUSED_SLOT (4 * 64 * FEW_WAVES)
 
-template <typename T, int RT>
+// FUSED: the number of rows of x that a block has room for (1, 2 or 4), or 0.
+template <typename TX, typename T, int RT, int FUSED, int AHEAD>
 __global__ void __launch_bounds__(64 * FEW_WAVES)
-gemm_int8_few_kernel(const int8_t* __restrict__ X, long ldx, const float* __restrict__ a, const int8_t* __restrict__ W, long ldw,
-                     const float* __restrict__ w_scale, const float* __restrict__ bias, T* __restrict__ y, long ldy, int M, int N, int K) {
-  __shared__ __attribute__((aligned(16))) int4v sums[FEW_WAVES][RT][64];
+gemm_int8_few_kernel(const int8_t* __restrict__ X, long ldx, const float* __restrict__ a, const TX* __restrict__ x, long x_stride, bool x_aligned,
+                     const int8_t* __restrict__ W, long ldw, const float* __restrict__ w_scale, const float* __restrict__ bias, T* __restrict__ y,
+                     long ldy, int M, int N, int K, int rows_a_block) {
+  extern __shared__ __attribute__((aligned(16))) int8_t codes[];  // FUSED: [M][Kp]
+  __shared__ __attribute__((aligned(16))) int4v sums[2][FEW_WAVES][RT][64];
+  __shared__ float tops[FEW_WAVES][FUSED_ROWS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, j = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * RT;
-  const int8_t* w_row = W + (size_t)min(n0 + r, N - 1) * ldw + 32 * j;
+  const int m0 = blockIdx.y * 16 * RT;
+  const int steps = (K + 127) / 128, Kp = 128 * steps;
+  const int whole = K / 128;  // pieces that W holds whole
+  const int rounds = (whole + FEW_WAVES * AHEAD - 1) / (FEW_WAVES * AHEAD);
+  typedef const int4v* pieces;
+  const int4v zero = (int4v){0, 0, 0, 0};
+  int4v w[AHEAD][2];
+  const int n_begin = blockIdx.x * rows_a_block, n_end = min(n_begin + rows_a_block, N);
+  // lanes past the block's last row read that one again, which costs no memory
+  auto row_of = [&](int n0) { return W + (size_t)min(n0 + r, n_end - 1) * ldw + 32 * j; };
+  auto load_w = [&](int n0, int round) {  // no branch around a load: past the last piece that one again, which is not multiplied
+    const int8_t* row = row_of(n0);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[u][h] = __builtin_nontemporal_load((pieces)(row + 128 * min(wave + FEW_WAVES * (round * AHEAD + u), whole - 1) + 16 * h));
+  };
+  float scale_row[FUSED > 0 ? FUSED : 1];
+
+  if constexpr (FUSED > 0) {
+    // The rows of x, loaded ahead of W: loads return in order, so behind W's they would wait for the whole of it.
+    constexpr int A_ROW = FUSED_SLOTS / FUSED;
+    float v[FUSED_SLOTS][4];
+#pragma unroll
+    for (int i = 0; i < FUSED_SLOTS; ++i) {
+      const int m = i / A_ROW, k = i % A_ROW * FUSED_SLOT + 4 * threadIdx.x;
+      const bool have = m < M && k < K;  // K is a multiple of 16
+      const TX* p = x + (have ? (size_t)m * x_stride + k : 0);
+      if (x_aligned) {
+        load4(p, v[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = Elem<TX>::load(p + (have ? e : 0));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] = have ? v[i][e] : 0.f;
+    }
+    if (rounds > 0) load_w(n_begin, 0);
+#pragma unroll
+    for (int m = 0; m < FUSED; ++m) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < A_ROW; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v[m * A_ROW + i][e]) & 0x7fffffffu);
+      const float most = wave_max(top >= 0x7f800000u ? __builtin_inff() : __uint_as_float(top));
+      if (lane == 0) tops[wave][m] = most;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < FUSED; ++m) {
+      float most = tops[0][m];
+#pragma unroll
+      for (int u = 1; u < FEW_WAVES; ++u) most = fmaxf(most, tops[u][m]);
+      scale_row[m] = most == __builtin_inff() ? __uint_as_float(0x7fc00000u) : most / 127.f;
+    }
+#pragma unroll
+    for (int i = 0; i < FUSED_SLOTS; ++i) {
+      const int m = i / A_ROW, k = i % A_ROW * FUSED_SLOT + 4 * threadIdx.x;
+      if (m >= M || k >= Kp) continue;
+      uint32_t c = 0;
+      if (scale_row[m] > 0.f) {  // not of a row of zeros, nor where it is a NaN
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c |= ((uint32_t)int8_of(v[i][e], scale_row[m]) & 255u) << (8 * e);
+      }
+      *(uint32_t*)(codes + (size_t)m * Kp + k) = c;
+    }
+    __syncthreads();
+  } else {
+    if (rounds > 0) load_w(n_begin, 0);
+  }
+
   const int8_t* x_row[RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) x_row[rt] = X + (size_t)min(m0 + 16 * rt + r, M - 1) * ldx + 32 * j;
-  int4v acc[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) acc[rt] = (int4v){0, 0, 0, 0};
-  const int4v none = (int4v){0, 0, 0, 0};
-  // X holds zeros from K to the next multiple of 128, W ends at K: a piece of 16 columns lies before or past it as a whole
-  auto piece = [&](int k, int4v (&w)[2], int4v (&x)[RT][2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      w[h] = k + 32 * j + 16 * h < K ? __builtin_nontemporal_load((const int4v*)(w_row + k + 16 * h)) : none;
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) x[rt][h] = *(const int4v*)(x_row[rt] + k + 16 * h);
-    }
-  };
-  const int steps = (K + 127) / 128;
-#pragma unroll 4
-  for (int s = wave; s < steps; s += FEW_WAVES) {
-    int4v w[2], x[RT][2];
-    piece(128 * s, w, x);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) acc[rt] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[h], x[rt][h], acc[rt], 0, 0, 0);
+  for (int rt = 0; rt < RT; ++rt) {
+    if constexpr (FUSED > 0)
+      x_row[rt] = codes + (size_t)min(r, M - 1) * Kp + 32 * j;
+    else
+      x_row[rt] = X + (size_t)min(m0 + 16 * rt + r, M - 1) * ldx + 32 * j;
   }
+  for (int n0 = n_begin, buffer = 0; n0 < n_end; n0 += 16, buffer ^= 1) {
+    int4v acc[RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) sums[wave][rt][lane] = acc[rt];
-  __syncthreads();
-  // lane 16 j + r holds the sums of row r of X and the columns 4 j .. 4 j + 3
-  for (int rt = wave; rt < RT; rt += FEW_WAVES) {
-    int4v sum = sums[0][rt][lane];
+    for (int rt = 0; rt < RT; ++rt) acc[rt] = zero;
+    for (int round = 0; round < rounds; ++round) {
+      int4v xp[AHEAD][RT][2];
 #pragma unroll
-    for (int v = 1; v < FEW_WAVES; ++v) sum += sums[v][rt][lane];
-    const int m = m0 + 16 * rt + r;
-    if (m >= M) continue;
-    const float am = a[m];
+      for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int n = n0 + 4 * j + e;
-      if (n < N) Elem<T>::store(y + (size_t)m * ldy + n, (float)sum[e] * am * w_scale[n] + (bias ? bias[n] : 0.f));
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) xp[u][rt][h] = *(pieces)(x_row[rt] + 128 * min(wave + FEW_WAVES * (round * AHEAD + u), whole - 1) + 16 * h);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int4v wp = wave + FEW_WAVES * (round * AHEAD + u) < whole ? w[u][h] : zero;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) acc[rt] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wp, xp[u][rt][h], acc[rt], 0, 0, 0);
+        }
+      // the block's next loads are under way before its sums are joined
+      const bool more = round + 1 < rounds;
+      if (more || n0 + 16 < n_end) load_w(more ? n0 : n0 + 16, more ? round + 1 : 0);
+    }
+    // K's end: X holds zeros up to a multiple of 128, W ends at K, a multiple of 16
+    if (whole < steps && wave == whole % FEW_WAVES) {
+      const int8_t* row = row_of(n0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int4v wp = 128 * whole + 32 * j + 16 * h < K ? *(pieces)(row + 128 * whole + 16 * h) : zero;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wp, *(pieces)(x_row[rt] + 128 * whole + 16 * h), acc[rt], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) sums[buffer][wave][rt][lane] = acc[rt];
+    __syncthreads();  // two buffers: what is written next is read two barriers on
+    // lane 16 j + r holds the sums of row r of X and the columns 4 j .. 4 j + 3
+    for (int rt = wave; rt < RT; rt += FEW_WAVES) {
+      int4v sum = sums[buffer][0][rt][lane];
+#pragma unroll
+      for (int v = 1; v < FEW_WAVES; ++v) sum += sums[buffer][v][rt][lane];
+      const int m = m0 + 16 * rt + r;
+      if (m >= M) continue;
+      float am = 0.f;
+      if constexpr (FUSED > 0) {
+#pragma unroll
+        for (int u = 0; u < FUSED; ++u) am = r == u ? scale_row[u] : am;
+      } else {
+        am = a[m];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = n0 + 4 * j + e;
+        if (n < n_end) Elem<T>::store(y + (size_t)m * ldy + n, (float)sum[e] * am * w_scale[n] + (bias ? bias[n] : 0.f));
+      }
     }
   }
 }
@@ -160,7 +275,7 @@ template <int WM, int WN>
 struct Int8Source {
   const bf16_t *A, *W;
   long lda, ldw;  // in pairs of bytes
-  int M, N, lane, wave;
+  int M, N, w_last, lane, wave;
   Int8Order order;
   const bf16_t *a, *w;
   uint32_t off[WideShape<WM, WN>::ND];
@@ -194,7 +309,7 @@ struct Int8Sink {
   int M, N, lane, wave;
   bool vector;
   Int8Order order;
-  static constexpr int STORES = 0;  // its loads and stores are waited for before the next tile's are counted
+  static constexpr int STORES = sizeof(T) == 4 ? WM * WN : WM * WN / 2;
 
   __device__ __forceinline__ bool store(int tile, int4v (&acc)[WM][WN]) const {
     constexpr int BM = WideShape<WM, WN>::BM, BN = WideShape<WM, WN>::BN;
@@ -203,7 +318,9 @@ struct Int8Sink {
     const int r = lane & 15, j = lane >> 4, wm = wave >> 2, wn = wave & 3;
     const int m0 = tm * BM + wm * WM * 16 + r;
     const int n0 = tn * BN + wn * WN * 16 + 4 * WN * j;
-    float ws[WN][4], bs[WN][4];
+    float am[WM], ws[WN][4], bs[WN][4];
+#pragma unroll
+    for (int i = 0; i < WM; ++i) am[i] = a[min(m0 + 16 * i, M - 1)];
 #pragma unroll
     for (int b = 0; b < WN; ++b)
 #pragma unroll
@@ -212,38 +329,46 @@ struct Int8Sink {
         ws[b][e] = w_scale[n];
         bs[b][e] = bias ? bias[n] : 0.f;
       }
+    // Waited for here, by an instruction that the compiler knows of: loads that it takes to be under way at the loop's head
+    // make it wait for all of the loop's own loads in every step (2,048 x 43,008 x 6,144 663 us, 1.24 us a step).
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    const bool full = vector && (tm + 1) * BM <= M && (tn + 1) * BN <= N;
 #pragma unroll
     for (int i = 0; i < WM; ++i) {
       const int m = m0 + 16 * i;
       if (m >= M) continue;
-      const float am = a[m];
       T* row = C + (size_t)m * ldc + n0;
+      float v[WN][4];
 #pragma unroll
-      for (int b = 0; b < WN; ++b) {
-        float v[4];
+      for (int b = 0; b < WN; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][b][e] * am * ws[b][e] + bs[b][e];
-        if (vector && n0 + 4 * b + 3 < N) {
-          if constexpr (sizeof(T) == 4)
-            *(float4*)(row + 4 * b) = make_float4(v[0], v[1], v[2], v[3]);
-          else
-            *(uint2*)(row + 4 * b) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+        for (int e = 0; e < 4; ++e) v[b][e] = (float)acc[i][b][e] * am[i] * ws[b][e] + bs[b][e];
+#pragma unroll
+      for (int b = 0; b < WN; b += 2) {
+        if (vector && n0 + 4 * b + 7 < N) {
+          if constexpr (sizeof(T) == 4) {
+            *(float4*)(row + 4 * b) = make_float4(v[b][0], v[b][1], v[b][2], v[b][3]);
+            *(float4*)(row + 4 * b + 4) = make_float4(v[b + 1][0], v[b + 1][1], v[b + 1][2], v[b + 1][3]);
+          } else {
+            *(uint4*)(row + 4 * b) = make_uint4(pack2_bf16(v[b][0], v[b][1]), pack2_bf16(v[b][2], v[b][3]), pack2_bf16(v[b + 1][0], v[b + 1][1]),
+                                                pack2_bf16(v[b + 1][2], v[b + 1][3]));
+          }
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n0 + 4 * b + e < N) Elem<T>::store(row + 4 * b + e, v[e]);
+          for (int e = 0; e < 8; ++e)
+            if (n0 + 4 * b + e < N) Elem<T>::store(row + 4 * b + e, v[b + e / 4][e % 4]);
         }
       }
     }
-    return false;
+    return full;
   }
 };
 
-template <int WM, int WN, typename T>
+template <int WM, int WN, typename T, bool ONCE>
 __global__ void __launch_bounds__(512, 2)
 gemm_int8_wide_kernel(const int8_t* __restrict__ X, long ldx, const float* __restrict__ a, const int8_t* __restrict__ W, long ldw,
                       const float* __restrict__ w_scale, const float* __restrict__ bias, T* __restrict__ y, long ldy, bool vector, int M, int N,
-                      int steps, int m_tiles, int n_tiles) {
+                      int K, int m_tiles, int n_tiles) {
   typedef WideShape<WM, WN> Shape;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[Shape::S * Shape::STAGE];
   const int lane = threadIdx.x & 63;
@@ -256,60 +381,119 @@ gemm_int8_wide_kernel(const int8_t* __restrict__ X, long ldx, const float* __res
   const int first = xcd * per + min(xcd, rest), count = per + (xcd < rest ? 1 : 0);
   const int mine = (count - idx + blocks - 1) / blocks;
   const Int8Order order = {m_tiles, n_tiles};
-  Int8Source<WM, WN> src = {(const bf16_t*)X, (const bf16_t*)W, ldx / 2, ldw / 2, M, N, lane, wave, order};
+  Int8Source<WM, WN> src = {(const bf16_t*)X, (const bf16_t*)W, ldx / 2, ldw / 2, M, N, (K - 128) / 2, lane, wave, order};
   Int8Sink<WM, WN, T> sink = {y, ldy, a, w_scale, bias, M, N, lane, wave, vector, order};
-  wide_loop<WM, WN, Int8Sink<WM, WN, T>::STORES, WideInt8>(lds, src, sink, first + idx, blocks, mine, steps);
+  wide_loop<WM, WN, Int8Sink<WM, WN, T>::STORES, WideInt8<ONCE>>(lds, src, sink, first + idx, blocks, mine, (K + 127) / 128);
 }
 
-// X [M][ldx] int8 with zeros from K to the next multiple of 128 within ldx, a float32 [M]; W [N][ldw] int8; y of `dtype`.
-// `tile`: 0 few rows; 1 to 4 the tiles of many rows (256 x 128, 128 x 256, 64 x 128, 128 x 128), which need K % 128 == 0.
-extern "C" int cwm_gemm_int8(const void* X, long ldx, const float* a, const void* W, long ldw, const float* w_scale, const float* bias, void* y,
-                             int dtype, long ldy, int M, int N, int K, int units, int tile, hipStream_t stream) {
-  CWM_REQUIRE(M >= 0 && N > 0 && K > 0 && K % 16 == 0 && K <= INT8_MAX_K && units > 0, "gemm_int8: bad sizes M=%d N=%d K=%d units=%d", M, N, K, units);
+// y = x W^T (+ bias): x [M][x_stride] of x_dtype; W int8 [N][ldw] with its float32 scales [N]; y of y_dtype.  `codes`, `a`: room
+// for the integers of x, [M][K rounded up to 128] bytes, and their scales, M floats (neither with tile -1).
+// `tile`: -1 few rows whose integers every block makes itself (M <= 4); 0 few rows; 1 to 4 the tiles of many rows (256 x 128,
+// 128 x 256, 64 x 128, 128 x 128), which need a K of 128 at least.
+extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* codes, float* a, const void* W, long ldw, const float* w_scale,
+                               const float* bias, void* y, int dtype, long ldy, int M, int N, int K, int units, int tile, hipStream_t stream) {
+  CWM_REQUIRE(M >= 0 && N > 0 && K > 0 && K % 16 == 0 && K <= INT8_MAX_K && units > 0, "linear_int8: bad sizes M=%d N=%d K=%d units=%d", M, N, K, units);
   if (M == 0) return 0;
-  CWM_REQUIRE(X && a && W && w_scale && y, "gemm_int8: a tensor is missing");
-  CWM_REQUIRE(ldx % 16 == 0 && ldw % 16 == 0 && (uintptr_t)X % 16 == 0 && (uintptr_t)W % 16 == 0, "gemm_int8: rows must be 16-byte aligned");
-  CWM_REQUIRE(ldx >= (K + 127) / 128 * 128 && ldw >= K && ldy >= N, "gemm_int8: row strides shorter than rows");
+  CWM_REQUIRE(x && W && w_scale && y, "linear_int8: a tensor is missing");
+  CWM_REQUIRE(ldw % 16 == 0 && (uintptr_t)W % 16 == 0, "linear_int8: the weight's rows must be 16-byte aligned");
+  CWM_REQUIRE(ldw >= K && ldy >= N, "linear_int8: row strides shorter than rows");
+  const int x_size = x_dtype == CWM_BF16 ? 2 : 4, Kp = (K + 127) / 128 * 128;
+  const int a_wave = (K / 128 + FEW_WAVES - 1) / FEW_WAVES;  // pieces of a wavefront of few rows
+  // Two blocks a compute unit stay, each with the same number of rows of W: what one unit can have in flight is limited, so with
+  // tiles dealt out one by one the units that get one more take that much longer (6,144 rows: 384 tiles 12.7 us, 512 blocks of 12
+  // rows 9).
+  const int few_rows = (N + 2 * units - 1) / (2 * units) > 4 ? (N + 2 * units - 1) / (2 * units) : 4, few_blocks = (N + few_rows - 1) / few_rows;
+  if (tile == -1) {
+    const int rows = M <= 2 ? M : 4;
+    CWM_REQUIRE(M <= FUSED_ROWS && K <= FUSED_SLOTS / rows * FUSED_SLOT, "linear_int8: %d rows of %d columns are too many for one launch", M, K);
+    const bool x_aligned = x_stride % 4 == 0 && (uintptr_t)x % (4 * x_size) == 0;
+#define INT8_FUSED_RUN(TX, T, ROWS, AHEAD)                                                                                                       \
+  hipLaunchKernelGGL((gemm_int8_few_kernel<TX, T, 1, ROWS, AHEAD>), dim3(few_blocks), dim3(64 * FEW_WAVES), M * Kp, stream, (const int8_t*)nullptr, \
+                     0l, (const float*)nullptr, (const TX*)x, x_stride, x_aligned, (const int8_t*)W, ldw, w_scale, bias, (T*)y, ldy, M, N, K, few_rows)
+#define INT8_FUSED_AHEAD(TX, T, ROWS)     \
+  {                                       \
+    if (a_wave <= 2)                      \
+      INT8_FUSED_RUN(TX, T, ROWS, 2);     \
+    else if (a_wave <= 4 || a_wave == 8)  \
+      INT8_FUSED_RUN(TX, T, ROWS, 4);     \
+    else                                  \
+      INT8_FUSED_RUN(TX, T, ROWS, 6);     \
+  }
+#define INT8_FUSED(TX, T)             \
+  {                                   \
+    if (rows == 1)                    \
+      INT8_FUSED_AHEAD(TX, T, 1)      \
+    else if (rows == 2)               \
+      INT8_FUSED_AHEAD(TX, T, 2)      \
+    else                              \
+      INT8_FUSED_AHEAD(TX, T, 4)      \
+  }
+    if (x_dtype == CWM_BF16 && dtype == CWM_BF16)
+      INT8_FUSED(bf16_t, bf16_t)
+    else if (x_dtype == CWM_BF16)
+      INT8_FUSED(bf16_t, float)
+    else if (dtype == CWM_BF16)
+      INT8_FUSED(float, bf16_t)
+    else
+      INT8_FUSED(float, float)
+    return cwm_launch_status("linear_int8 (one launch)");
+  }
+  CWM_REQUIRE(codes && a && (uintptr_t)codes % 16 == 0, "linear_int8: room for the integers is missing");
+  const int shift = tile > 0 ? Kp - K : 0;
+  if (int status = quantize_rows(x, x_stride, x_dtype, codes, Kp, a, M, K, Kp, shift, stream)) return status;
+  const int8_t* X = (const int8_t*)codes;
+  const long ldx = Kp;
   if (tile == 0) {
     const int row_tiles = (M + 15) / 16, rt = row_tiles >= 4 ? 4 : row_tiles >= 2 ? 2 : 1;
-    CWM_REQUIRE((row_tiles + rt - 1) / rt <= 65535, "gemm_int8: too many rows");
-    const dim3 grid((N + 15) / 16, (row_tiles + rt - 1) / rt);
-#define INT8_FEW(T, RT)                                                                                                                       \
-  hipLaunchKernelGGL((gemm_int8_few_kernel<T, RT>), grid, dim3(64 * FEW_WAVES), 0, stream, (const int8_t*)X, ldx, a, (const int8_t*)W, ldw,    \
-                     w_scale, bias, (T*)y, ldy, M, N, K)
-#define INT8_FEW_ROWS(T) \
-  if (rt == 4)           \
-    INT8_FEW(T, 4);      \
-  else if (rt == 2)      \
-    INT8_FEW(T, 2);      \
-  else                   \
-    INT8_FEW(T, 1)
+    CWM_REQUIRE((row_tiles + rt - 1) / rt <= 65535, "linear_int8: too many rows");
+    const dim3 grid(few_blocks, (row_tiles + rt - 1) / rt);
+#define INT8_FEW(T, RT, AHEAD)                                                                                                                       \
+  hipLaunchKernelGGL((gemm_int8_few_kernel<float, T, RT, 0, AHEAD>), grid, dim3(64 * FEW_WAVES), 0, stream, X, ldx, a, (const float*)nullptr, 0l, \
+                     false, (const int8_t*)W, ldw, w_scale, bias, (T*)y, ldy, M, N, K, few_rows)
+#define INT8_FEW_ROWS(T)          \
+  if (rt == 4)                    \
+    INT8_FEW(T, 4, 2);            \
+  else if (rt == 2 && a_wave <= 2) \
+    INT8_FEW(T, 2, 2);            \
+  else if (rt == 2)               \
+    INT8_FEW(T, 2, 4);            \
+  else if (a_wave <= 2)           \
+    INT8_FEW(T, 1, 2);            \
+  else if (a_wave <= 4 || a_wave == 8) \
+    INT8_FEW(T, 1, 4);            \
+  else                            \
+    INT8_FEW(T, 1, 6)
     if (dtype == CWM_BF16) {
       INT8_FEW_ROWS(bf16_t);
     } else {
       INT8_FEW_ROWS(float);
     }
-    return cwm_launch_status("gemm_int8 (few rows)");
+    return cwm_launch_status("linear_int8 (few rows)");
   }
-  CWM_REQUIRE(K % 128 == 0, "gemm_int8: the tiles of many rows take a K of a multiple of 128, not %d", K);
-  CWM_REQUIRE(ldx < (1L << 23) && ldw < (1L << 23), "gemm_int8: row strides too long for 32-bit offsets");
-  CWM_REQUIRE(tile >= 1 && tile <= 4, "gemm_int8: no tile %d", tile);
-  const bool vector = ldy % 4 == 0 && (uintptr_t)y % 16 == 0;
-#define INT8_WIDE(WM, WN)                                                                                                                           \
-  {                                                                                                                                                 \
-    const long m_tiles = (M + 32 * WM - 1) / (32 * WM), n_tiles = (N + 64 * WN - 1) / (64 * WN);                                                    \
-    CWM_REQUIRE(m_tiles * n_tiles * (K / 128) < (1L << 31), "gemm_int8: too many steps of tiles");                                                  \
-    const dim3 grid((unsigned)(m_tiles * n_tiles < units ? m_tiles * n_tiles : units));                                                             \
-    if (dtype == CWM_BF16)                                                                                                                          \
-      hipLaunchKernelGGL((gemm_int8_wide_kernel<WM, WN, bf16_t>), grid, dim3(512), 0, stream, (const int8_t*)X, ldx, a, (const int8_t*)W, ldw,      \
-                         w_scale, bias, (bf16_t*)y, ldy, vector, M, N, K / 128, (int)m_tiles, (int)n_tiles);                                         \
-    else                                                                                                                                            \
-      hipLaunchKernelGGL((gemm_int8_wide_kernel<WM, WN, float>), grid, dim3(512), 0, stream, (const int8_t*)X, ldx, a, (const int8_t*)W, ldw,       \
-                         w_scale, bias, (float*)y, ldy, vector, M, N, K / 128, (int)m_tiles, (int)n_tiles);                                          \
+  CWM_REQUIRE(K >= 128, "linear_int8: the tiles of many rows take a K of 128 and more, not %d", K);
+  CWM_REQUIRE(ldx < (1L << 23) && ldw < (1L << 23), "linear_int8: row strides too long for 32-bit offsets");
+  CWM_REQUIRE(tile >= 1 && tile <= 4, "linear_int8: no tile %d", tile);
+  const bool vector = ldy % 8 == 0 && (uintptr_t)y % 16 == 0;
+#define INT8_WIDE_RUN(WM, WN, T, ONCE)                                                                                                      \
+  hipLaunchKernelGGL((gemm_int8_wide_kernel<WM, WN, T, ONCE>), grid, dim3(512), 0, stream, (const int8_t*)X, ldx, a, (const int8_t*)W, ldw,  \
+                     w_scale, bias, (T*)y, ldy, vector, M, N, K, (int)m_tiles, (int)n_tiles)
+#define INT8_WIDE(WM, WN)                                                                                          \
+  {                                                                                                                \
+    const long m_tiles = (M + 32 * WM - 1) / (32 * WM), n_tiles = (N + 64 * WN - 1) / (64 * WN);                   \
+    CWM_REQUIRE(m_tiles * n_tiles * (Kp / 128) < (1L << 31), "linear_int8: too many steps of tiles");                 \
+    const dim3 grid((unsigned)(m_tiles * n_tiles < units ? m_tiles * n_tiles : units));                            \
+    if (dtype == CWM_BF16 && m_tiles == 1)                                                                         \
+      INT8_WIDE_RUN(WM, WN, bf16_t, true);                                                                         \
+    else if (dtype == CWM_BF16)                                                                                    \
+      INT8_WIDE_RUN(WM, WN, bf16_t, false);                                                                        \
+    else if (m_tiles == 1)                                                                                         \
+      INT8_WIDE_RUN(WM, WN, float, true);                                                                          \
+    else                                                                                                           \
+      INT8_WIDE_RUN(WM, WN, float, false);                                                                         \
   }
   if (tile == 1) INT8_WIDE(8, 2)
   if (tile == 2) INT8_WIDE(4, 4)
   if (tile == 3) INT8_WIDE(2, 2)
   if (tile == 4) INT8_WIDE(4, 2)
-  return cwm_launch_status("gemm_int8 (many rows)");
+  return cwm_launch_status("linear_int8 (many rows)");
 }

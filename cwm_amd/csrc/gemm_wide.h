@@ -47,11 +47,20 @@ struct WideShape {
 // rows in pairs of bytes as if they were bfloat16 (K and the row strides in units of two bytes).
 struct WideBf16 {
   typedef float4v Sums;
+  static constexpr bool W_ONCE = false;  // whether the rows of W go past the caches: with one tile of rows each is read once
+  // where a step of W's rows begins
+  template <typename SOURCE> static __device__ __forceinline__ size_t w_step(const SOURCE&, int step, int length) { return (size_t)step * length; }
   static __device__ __forceinline__ Sums run(const Frag8& w, const Frag8& a, const Sums& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v, a.v, c, 0, 0, 0); }
 };
 typedef int int4v __attribute__((ext_vector_type(4)));
-struct WideInt8 {  // K goes in steps of 128
+template <bool ONCE> struct WideInt8 {  // K goes in steps of 128
   typedef int4v Sums;
+  static constexpr bool W_ONCE = ONCE;
+  // A last step that reaches past K begins earlier instead, at the row's end less a step: A's row has zeros in the place of what
+  // it reads a second time.
+  template <typename SOURCE> static __device__ __forceinline__ size_t w_step(const SOURCE& src, int step, int length) {
+    return min(step * length, src.w_last);
+  }
   static __device__ __forceinline__ Sums run(const Frag8& w, const Frag8& a, const Sums& c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4v, w.u), __builtin_bit_cast(int4v, a.u), c, 0, 0, 0);
   }
@@ -81,7 +90,11 @@ __device__ __forceinline__ void wide_loop(unsigned char* lds, SOURCE& src, SINK&
   src.enter(i_tile);
   auto issue_one = [&](int i, uint32_t stage) __attribute__((always_inline)) {
     const int p = min(wave + 8 * i, PIECES - 1);
-    dma16(src.base(p) + (size_t)i_step * (SOURCE::W_TILES && p >= BM / 8 ? 1024 : WIDE_BK), src.off[i], lds0 + stage + p * 1024);
+    const bf16_t* from = src.base(p) + (p >= BM / 8 ? MMA::w_step(src, i_step, SOURCE::W_TILES ? 1024 : WIDE_BK) : (size_t)i_step * WIDE_BK);
+    if (MMA::W_ONCE && p >= BM / 8)
+      dma16_once(from, src.off[i], lds0 + stage + p * 1024);
+    else
+      dma16(from, src.off[i], lds0 + stage + p * 1024);
   };
   auto advance = [&]() __attribute__((always_inline)) {  // past the last step: that step again, into a buffer nobody reads
     if (i_left > 1) {

@@ -16,12 +16,66 @@ from . import build as _build
 CACHE_BITS = (4, 8)
 QUANT_MAX_DIM = 256  # csrc/quant_cache.h
 
+_P, _L, _I, _F = ctypes.c_void_p, ctypes.c_long, ctypes.c_int, ctypes.c_float
+# The C entry points by library, with their arguments' types: with these ctypes converts plain numbers by itself, which for
+# twenty arguments is 3 us less a call than objects made one by one.
+_ARGTYPES = {
+    "cwm_quant_kv_write": (_P, _L, _P, _L, _P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P),
+    "cwm_quant_kv_read": (_P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P),
+    "cwm_attention_quant": (_P, _L, _I, _P, _L, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P),
+    "cwm_quantize_rows": (_P, _L, _I, _P, _L, _P, _I, _I, _I, _P),
+    "cwm_linear_int8": (_P, _L, _I, _P, _P, _P, _L, _P, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P),
+}
+_entries: dict = {}
+
+
+def _entry(library: str, name: str, head_dim: Optional[int] = None):
+    """The entry point `name` of a library, and the library (for its error message)."""
+    found = _entries.get((name, head_dim))
+    if found is None:
+        lib = _build.load(library, None if head_dim is None else {"HEAD_DIM": head_dim})
+        function = getattr(lib, name)
+        function.argtypes = _ARGTYPES[name]
+        found = _entries[(name, head_dim)] = (function, lib)
+    return found
+
 
 @functools.cache  # an import statement costs a launch-bound step a microsecond and more a call
 def _base():
-    from . import KernelError, _check, _code, _i32, _need_gpu, _ptr, _stream  # the shared helpers of this package
+    from . import KernelError, _check, _code  # the shared helpers of this package
 
-    return KernelError, _check, _code, _i32, _need_gpu, _ptr, _stream
+    return KernelError, _check, _code
+
+
+def _stream() -> int:
+    """The current HIP stream of the current device, as a plain handle."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _check_device(*tensors: Optional[torch.Tensor]) -> None:
+    """All on one HIP device, and that the current one: kernels are launched on its stream."""
+    current = None
+    for t in tensors:
+        if t is None:
+            continue
+        if current is None:
+            if not t.is_cuda:
+                break
+            current = torch._C._cuda_getDevice()
+        if t.get_device() != current:
+            break
+    else:
+        return
+    KernelError = _base()[0]
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise KernelError(f"cwm_amd kernels run on a HIP device only; got a tensor on {t.device}. There is no CPU path.")
+    raise KernelError(f"tensors are on {', '.join(sorted({str(t.device) for t in tensors if t is not None}))}, the current device is cuda:{current}")
+
+
+def _check_vector(t: torch.Tensor, n: int, what: str) -> None:
+    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+        raise _base()[0](f"{what} must be a contiguous int32 [T] tensor for {n} tokens, found {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
 
 
 def _token_bytes(head_dim: int, bits: int) -> int:
@@ -29,6 +83,7 @@ def _token_bytes(head_dim: int, bits: int) -> int:
     return 2 * (head_dim * bits // 8) + head_dim // 32 * 4 + 4
 
 
+@functools.lru_cache(maxsize=1024)
 def quant_cache_limits(head_dim: int, page_size: int, bits: int) -> Optional[str]:
     """Why a cache of `bits` bits cannot hold heads of this size in pages of this many tokens, or None if it can."""
     if bits not in CACHE_BITS:
@@ -47,36 +102,36 @@ def quant_page_shape(n_kv_heads: int, head_dim: int, page_size: int, bits: int) 
     return (n_kv_heads, page_size * _token_bytes(head_dim, bits))
 
 
+@functools.lru_cache(maxsize=1024)
+def _page_size(shape: Tuple[int, ...], n_kv: Optional[int], head_dim: int, bits: int) -> Tuple[int, Optional[str]]:
+    """Tokens of a page of a cache of this shape, and why it is none."""
+    why = quant_cache_limits(head_dim, 8, bits)
+    if why is not None:
+        return 0, why
+    token = _token_bytes(head_dim, bits)
+    if len(shape) != 3 or min(shape) < 1 or (n_kv is not None and shape[1] != n_kv) or shape[2] % token != 0:
+        return 0, f"cache {shape} does not fit {n_kv or 'any'} heads of size {head_dim} in {bits} bits"
+    return shape[2] // token, quant_cache_limits(head_dim, shape[2] // token, bits)
+
+
 def _check_cache(cache: torch.Tensor, block_table: torch.Tensor, n_kv: Optional[int], head_dim: int, bits: int) -> int:
     """The tokens of a page of `cache`, a contiguous uint8 [pages, key/value heads, head bytes]."""
-    KernelError, _, _, _i32, *_ = _base()
-    if bits not in CACHE_BITS:
-        raise KernelError(f"a quantised cache holds 4 or 8 bits a value, not {bits}")
-    if head_dim % 32 != 0 or not 32 <= head_dim <= QUANT_MAX_DIM:
-        raise KernelError(f"a quantised cache takes head sizes of a multiple of 32 up to {QUANT_MAX_DIM}, not {head_dim}")
-    token = 2 * (head_dim * bits // 8) + head_dim // 32 * 4 + 4
-    if (
-        cache.dtype != torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or cache.shape[0] < 1 or cache.shape[1] < 1
-        or (n_kv is not None and cache.shape[1] != n_kv) or cache.shape[2] < 1 or cache.shape[2] % token != 0
-    ):
-        raise KernelError(f"cache {tuple(cache.shape)} {cache.dtype} does not fit {n_kv or 'any'} heads of size {head_dim} in {bits} bits")
-    page_size = cache.shape[2] // token
-    why = quant_cache_limits(head_dim, page_size, bits)
+    page_size, why = _page_size(tuple(cache.shape), n_kv, head_dim, bits)
+    if why is None and (cache.dtype != torch.uint8 or not cache.is_contiguous()):
+        why = f"the cache does not fit: it is contiguous and of bytes (uint8), found {cache.dtype} with strides {cache.stride()}"
+    if why is None and (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[1] < 1 or not block_table.is_contiguous()):
+        why = f"block_table must be a contiguous int32 [B, W] tensor, found {block_table.dtype} {tuple(block_table.shape)}"
     if why is not None:
-        raise KernelError(why)
-    _i32(block_table, "block_table")
-    if block_table.dim() != 2 or block_table.shape[1] < 1:
-        raise KernelError("block_table must be [B, W]")
+        raise _base()[0](why)
     return page_size
 
 
-def _check_device(*tensors: Optional[torch.Tensor]) -> None:
-    """All on one device, and that the current one: kernels are launched on its stream."""
-    KernelError, *_ = _base()
-    current = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t is not None and t.get_device() != current:
-            raise KernelError(f"a tensor is on {t.device}, the current device is cuda:{current}")
+def _bad_heads(name: str, t: torch.Tensor, n_tokens: int, heads: Optional[int], hd: int, dtype: torch.dtype) -> None:
+    """Raise what is wrong with queries, keys or values that are not [T, heads, hd] of `dtype` with contiguous heads."""
+    KernelError = _base()[0]
+    if t.dim() == 3 and t.shape[0] == n_tokens and t.shape[2] == hd and (heads is None or t.shape[1] == heads) and t.dtype != dtype:
+        raise KernelError("q, k and v must have one type")
+    raise KernelError(f"{name} must be [T, {'Hq' if name == 'q' else 'Hkv'}, hd] with contiguous heads, found {tuple(t.shape)} with strides {t.stride()}")
 
 
 def quant_kv_write(
@@ -96,39 +151,39 @@ def quant_kv_write(
     views into one wider tensor (token stride free, heads contiguous).  `q` [T, Hq, hd], where given, is rotated in place by the
     same angles.  No two tokens of a call may have the same place.  A group of values with an infinity or a NaN is
     held as NaN."""
-    KernelError, _check, _code, _i32, _need_gpu, _ptr, _stream = _base()
-    _need_gpu(k, v, q, positions, inv_freq, cache, block_table, seq_of_token)
+    KernelError, _check, _code = _base()
     _check_device(k, v, q, positions, inv_freq, cache, block_table, seq_of_token)
     if k.dim() != 3:
         raise KernelError("k must be [T, Hkv, hd] with contiguous heads")
-    n_tokens, n_kv, hd = k.shape
-    for name, t in (("k", k), ("v", v), ("q", q)):
-        if t is None:
-            continue
-        if t.dim() != 3 or t.shape[0] != n_tokens or t.shape[2] != hd or t.stride(2) != 1 or t.stride(1) != hd or (name == "v" and t.shape[1] != n_kv):
-            raise KernelError(f"{name} must be [T, {'Hq' if name == 'q' else 'Hkv'}, hd] with contiguous heads")
-        if t.dtype != k.dtype:
-            raise KernelError("q, k and v must have one type")
-    code = _code(k.dtype)
+    dtype = k.dtype
+    n_tokens, n_kv, hd = shape = k.shape
+    k_token, k_head, k_one = k.stride()
+    if k_one != 1 or k_head != hd:
+        _bad_heads("k", k, n_tokens, n_kv, hd, dtype)
+    if v.shape != shape or v.dtype != dtype or v.stride()[1:] != (hd, 1):
+        _bad_heads("v", v, n_tokens, n_kv, hd, dtype)
+    n_q = q_token = 0
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != n_tokens or q.shape[2] != hd or q.dtype != dtype or q.stride()[1:] != (hd, 1):
+            _bad_heads("q", q, n_tokens, None, hd, dtype)
+        n_q, q_token = q.shape[1], q.stride(0)
+        if n_tokens > 1 and q_token < n_q * hd:
+            raise KernelError("q is rotated in place: its rows must not overlap")
+    code = _code(dtype)
     page_size = _check_cache(cache, block_table, n_kv, hd, bits)
-    _i32(positions, "positions")
-    _i32(seq_of_token, "seq_of_token")
-    if positions.numel() != n_tokens or seq_of_token.numel() != n_tokens:
-        raise KernelError("positions and seq_of_token must be [T]")
+    _check_vector(positions, n_tokens, "positions")
+    _check_vector(seq_of_token, n_tokens, "seq_of_token")
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != hd // 2 or not inv_freq.is_contiguous()):
         raise KernelError(f"the rotary table must be float32 [{hd // 2}]")
-    if q is not None and n_tokens > 1 and q.stride(0) < q.shape[1] * hd:
-        raise KernelError("q is rotated in place: its rows must not overlap")
-    lib = _build.load("quant_cache")
-    _check(
-        lib,
-        lib.cwm_quant_kv_write(
-            _ptr(k), ctypes.c_long(k.stride(0)), _ptr(v), ctypes.c_long(v.stride(0)), _ptr(q), ctypes.c_long(q.stride(0) if q is not None else 0),
-            code, _ptr(positions), _ptr(seq_of_token), _ptr(inv_freq), _ptr(cache), _ptr(block_table),
-            block_table.shape[0], block_table.shape[1], page_size, cache.shape[0], n_tokens, n_kv, q.shape[1] if q is not None else 0, hd, bits,
-            _stream(),
-        ),
+    function, lib = _entry("quant_cache", "cwm_quant_kv_write")
+    n_seqs, width = block_table.shape
+    status = function(
+        k.data_ptr(), k_token, v.data_ptr(), v.stride(0), None if q is None else q.data_ptr(), q_token, code, positions.data_ptr(),
+        seq_of_token.data_ptr(), None if inv_freq is None else inv_freq.data_ptr(), cache.data_ptr(), block_table.data_ptr(), n_seqs, width, page_size,
+        cache.shape[0], n_tokens, n_kv, n_q, hd, bits, _stream(),
     )
+    if status:
+        _check(lib, status)
 
 
 def quant_kv_read(
@@ -142,26 +197,24 @@ def quant_kv_read(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values, each [T, Hkv, head_dim] of `dtype` (float32 or bfloat16), that a quantised `cache` holds of the
     tokens at `positions` [T] of the sequences `seq_of_token` [T] (rows of the block table); zeros where no page is held."""
-    KernelError, _check, _code, _i32, _need_gpu, _ptr, _stream = _base()
-    _need_gpu(cache, block_table, positions, seq_of_token)
+    _, _check, _code = _base()
     _check_device(cache, block_table, positions, seq_of_token)
     page_size = _check_cache(cache, block_table, None, head_dim, bits)
-    _i32(positions, "positions")
-    _i32(seq_of_token, "seq_of_token")
     n_tokens = positions.numel()
-    if seq_of_token.numel() != n_tokens:
-        raise KernelError("positions and seq_of_token must be [T]")
+    _check_vector(positions, n_tokens, "positions")
+    _check_vector(seq_of_token, n_tokens, "seq_of_token")
     code = _code(dtype)
-    k = torch.empty((n_tokens, cache.shape[1], head_dim), dtype=dtype, device=cache.device)
-    v = torch.empty_like(k)
-    lib = _build.load("quant_cache")
-    _check(
-        lib,
-        lib.cwm_quant_kv_read(
-            _ptr(k), _ptr(v), code, _ptr(positions), _ptr(seq_of_token), _ptr(cache), _ptr(block_table), block_table.shape[0],
-            block_table.shape[1], page_size, cache.shape[0], n_tokens, cache.shape[1], head_dim, bits, _stream(),
-        ),
+    pages, n_kv, _ = cache.shape
+    both = torch.empty((2, n_tokens, n_kv, head_dim), dtype=dtype, device=cache.device)
+    k, v = both.unbind(0)
+    function, lib = _entry("quant_cache", "cwm_quant_kv_read")
+    n_seqs, width = block_table.shape
+    status = function(
+        k.data_ptr(), v.data_ptr(), code, positions.data_ptr(), seq_of_token.data_ptr(), cache.data_ptr(), block_table.data_ptr(), n_seqs, width,
+        page_size, pages, n_tokens, n_kv, head_dim, bits, _stream(),
     )
+    if status:
+        _check(lib, status)
     return k, v
 
 
@@ -177,50 +230,50 @@ def quant_paged_attention(
     """Attention of the step's tokens over a quantised cache (`quant_kv_write`), prompt portions and decoded tokens in one
     call: `q` [T, Hq, hd] (float32 or bfloat16, rotated), `batch` the step's `StepBatch`, `window` the keys a query reads, its
     own included (None: all).  Returns [T, Hq * hd] in q's type.  A query one of whose keys has no page gets NaN."""
-    KernelError, _check, _code, _i32, _need_gpu, _ptr, _stream = _base()
+    KernelError, _check, _code = _base()
     from . import _attention_plan, _check_mask
 
-    _need_gpu(q, cache, block_table)
     _check_device(q, cache, block_table, batch.cu_q, batch.kv_len)
     _check_mask(window, None, None)
     if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
         raise KernelError("q must be [T, Hq, hd] with contiguous heads")
     n_tokens, n_q, hd = q.shape
     page_size = _check_cache(cache, block_table, None, hd, bits)
-    n_kv = cache.shape[1]
+    pages, n_kv, _ = cache.shape
     if n_q % n_kv != 0 or n_q == 0:
         raise KernelError(f"{n_q} query heads do not divide into {n_kv} key/value heads")
-    code = _code(q.dtype)
+    dtype = q.dtype
+    code = _code(dtype)
     if not scale > 0:
         raise KernelError("the scale of the scores must be positive")
     if block_table.shape[0] != batch.n_seqs or n_tokens != batch.n_tokens:
         raise KernelError("block_table must be [B, W] for the batch's sequences, q [T, ...] for its tokens")
-    if (n_tokens > 1 and q.stride(0) % (16 // q.element_size()) != 0) or q.data_ptr() % 16 != 0:
+    token = q.stride(0) if n_tokens > 1 else n_q * hd
+    if token % (4 if dtype == torch.float32 else 8) != 0 or q.data_ptr() % 16 != 0:
         raise KernelError("q rows must be 16-byte aligned")
-    out = torch.empty((n_tokens, n_q * hd), dtype=q.dtype, device=q.device)
+    out = torch.empty((n_tokens, n_q * hd), dtype=dtype, device=q.device)
     if n_tokens == 0:
         return out
     plan = _attention_plan(batch, n_q // n_kv, n_kv, hd, window, q.device)
     partial = None
     if plan.n_partials:
         partial = torch.empty(plan.n_partials * n_kv * 16 * (hd + 4), dtype=torch.float32, device=q.device)
-    lib = _build.load("attention_quant", {"HEAD_DIM": hd})
-    _check(
-        lib,
-        lib.cwm_attention_quant(
-            _ptr(q), ctypes.c_long(q.stride(0) if n_tokens > 1 else n_q * hd), code, _ptr(out), ctypes.c_long(n_q * hd), _ptr(cache), _ptr(block_table), block_table.shape[1],
-            _ptr(batch.cu_q), _ptr(batch.kv_len), _ptr(plan.work), plan.n_work, _ptr(plan.wide), plan.n_wide, plan.item_tiles,
-            _ptr(plan.merge), plan.n_merge, _ptr(partial), n_q, n_kv, hd, page_size, cache.shape[0],
-            -1 if window is None else window - 1, ctypes.c_float(scale), bits, _stream(),
-        ),
+    function, lib = _entry("attention_quant", "cwm_attention_quant", hd)
+    status = function(
+        q.data_ptr(), token, code, out.data_ptr(), n_q * hd, cache.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+        batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), plan.work.data_ptr(), plan.n_work, plan.wide.data_ptr(), plan.n_wide, plan.item_tiles,
+        plan.merge.data_ptr(), plan.n_merge, None if partial is None else partial.data_ptr(), n_q, n_kv, hd, page_size, pages,
+        -1 if window is None else window - 1, scale, bits, _stream(),
     )
+    if status:
+        _check(lib, status)
     return out
 
 
 # --------------------------------------------------------------------------- #
 INT8_MAX_K = 131072  # csrc/gemm_int8.hip: 127^2 K fits the 32 bits of a sum
-INT8_FEW_ROWS = 64
-_INT8_TILES = {1: (256, 128), 2: (128, 256), 3: (64, 128), 4: (128, 128)}
+INT8_FEW_ROWS = 16
+INT8_FUSED_ROWS, INT8_FUSED_K = 4, 16384  # csrc/gemm_int8.hip: rows of x, and the columns of one row, that every block makes the integers of
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -228,8 +281,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     127, the integers x / scale rounded, ties to even.  A row of zeros has a scale of 0; one with an infinity or a NaN has a NaN
     for its scale.  The integers are a view of rows padded with zeros to a multiple of 128, which `linear_int8` likes best for
     its weights."""
-    KernelError, _check, _code, _i32, _need_gpu, _ptr, _stream = _base()
-    _need_gpu(x)
+    KernelError, _check, _code = _base()
     _check_device(x)
     if x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise KernelError("rows to quantise must be [M, K] with contiguous rows")
@@ -238,8 +290,10 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     padded = -(-k // 128) * 128
     codes = torch.empty((m, padded), dtype=torch.int8, device=x.device)
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    lib = _build.load("gemm_int8")
-    _check(lib, lib.cwm_quantize_rows(_ptr(x), ctypes.c_long(x.stride(0)), code, _ptr(codes), ctypes.c_long(padded), _ptr(scale), m, k, padded, _stream()))
+    function, lib = _entry("gemm_int8", "cwm_quantize_rows")
+    status = function(x.data_ptr(), x.stride(0), code, codes.data_ptr(), padded, scale.data_ptr(), m, k, padded, _stream())
+    if status:
+        _check(lib, status)
     return codes[:, :k], scale
 
 
@@ -262,10 +316,9 @@ def linear_int8(
     multiplied with the int8 `weight` [N, K] with exact 32-bit sums, and scaled by the rows' scales and the float32
     `weight_scale` [N] (`quantize_rows` of the weight); `bias` float32 [N].  K a multiple of 16, rows of the weight 16-byte
     aligned.  Returns [M, N] in `out_dtype` (default: x's).  `tile` (tests) names one of the kernels."""
-    KernelError, _check, _code, _i32, _need_gpu, _ptr, _stream = _base()
+    KernelError, _check, _code = _base()
     from . import _compute_units
 
-    _need_gpu(x, weight, weight_scale, bias)
     _check_device(x, weight, weight_scale, bias)
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise KernelError(f"linear_int8: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
@@ -280,27 +333,44 @@ def linear_int8(
         raise KernelError(f"the weight's scales must be a contiguous float32 [{n}] tensor")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
         raise KernelError(f"linear_int8: the bias must be a contiguous float32 [{n}] tensor")
+    if k > 1 and x.stride(1) != 1:
+        raise KernelError("linear_int8: x must have contiguous rows")
+    x_code = _code(x.dtype)
     y = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
     code = _code(y.dtype)
     if m == 0:
-        _code(x.dtype)
         return y
-    codes, scale = quantize_rows(x)
     if tile is None:
-        tile = _int8_tile(m, n, k)
-    lib = _build.load("gemm_int8")
-    _check(
-        lib,
-        lib.cwm_gemm_int8(
-            _ptr(codes), ctypes.c_long(codes.stride(0)), _ptr(scale), _ptr(weight), ctypes.c_long(weight.stride(0) if n > 1 else max(k, weight.stride(0))),
-            _ptr(weight_scale), _ptr(bias), _ptr(y), code, ctypes.c_long(n), m, n, k, _compute_units(x.device), tile, _stream(),
-        ),
+        tile = _int8_tile(m, n, k, _compute_units(x.device))
+    codes = scale = None
+    if tile >= 0:
+        padded = -(-k // 128) * 128
+        room = torch.empty(m * (padded + 4), dtype=torch.uint8, device=x.device)  # the integers of x, then their scales
+        codes = room.data_ptr()
+        scale = codes + m * padded
+    function, lib = _entry("gemm_int8", "cwm_linear_int8")
+    status = function(
+        x.data_ptr(), x.stride(0), x_code, codes, scale, weight.data_ptr(), weight.stride(0) if n > 1 else max(k, weight.stride(0)),
+        weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), code, n, m, n, k, _compute_units(x.device), tile, _stream(),
     )
+    if status:
+        _check(lib, status)
     return y
 
 
-def _int8_tile(m: int, n: int, k: int) -> int:
-    """The kernel for a product's sizes."""
-    if m <= INT8_FEW_ROWS or k % 128 != 0:
+# The tiles of many rows (number of the kernel's, rows, columns), and what each costs: us a round of tiles, and a step of 128 columns of K
+# of a round.  Fitted to 2,048 x 43,008 with a K of 1,536, 3,200 and 6,144 (tiles of 256 x 128: 161, 281 and 509 us, 128 x 256 162, 290 and
+# 495, 64 x 128 259, 465 and 820, 128 x 128 199, 346 and 590).
+_INT8_TILES = ((1, 256, 128, 2.9, 0.98), (2, 128, 256, 5.6, 0.85), (3, 64, 128, 1.6, 0.38), (4, 128, 128, 3.2, 0.52))
+
+
+@functools.lru_cache(maxsize=1024)
+def _int8_tile(m: int, n: int, k: int, units: int) -> int:
+    """The kernel for a product's sizes.  Up to four rows one launch does all (1 x 6,144 x 6,144 14.5 us, in two launches 16.2);
+    up to 16 W is read straight into the matrix instruction (16 x 6,144 x 6,144 20.3 us, tiles of 64 rows 27.2; 16 x 28,672 x 4,096 41.5
+    and 32.1: there the tiles' loads, further ahead, are the faster ones); more rows take the tile of least cost."""
+    if m <= INT8_FUSED_ROWS and k <= INT8_FUSED_K // (m if m <= 2 else 4):
+        return -1
+    if k < 128 or (m <= INT8_FEW_ROWS and n * k < 1 << 26):
         return 0
-    return 1
+    return min(_INT8_TILES, key=lambda t: -(-(-(-m // t[1]) * -(-n // t[2])) // units) * (t[3] + -(-k // 128) * t[4]))[0]

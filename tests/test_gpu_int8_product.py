@@ -86,9 +86,31 @@ def test_products_of_few_rows(dtype):
         _check(x, w, s, None, torch.float32, 0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_products_of_one_launch(dtype):
+    """Up to four rows, whose integers every block makes itself."""
+    for i, (m, n, k) in enumerate([(1, 1, 16), (1, 100, 48), (2, 33, 2048), (3, 16, 144), (3, 9000, 256), (4, 70, 1040), (4, 130, 4096), (1, 20, 16384), (2, 20, 8176)]):
+        x = _rows(m, k, dtype, i)
+        w, s = _weight(n, k, i, stride=k + 16 * (i % 2))
+        bias = torch.randn(n) if i % 2 else None
+        for out in (torch.bfloat16, torch.float32):
+            _check(x, w, s, bias, out, -1)
+        y = ops.linear_int8(x.to(DEV), w.to(DEV), s.to(DEV), tile=-1)
+        assert torch.equal(y, ops.linear_int8(x.to(DEV), w.to(DEV), s.to(DEV), tile=0))
+        wide = torch.cat([x, x], 1).to(DEV)[:, 1 : 1 + k]  # rows that no vector load takes
+        _check(wide.cpu(), w, s, bias, dtype, -1)
+        assert torch.equal(ops.linear_int8(wide, w.to(DEV), s.to(DEV), tile=-1), ops.linear_int8(wide, w.to(DEV), s.to(DEV), tile=0))
+    x = _rows(4, 64, dtype, 1)
+    x[0] *= 0
+    x[1, 3], x[2, 60] = math.nan, math.inf
+    w, s = _weight(40, 64, 2)
+    y = ops.linear_int8(x.to(DEV), w.to(DEV), s.to(DEV), tile=-1)
+    assert torch.isnan(y[1:3]).all() and not y[0].any() and torch.isfinite(y[3]).all()
+
+
 @pytest.mark.parametrize("tile", [1, 2, 3, 4])
 def test_products_of_many_rows(tile):
-    for i, (m, n, k) in enumerate([(1, 1, 128), (65, 100, 256), (300, 130, 384), (257, 513, 1024), (1000, 2000, 512), (513, 1027, 128)]):
+    for i, (m, n, k) in enumerate([(1, 1, 128), (65, 100, 256), (300, 130, 384), (257, 513, 1024), (1000, 2000, 512), (513, 1027, 128), (70, 300, 144), (130, 131, 2032), (5, 17, 1104)]):
         x = _rows(m, k, torch.bfloat16, i)
         w, s = _weight(n, k, i, stride=k + 128 * (i % 2))
         _check(x, w, s, torch.randn(n) if i % 2 else None, torch.bfloat16 if i % 3 else torch.float32, tile)
@@ -104,7 +126,7 @@ def test_sums_at_the_end_of_their_range():
 
 
 def test_the_call_chooses_among_its_kernels():
-    for m, n, k in [(1, 2048, 2048), (5, 512, 8192), (40, 4096, 512), (100, 1024, 1024), (600, 1536, 640), (200, 256, 2064)]:
+    for m, n, k in [(1, 2048, 2048), (5, 512, 8192), (40, 4096, 512), (100, 1024, 1024), (600, 1536, 640), (200, 256, 2064), (17, 300, 112), (300, 9000, 4080)]:
         x = _rows(m, k, torch.bfloat16, m)
         w, s = _weight(n, k, m)
         _check(x, w, s, None, torch.bfloat16)
