@@ -58,19 +58,47 @@ template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, ui
   }
 }
 
+// The same through a buffer resource, which bounds the offsets: past its size a load gives zeros and reads nothing, so one of size
+// 0 takes the place of a branch around the loads.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int N> __device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t r, uint32_t offset, uint32_t (&w)[N]) {
+  constexpr int ONCE = 2;  // non-temporal: every block reads keys and values of its own
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const u32x4 u = __builtin_amdgcn_raw_buffer_load_b128(r, offset + 4 * i, 0, ONCE);
+      w[i] = u[0], w[i + 1] = u[1], w[i + 2] = u[2], w[i + 3] = u[3];
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const u32x2 u = __builtin_amdgcn_raw_buffer_load_b64(r, offset + 4 * i, 0, ONCE);
+      w[i] = u[0], w[i + 1] = u[1];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, offset + 4 * i, 0, ONCE);
+  }
+}
+
 // How codes become numbers of bfloat16.  EXACT: c - H.  Else OFF' + c, OFF' = 128 for 4 bits and 0 for 8.
 template <int BITS, bool EXACT> struct Codes {
   static constexpr int H = 1 << (BITS - 1);
   static constexpr float OFF = EXACT ? 0.f : (BITS == 4 ? 128.f + H : (float)H);
+  // The constants of `nibbles` in registers that the compiler knows nothing of: it then forms one instruction of mask and "or", which
+  // takes no two literals.  (Not one written by hand: it could not see to the wait between that and the matrix instruction.)
+  uint32_t mask = 0x000f000fu, base = 0x43004300u;
+  __device__ __forceinline__ Codes() { asm volatile("" : "+s"(mask), "+v"(base)); }
   // four bits from bit 0 and from bit 16 on
-  static __device__ __forceinline__ uint32_t nibbles(uint32_t w) {
+  __device__ __forceinline__ uint32_t nibbles(uint32_t w) const {
     if constexpr (EXACT) {
       const float a = (float)((int)(w & 15u) - H), b = (float)((int)((w >> 16) & 15u) - H);
       return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
     }
-    return (w & 0x000f000fu) | 0x43004300u;
+    return (w & mask) | base;
   }
-  static __device__ __forceinline__ uint32_t bytes(uint32_t w, int first) {  // bytes `first` and `first + 1`
+  __device__ __forceinline__ uint32_t bytes(uint32_t w, int first) const {  // bytes `first` and `first + 1`
     float a = (float)((w >> (8 * first)) & 255u), b = (float)((w >> (8 * first + 8)) & 255u);
     if constexpr (EXACT) a -= H, b -= H;
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
@@ -133,7 +161,9 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
   bool row_valid[RT];
   int ti[RT], hq[RT], row_end[RT], row_start[RT];
   Frag8 qf[RT][PARTS][G], qs[RT][QUADS];
-  int lo_any = 0x7fffffff, hi_any = -1, lo_all = key_begin, hi_all = key_end - 1;
+  Frag8 ones;  // a row of ones
+  ones.u = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+  const float4v zero = (float4v){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = w[1] + 16 * (SPLIT ? rt : RT * wave + rt) + n;
@@ -142,30 +172,26 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
     hq[rt] = g0 * group + (row_valid[rt] ? r - ti[rt] * group : 0);
     row_end[rt] = n_old + ti[rt];
     row_start[rt] = window_left >= 0 ? max(0, row_end[rt] - window_left) : 0;
-    lo_any = min(lo_any, row_valid[rt] ? row_start[rt] : 0x7fffffff);
-    hi_any = max(hi_any, row_valid[rt] ? row_end[rt] : -1);
-    lo_all = max(lo_all, row_valid[rt] ? row_start[rt] : 0x7fffffff);
-    hi_all = min(hi_all, row_valid[rt] ? row_end[rt] : -1);
 
     // queries: the B operands, and the sums over a group's elements in three parts, one part for each j < 3
     const T* qrow = q + (size_t)(q0 + ti[rt]) * q_stride + (size_t)hq[rt] * HEAD_DIM + 8 * j;
-    float sum[G];
+    float sum[G];  // a product with the row of ones
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      float x[8];
       if constexpr (EXACT) {
         float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
         if (row_valid[rt]) lo = *(const float4*)(qrow + 32 * g), hi = *(const float4*)(qrow + 32 * g + 4);
-        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
-        { Frag8 part[3]; three_parts(x, part); qf[rt][0][g] = part[0], qf[rt][1 % PARTS][g] = part[1], qf[rt][2 % PARTS][g] = part[2]; }
+        const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        Frag8 part[3];
+        three_parts(x, part);
+        qf[rt][0][g] = part[0], qf[rt][1 % PARTS][g] = part[1], qf[rt][2 % PARTS][g] = part[2];
       } else {
         qf[rt][0][g].u = row_valid[rt] ? *(const uint4*)(qrow + 32 * g) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = bf16_to_f32(qf[rt][0][g].h[e]);
       }
-      sum[g] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-      sum[g] += __shfl_xor(sum[g], 16, 64);
-      sum[g] += __shfl_xor(sum[g], 32, 64);
+      float4v d = zero;
+#pragma unroll
+      for (int p = PARTS - 1; p >= 0; --p) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones.v, qf[rt][p][g].v, d, 0, 0, 0);
+      sum[g] = d[0];
     }
 #pragma unroll
     for (int u = 0; u < QUADS; ++u) {
@@ -180,31 +206,41 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
       qs[rt][u].u = j == 0 ? part[0].u : j == 1 ? part[1].u : j == 2 ? part[2].u : make_uint4(0, 0, 0, 0);
     }
   }
-#pragma unroll
-  for (int off = 1; off < 16; off <<= 1) {
-    lo_any = min(lo_any, __shfl_xor(lo_any, off, 64));
-    hi_any = max(hi_any, __shfl_xor(hi_any, off, 64));
-    lo_all = max(lo_all, __shfl_xor(lo_all, off, 64));
-    hi_all = min(hi_all, __shfl_xor(hi_all, off, 64));
+  // The span of keys that any of the wavefront's rows reads, and the span that all of them read: tiles within it need no masks.  Rows
+  // that do not exist have queries of zeros and are not stored: they read whatever the others do.
+  int lo_any = 0x7fffffff, hi_any = -1, lo_all = 0, hi_all = 0x7fffffff;
+  const int first_row = w[1] + (SPLIT ? 0 : 16 * RT * wave), last_row = min(first_row + 16 * RT, n_rows) - 1;
+  if (first_row <= last_row) {
+    const int first_end = n_old + first_row / group, last_end = n_old + last_row / group;
+    lo_any = max(key_begin, window_left >= 0 ? first_end - window_left : 0);
+    hi_any = min(key_end - 1, last_end);
+    lo_all = max(key_begin, window_left >= 0 ? last_end - window_left : 0);
+    hi_all = min(key_end - 1, first_end);
   }
-  lo_any = max(lo_any, key_begin);
-  hi_any = min(hi_any, key_end - 1);
+  // a row reads its keys first .. first + count - 1 of the item
+  int first_key[RT];
+  unsigned key_count[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    first_key[rt] = max(row_start[rt], key_begin);
+    key_count[rt] = row_valid[rt] ? max(0, min(row_end[rt], key_end - 1) - first_key[rt] + 1) : 0;
+  }
 
   const int* table = block_table + (size_t)b * table_width;
   const scalar_ints table_s = (scalar_ints)table;
   const bool page_missing = span_lacks_page(table, table_width, num_pages, page_size, lo_any, hi_any, lane);
   const QuantHead at = quant_head(page_size, HEAD_DIM, BITS);
+  // a head of a page has less than 2 GiB: offsets within it are 32 bits, beside a page's address in scalar registers
+  const uint32_t values_at = (uint32_t)at.values, key_words_at = (uint32_t)at.key_words, value_words_at = (uint32_t)at.value_words;
   const size_t page_bytes = (size_t)at.bytes * n_kv_heads;
   const uint8_t* base = cache + (size_t)at.bytes * g0;
 
-  // the operands that pick one group's step out of a key's words (element 2 i + 1 of the first eight), and a row of ones
-  Frag8 pick[4], ones;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t one = j == 0 ? 0x3f800000u : 0u;
-    pick[i].u = make_uint4(i == 0 ? one : 0, i == 1 ? one : 0, i == 2 ? one : 0, i == 3 ? one : 0);
-  }
-  ones.u = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+  // The operands that bring a group's step out of a pair of words to all columns (1 at the upper half of the first or of the second
+  // word, in one lane of four).
+  typedef short Pair __attribute__((ext_vector_type(4)));
+  const uint32_t one = j == 0 ? 0x3f800000u : 0u;
+  const Pair pick[2] = {__builtin_bit_cast(Pair, make_uint2(one, 0)), __builtin_bit_cast(Pair, make_uint2(0, one))};
+  const C codes;
 
   // page of a key; keys outside the item and slots without a page read page 0 and are masked
   auto page_of = [&](int key, int& slot_in_page) -> int {
@@ -214,31 +250,52 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
     return (page >= 0 && page < num_pages) ? page : 0;
   };
   const int krel = 8 * (n >> 2) + (n & 3);
-  auto issue = [&](Keys& L, int kt) {
-    const uint8_t *kpage, *vpage;
-    int ks, vs;
-    if constexpr (PAGE32) {  // a tile lies in one page, whose number is read as a scalar
-      const int lp = page_shift >= 0 ? (kt >> page_shift) : (kt / page_size);
-      int page = lp < table_width ? table_s[lp] : 0;
-      page = (page >= 0 && page < num_pages) ? page : 0;
-      kpage = vpage = base + (size_t)page * page_bytes;
-      ks = kt - lp * page_size + krel;
-      vs = kt - lp * page_size + 8 * j;
-    } else {
-      kpage = base + (size_t)page_of(kt + krel, ks) * page_bytes;
-      vpage = base + (size_t)page_of(kt + 8 * j, vs) * page_bytes;
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      load_words<Keys::KC>(kpage + (uint32_t)((ks + 4 * t) * 4 + j) * (Keys::KC * 4), L.kc[t]);
-      load_words<G>(kpage + at.key_words + (uint32_t)(ks + 4 * t) * (G * 4), L.kw[t]);
-    }
-    load_words<8>(vpage + at.value_words + (uint32_t)vs * 4, L.vw);
-    const uint8_t* vb = vpage + at.values + (uint32_t)(vs >> 3) * (HEAD_DIM * BITS);
+  // as many tiles' registers as there is room for: 4 bits and heads of up to 128 three, others two
+  constexpr int BUFFERS = PAGE32 && BITS == 4 && !EXACT && HEAD_DIM <= 128 ? 3 : 2;
+  constexpr int STEP = SPLIT ? TEAM : 1;  // wavefront w starts at the item's tile w and goes on in steps of TEAM tiles, or takes every tile
+  // PAGE32: a tile lies in one page, whose number is read as a scalar a tile ahead
+  auto look_up = [&](int kt) -> int {
+    const int lp = min(page_shift >= 0 ? (kt >> page_shift) : (kt / page_size), table_width - 1);
+    return PAGE32 ? table_s[lp] : 0;
+  };
+  int page_ahead = 0;
+  const int tile0 = key_begin >> 5, tiles = ((key_end + 31) >> 5) - tile0;
+  // the loads of the item's tile `t`, which may lie past its last one: then of nothing
+  auto issue = [&](Keys& L, int t) {
+    const int kt = 32 * (tile0 + t);
     constexpr int PIECES = Keys::VC / 4;
+    if constexpr (PAGE32) {
+      const int lp = page_shift >= 0 ? (kt >> page_shift) : (kt / page_size);
+      const int page = (unsigned)page_ahead < (unsigned)num_pages ? page_ahead : 0;
+      page_ahead = look_up(kt + 32 * STEP);
+      const __amdgpu_buffer_rsrc_t head =
+          __builtin_amdgcn_make_buffer_rsrc((void*)(base + (size_t)page * page_bytes), 0, t < tiles ? (int)at.bytes : 0, 0x00027000);
+      const int ks = kt - lp * page_size + krel, vs = kt - lp * page_size + 8 * j;
 #pragma unroll
-    for (int c = 0; c < PIECES; ++c) load_words<4>(vb + 256 * c + 16 * n, *(uint32_t(*)[4])&L.vc[4 * c]);
-    if constexpr (Keys::VC % 4 != 0) load_words<2>(vb + 256 * PIECES + 8 * n, *(uint32_t(*)[2])&L.vc[4 * PIECES]);
+      for (int i = 0; i < 2; ++i) {
+        load_words<Keys::KC>(head, (uint32_t)(((ks + 4 * i) * 4 + j) * (Keys::KC * 4)), L.kc[i]);
+        load_words<G>(head, key_words_at + (uint32_t)(ks + 4 * i) * (G * 4), L.kw[i]);
+      }
+      load_words<8>(head, value_words_at + (uint32_t)vs * 4, L.vw);
+      const uint32_t vb = values_at + (uint32_t)(vs >> 3) * (HEAD_DIM * BITS);
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c) load_words<4>(head, vb + 256 * c + 16 * n, *(uint32_t(*)[4])&L.vc[4 * c]);
+      if constexpr (Keys::VC % 4 != 0) load_words<2>(head, vb + 256 * PIECES + 8 * n, *(uint32_t(*)[2])&L.vc[4 * PIECES]);
+    } else {
+      int ks, vs;
+      const uint8_t* kpage = base + (size_t)page_of(kt + krel, ks) * page_bytes;
+      const uint8_t* vpage = base + (size_t)page_of(kt + 8 * j, vs) * page_bytes;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        load_words<Keys::KC>(kpage + (uint32_t)(((ks + 4 * i) * 4 + j) * (Keys::KC * 4)), L.kc[i]);
+        load_words<G>(kpage + (key_words_at + (uint32_t)(ks + 4 * i) * (G * 4)), L.kw[i]);
+      }
+      load_words<8>(vpage + (value_words_at + (uint32_t)vs * 4), L.vw);
+      const uint32_t vb = values_at + (uint32_t)(vs >> 3) * (HEAD_DIM * BITS);
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c) load_words<4>(vpage + (vb + 256 * c + 16 * n), *(uint32_t(*)[4])&L.vc[4 * c]);
+      if constexpr (Keys::VC % 4 != 0) load_words<2>(vpage + (vb + 256 * PIECES + 8 * n), *(uint32_t(*)[2])&L.vc[4 * PIECES]);
+    }
   };
 
   float4v acc[RT][D_TILES], bsum[RT];
@@ -253,7 +310,6 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
   }
 
   auto compute = [&](const Keys& L, int kt) {
-    const float4v zero = (float4v){0.f, 0.f, 0.f, 0.f};
     float4v st[RT][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -272,12 +328,13 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
         Frag8 kf;
         if constexpr (BITS == 4) {
           const uint32_t c = L.kc[t][g % Keys::KC];
-          kf.u = make_uint4(C::nibbles(c), C::nibbles(c >> 4), C::nibbles(c >> 8), C::nibbles(c >> 12));
+          kf.u = make_uint4(codes.nibbles(c), codes.nibbles(c >> 4), codes.nibbles(c >> 8), codes.nibbles(c >> 12));
         } else {
           const uint32_t c0 = L.kc[t][(2 * g) % Keys::KC], c1 = L.kc[t][(2 * g + 1) % Keys::KC];
-          kf.u = make_uint4(C::bytes(c0, 0), C::bytes(c0, 2), C::bytes(c1, 0), C::bytes(c1, 2));
+          kf.u = make_uint4(codes.bytes(c0, 0), codes.bytes(c0, 2), codes.bytes(c1, 0), codes.bytes(c1, 2));
         }
-        const float4v step = __builtin_amdgcn_mfma_f32_16x16x32_bf16(words[g / 4].v, pick[g % 4].v, zero, 0, 0, 0);
+        const uint2 pair = make_uint2(L.kw[t][g / 2 * 2], g / 2 * 2 + 1 < G ? L.kw[t][(g / 2 * 2 + 1) % G] : 0u);
+        const float4v step = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(Pair, pair), pick[g % 2], zero, 0, 0, 0);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           float4v d = zero;
@@ -297,8 +354,7 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
       if (need_mask) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int key = kt + 8 * j + e;
-          const bool ok = row_valid[rt] && key <= row_end[rt] && key >= row_start[rt] && key >= key_begin && key < key_end;
+          const bool ok = (unsigned)(kt + 8 * j + e - first_key[rt]) < key_count[rt];
           hidden |= ok ? 0u : 1u << e;
           x[e] = ok ? x[e] : neg_inf;
         }
@@ -320,22 +376,25 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
         for (int d = 0; d < D_TILES; ++d) acc[rt][d] *= alpha;
         m_run[rt] = m_new, neg_mc[rt] = neg;
       }
-      float bv[8];
+      float bv[8], z[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(x[e], scale_log2e, neg_mc[rt]));
-        l_run[rt] += p;
-        bv[e] = p * word_step(L.vw[e]);
-        x[e] = p * word_offset(L.vw[e]);
-      }
+      for (int e = 0; e < 8; ++e) bv[e] = word_step(L.vw[e]), z[e] = word_offset(L.vw[e]);
       if (need_mask) {  // a key that a row does not read may hold anything, a NaN among it
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           bv[e] = (hidden >> e) & 1 ? 0.f : bv[e];
-          x[e] = (hidden >> e) & 1 ? 0.f : x[e];
+          z[e] = (hidden >> e) & 1 ? 0.f : z[e];
         }
       }
-      z_run[rt] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+      float z_even = z_run[rt], z_odd = 0.f, l_even = l_run[rt], l_odd = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(x[e], scale_log2e, neg_mc[rt])), p1 = __builtin_amdgcn_exp2f(fmaf(x[e + 1], scale_log2e, neg_mc[rt]));
+        l_even += p0, l_odd += p1;
+        z_even = fmaf(p0, z[e], z_even), z_odd = fmaf(p1, z[e + 1], z_odd);
+        bv[e] *= p0, bv[e + 1] *= p1;
+      }
+      l_run[rt] = l_even + l_odd, z_run[rt] = z_even + z_odd;
       if constexpr (EXACT) {
         Frag8 part[3]; three_parts(bv, part); bf[rt][0] = part[0], bf[rt][1 % PARTS] = part[1], bf[rt][2 % PARTS] = part[2];
       } else {
@@ -350,10 +409,10 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
       Frag8 vf;
       if constexpr (BITS == 4) {
         const uint32_t c0 = L.vc[2 * (d / 2)] >> (4 * (d & 1)), c1 = L.vc[2 * (d / 2) + 1] >> (4 * (d & 1));
-        vf.u = make_uint4(C::nibbles(c0), C::nibbles(c0 >> 8), C::nibbles(c1), C::nibbles(c1 >> 8));
+        vf.u = make_uint4(codes.nibbles(c0), codes.nibbles(c0 >> 8), codes.nibbles(c1), codes.nibbles(c1 >> 8));
       } else {
         const uint32_t c0 = L.vc[(2 * d) % Keys::VC], c1 = L.vc[(2 * d + 1) % Keys::VC];
-        vf.u = make_uint4(C::bytes(c0, 0), C::bytes(c0, 2), C::bytes(c1, 0), C::bytes(c1, 2));
+        vf.u = make_uint4(codes.bytes(c0, 0), codes.bytes(c0, 2), codes.bytes(c1, 0), codes.bytes(c1, 2));
       }
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -362,19 +421,26 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
     }
   };
 
-  // wavefront w starts at the item's tile w and goes on in steps of TEAM tiles, or takes every tile
-  constexpr int STEP = SPLIT ? TEAM : 1;
-  const int tile0 = key_begin >> 5, tiles = ((key_end + 31) >> 5) - tile0;
+  // The registers of BUFFERS tiles in turn, the loads of the tile BUFFERS - 1 on ahead of this one's arithmetic (a copy from one to
+  // the other would wait for the loads).  A tile past the last one reads page 0's first keys where it is not a load of nothing.
   int tile = SPLIT ? wave : 0;
   if (tile < tiles) {
-    Keys now, next;
-    issue(now, 32 * (tile0 + tile));
-    for (; tile + STEP < tiles; tile += STEP) {
-      issue(next, 32 * (tile0 + tile + STEP));
-      compute(now, 32 * (tile0 + tile));
-      now = next;
+    Keys held[BUFFERS];
+    page_ahead = look_up(32 * (tile0 + tile));
+#pragma unroll
+    for (int u = 0; u < BUFFERS - 1; ++u) issue(held[u], tile + u * STEP);
+    for (bool more = true; more;) {
+#pragma unroll
+      for (int u = 0; u < BUFFERS; ++u) {
+        issue(held[(u + BUFFERS - 1) % BUFFERS], tile + (BUFFERS - 1) * STEP);
+        compute(held[u], 32 * (tile0 + tile));
+        tile += STEP;
+        if (tile >= tiles) {
+          more = false;
+          break;
+        }
+      }
     }
-    compute(now, 32 * (tile0 + tile));
   }
 
   // ---- a row's sums over its lanes, and the output that the sums stand for ------------------- //
@@ -484,46 +550,64 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
 }
 
 // Joins the partial results of a row: merge item {sequence, first row, first slot, number of partials}; grid (items,
-// key/value heads, 16 rows), a thread for each of 4 neighbouring dimensions and each `blockDim.y`-th partial.
+// key/value heads, 16 rows).  Wavefront w takes partials w, w + MERGE_WAVES, ..., four loads of each at a time.
+#define MERGE_WAVES 4
 template <typename T>
-__global__ void attention_quant_merge_kernel(T* __restrict__ out, long out_stride, const float* __restrict__ partial, const int* __restrict__ cu_q,
-                                             const int* __restrict__ merge, int n_q_heads, int n_kv_heads) {
+__global__ void __launch_bounds__(64 * MERGE_WAVES)
+attention_quant_merge_kernel(T* __restrict__ out, long out_stride, const float* __restrict__ partial, const int* __restrict__ cu_q,
+                             const int* __restrict__ merge, int n_q_heads, int n_kv_heads) {
   const int* item = merge + (size_t)blockIdx.x * 4;
   const int b = item[0], first = item[2], count = item[3];
   const int g = blockIdx.y, n = blockIdx.z, group = n_q_heads / n_kv_heads;
   const int q0 = cu_q[b], r = item[1] + n;
   if (r >= (cu_q[b + 1] - q0) * group || count <= 0) return;  // also null items, whose first row lies beyond every sequence's
+  constexpr int PER = (HEAD_DIM + 63) / 64;
   const float neg_inf = -__builtin_inff();
-  __shared__ __attribute__((aligned(16))) float o_of[16][HEAD_DIM];
-  __shared__ float l_of[16];
-  const float* rows = partial + ((size_t)first * n_kv_heads + g) * 16 * PARTIAL_STRIDE + (size_t)n * PARTIAL_STRIDE;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ float top_of[MERGE_WAVES], l_of[MERGE_WAVES], o_of[MERGE_WAVES][HEAD_DIM];
+  const float* rows = partial + (((size_t)first * n_kv_heads + g) * 16 + n) * PARTIAL_STRIDE;
   const size_t stride = (size_t)n_kv_heads * 16 * PARTIAL_STRIDE;
   float top = neg_inf;
-  for (int p = 0; p < count; ++p) top = fmaxf(top, rows[p * stride + HEAD_DIM]);
-  const int d = 4 * threadIdx.x;
-  float4v sum = (float4v){0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  for (int p = threadIdx.y; p < count; p += blockDim.y) {
-    const float m = rows[p * stride + HEAD_DIM];
-    if (m == neg_inf) continue;  // a chunk with no key of this row
-    const float f = __builtin_amdgcn_exp2f(m - top);
-    l += f * rows[p * stride + HEAD_DIM + 1];
-    sum += f * *(const float4v*)(rows + p * stride + d);
-  }
-  *(float4v*)&o_of[threadIdx.y][d] = sum;
-  if (threadIdx.x == 0) l_of[threadIdx.y] = l;
+  for (int p = threadIdx.x; p < count; p += 64 * MERGE_WAVES) top = fmaxf(top, rows[p * stride + HEAD_DIM]);
+  top = wave_max(top);
+  if (lane == 0) top_of[wave] = top;
   __syncthreads();
-  if (threadIdx.y != 0) return;
-  float total = l_of[0];
-  for (int y = 1; y < (int)blockDim.y; ++y) {
-    total += l_of[y];
-    sum += *(const float4v*)&o_of[y][d];
-  }
-  const int ti = r / group;
-  T* row = out + (size_t)(q0 + ti) * out_stride + (size_t)(g * group + r - ti * group) * HEAD_DIM + d;
-  const float inv = 1.0f / total;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) Elem<T>::store(row + e, sum[e] * inv);
+  for (int w = 0; w < MERGE_WAVES; ++w) top = fmaxf(top, top_of[w]);
+  float o[PER] = {}, l = 0.f;
+  for (int p0 = wave; p0 < count; p0 += 4 * MERGE_WAVES) {
+    float m[4], lp[4], op[4][PER];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float* row = rows + min(p0 + u * MERGE_WAVES, count - 1) * stride;
+      m[u] = row[HEAD_DIM], lp[u] = row[HEAD_DIM + 1];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) op[u][i] = row[min(lane + 64 * i, HEAD_DIM - 1)];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      // past the last partial, or of a chunk with no key of this row: nothing
+      const bool none = p0 + u * MERGE_WAVES >= count || m[u] == neg_inf;
+      const float f = none ? 0.f : __builtin_amdgcn_exp2f(m[u] - top);
+      l += none ? 0.f : f * lp[u];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) o[i] += none ? 0.f : f * op[u][i];
+    }
+  }
+  if (lane == 0) l_of[wave] = l;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (lane + 64 * i < HEAD_DIM) o_of[wave][lane + 64 * i] = o[i];
+  __syncthreads();
+  float total = 0.f;
+#pragma unroll
+  for (int w = 0; w < MERGE_WAVES; ++w) total += l_of[w];
+  const int ti = r / group, d = threadIdx.x;
+  if (d >= HEAD_DIM) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < MERGE_WAVES; ++w) sum += o_of[w][d];
+  Elem<T>::store(out + (size_t)(q0 + ti) * out_stride + (size_t)(g * group + r - ti * group) * HEAD_DIM + d, sum / total);
 }
 
 extern "C" int cwm_attention_quant_head_dim() { return HEAD_DIM; }
@@ -565,7 +649,6 @@ extern "C" int cwm_attention_quant(const void* q, long q_stride, int dtype, void
   } else {                                         \
     CALL_BITS(T, RT, SPLIT, false, WORK, COUNT);   \
   }
-  // float32 queries need three operands for each of theirs: one row tile a wavefront is what its registers hold
   if (n_work > 0) {
     if (dtype == CWM_BF16) {
       CALL_PAGES(bf16_t, 1, true, work, n_work)
@@ -575,15 +658,12 @@ extern "C" int cwm_attention_quant(const void* q, long q_stride, int dtype, void
     if (int status = cwm_launch_status("attention_quant")) return status;
   }
   if (n_work_wide > 0) {
-    if (dtype == CWM_BF16) {
-      CALL_PAGES(bf16_t, 2, false, work_wide, n_work_wide)
-    } else {
-      CALL_PAGES(float, 2, false, work_wide, n_work_wide)
-    }
+    CWM_REQUIRE(dtype == CWM_F32, "attention_quant: bfloat16 portions of many rows read unpacked keys and values");
+    CALL_PAGES(float, 2, false, work_wide, n_work_wide)
     if (int status = cwm_launch_status("attention_quant (rows)")) return status;
   }
   if (n_merge > 0) {
-    const dim3 grid(n_merge, n_kv_heads, 16), block(HEAD_DIM / 4, HEAD_DIM <= 128 ? 8 : 4);
+    const dim3 grid(n_merge, n_kv_heads, 16), block(64 * MERGE_WAVES);
     if (dtype == CWM_BF16)
       hipLaunchKernelGGL((attention_quant_merge_kernel<bf16_t>), grid, block, 0, stream, (bf16_t*)out, out_stride, partial, cu_q, merge, n_q_heads, n_kv_heads);
     else

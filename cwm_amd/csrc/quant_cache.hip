@@ -394,6 +394,91 @@ quant_kv_read_kernel(T* __restrict__ k, T* __restrict__ v, const int* __restrict
   }
 }
 
+// Unpacks keys and values of whole sequences to bfloat16 in the layout of a cache of that type, [pages][2][heads][PAGE * D], keys
+// [slot][D], values [slot / 8][D][8], for an attention of many rows: its blocks would each unpack the same keys (a prompt of 2,048
+// tokens with 6 query heads to a key/value head is 96 blocks a head).  List item: {sequence, first key (a multiple of UNPACK_KEYS),
+// page of the unpacked cache}; grid (items, heads, keys and values).  What a query must not read without a NaN (a key without a page, a
+// value held as NaN) becomes a key of NaN with a value of zeros: a masked score takes no part, where zero times NaN would.
+#define UNPACK_KEYS 64
+template <int G, int BITS>
+__global__ void __launch_bounds__(256)
+quant_unpack_kernel(bf16_t* __restrict__ out, int out_page, const int* __restrict__ list, const uint8_t* __restrict__ cache,
+                    const int* __restrict__ block_table, int table_width, int page_size, int num_pages, const int* __restrict__ kv_len, int n_kv_heads) {
+  constexpr int D = 32 * G;
+  constexpr int UNITS = BITS == 4 ? D / 2 : D;
+  constexpr int H = 1 << (BITS - 1);
+  constexpr int WORDS = BITS / 4;
+  const int* item = list + (size_t)blockIdx.x * 3;
+  const int b = item[0], key0 = item[1], head = blockIdx.y;
+  const int end = kv_len[b];
+  const QuantHead at = quant_head(page_size, D, BITS);
+  const size_t plane = (size_t)n_kv_heads * out_page * D;
+  bf16_t* to = out + (size_t)item[2] * 2 * plane + (size_t)head * out_page * D;
+  const int slot0 = key0 % out_page;
+  auto page_of = [&](int key, int& slot) -> const uint8_t* {  // the head's first byte in the key's page
+    const int lp = key / page_size;
+    slot = key - lp * page_size;
+    const int page = lp < table_width ? block_table[(size_t)b * table_width + lp] : -1;
+    return page >= 0 && page < num_pages ? cache + ((size_t)page * n_kv_heads + head) * at.bytes : nullptr;
+  };
+  if (blockIdx.z == 0) {
+    const int key = key0 + (threadIdx.x >> 2), j = threadIdx.x & 3;
+    if (key >= end) return;
+    int slot;
+    const uint8_t* from = page_of(key, slot);
+    uint32_t codes[G * WORDS] = {}, words[G];
+    bool bad = from == nullptr;
+    if (!bad) {
+      get_words<G * WORDS>((const uint32_t*)from + ((size_t)slot * 4 + j) * G * WORDS, codes);
+      get_words<G>((const uint32_t*)(from + at.key_words) + (size_t)slot * G, words);
+      const float vs = word_step(*(const uint32_t*)(from + at.value_words + (size_t)slot * 4));
+      bad = vs != vs;
+    }
+    bf16_t* row = to + (size_t)(slot0 + (threadIdx.x >> 2)) * D + 8 * j;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float s = bad ? __uint_as_float(0x7fc00000u) : word_step(words[g]), z = bad ? s : word_offset(words[g]);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = BITS == 4 ? (codes[g] >> (4 * (e / 2 + 4 * (e % 2)))) & 15 : (codes[(2 * g + e / 4) % (G * WORDS)] >> (8 * (e & 3))) & 255;
+        x[e] = fmaf(s, (float)(c - H), z);
+      }
+      store8(row + 32 * g, true, x);
+    }
+    return;
+  }
+  for (int i = threadIdx.x; i < UNPACK_KEYS / 8 * UNITS; i += 256) {
+    const int block = i / UNITS, u = i - block * UNITS, key = key0 + 8 * block;
+    if (key >= end) return;
+    int slot;
+    const uint8_t* from = page_of(key, slot);
+    uint2 codes = make_uint2(0, 0);
+    uint32_t words[8] = {};
+    if (from) {
+      codes = *(const uint2*)(from + at.values + ((size_t)(slot >> 3) * UNITS + u) * 8);
+      get_words<8>((const uint32_t*)(from + at.value_words) + slot, words);
+    }
+    float x[BITS == 4 ? 2 : 1][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int place = BITS == 4 ? (e & 4) | ((e & 1) << 1) | ((e >> 1) & 1) : e;
+      const int c = ((place < 4 ? codes.x : codes.y) >> (8 * (place & 3))) & 255;
+      const float s = word_step(words[e]), z = word_offset(words[e]);
+      const bool nan = s != s;
+      if constexpr (BITS == 4) {
+        x[0][e] = nan ? 0.f : fmaf(s, (float)((c & 15) - H), z);
+        x[1][e] = nan ? 0.f : fmaf(s, (float)((c >> 4) - H), z);
+      } else {
+        x[0][e] = nan ? 0.f : fmaf(s, (float)(c - H), z);
+      }
+    }
+    bf16_t* row = to + plane + ((size_t)((slot0 >> 3) + block) * D + (BITS == 4 ? 2 * u : u)) * 8;
+    store8(row, true, x[0]);
+    if constexpr (BITS == 4) store8(row + 8, true, x[BITS == 4 ? 1 : 0]);
+  }
+}
+
 // ---- entry points ------------------------------------------------------------------------ //
 #define FOR_GROUPS(CALL, BITS)                                    switch (head_dim / 32) {                                          case 1: CALL(1, BITS); break;                                   case 2: CALL(2, BITS); break;                                   case 3: CALL(3, BITS); break;                                   case 4: CALL(4, BITS); break;                                   case 5: CALL(5, BITS); break;                                   case 6: CALL(6, BITS); break;                                   case 7: CALL(7, BITS); break;                                   default: CALL(8, BITS); break;                                }
 
@@ -442,4 +527,25 @@ extern "C" int cwm_quant_kv_read(void* k, void* v, int dtype, const int* positio
     FOR_GROUPS(CALL_READ, 8)
   }
   return cwm_launch_status("quant_kv_read");
+}
+
+extern "C" int cwm_quant_unpack_keys() { return UNPACK_KEYS; }
+
+extern "C" int cwm_quant_unpack(void* out, int out_page, const int* list, int n_items, const void* cache, const int* block_table, int table_width,
+                                int page_size, int num_pages, const int* kv_len, int n_kv_heads, int head_dim, int bits, hipStream_t stream) {
+  QUANT_REQUIRE_SIZES("quant_unpack");
+  CWM_REQUIRE(n_items >= 0 && n_kv_heads <= 65535 && out_page > 0 && out_page % UNPACK_KEYS == 0, "quant_unpack: bad sizes");
+  if (n_items == 0) return 0;
+  CWM_REQUIRE(out && list && cache && block_table && kv_len, "quant_unpack: a tensor is missing");
+  CWM_REQUIRE((uintptr_t)cache % 16 == 0 && (uintptr_t)out % 16 == 0, "quant_unpack: tensors must be 16-byte aligned");
+  const dim3 grid(n_items, n_kv_heads, 2);
+#define CALL_UNPACK(G, BITS)                                                                                                                   \
+  hipLaunchKernelGGL((quant_unpack_kernel<G, BITS>), grid, dim3(256), 0, stream, (bf16_t*)out, out_page, list, (const uint8_t*)cache, block_table, \
+                     table_width, page_size, num_pages, kv_len, n_kv_heads)
+  if (bits == 4) {
+    FOR_GROUPS(CALL_UNPACK, 4)
+  } else {
+    FOR_GROUPS(CALL_UNPACK, 8)
+  }
+  return cwm_launch_status("quant_unpack");
 }

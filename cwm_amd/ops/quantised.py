@@ -9,6 +9,7 @@ import ctypes
 import functools
 from typing import Optional, Tuple
 
+import numpy as np
 import torch
 
 from . import build as _build
@@ -23,6 +24,10 @@ _ARGTYPES = {
     "cwm_quant_kv_write": (_P, _L, _P, _L, _P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P),
     "cwm_quant_kv_read": (_P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P),
     "cwm_attention_quant": (_P, _L, _I, _P, _L, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P),
+    "cwm_quant_unpack": (_P, _I, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _I, _P),
+    "cwm_attention_mfma": (
+        _P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P, _P, _I, _P,
+    ),
     "cwm_quantize_rows": (_P, _L, _I, _P, _L, _P, _I, _I, _I, _P),
     "cwm_linear_int8": (_P, _L, _I, _P, _P, _P, _L, _P, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P),
 }
@@ -34,7 +39,7 @@ def _entry(library: str, name: str, head_dim: Optional[int] = None):
     found = _entries.get((name, head_dim))
     if found is None:
         lib = _build.load(library, None if head_dim is None else {"HEAD_DIM": head_dim})
-        function = getattr(lib, name)
+        function = lib[name]  # an object of its own: other callers of the library hand in objects of ctypes
         function.argtypes = _ARGTYPES[name]
         found = _entries[(name, head_dim)] = (function, lib)
     return found
@@ -218,6 +223,38 @@ def quant_kv_read(
     return k, v
 
 
+UNPACK_KEYS = 64  # csrc/quant_cache.hip
+UNPACK_PAGE = 256  # tokens of a page of the unpacked cache
+
+
+def _unpack_list(batch, group: int, window: Optional[int], device: torch.device):
+    """The work of unpacking the sequences of a step that have blocks of many rows: the list of `cwm_quant_unpack` and the block table of
+    the unpacked cache in one device vector, the items, the table's width and the pages; made once a step."""
+    key = ("quant_unpack", group, window)
+    held = batch.scratch.get(key)
+    if held is None:
+        from .attention_plan import ROWS_PER_TILE, SPLIT_MAX_TILES, first_keys
+
+        width = max(-(-n // UNPACK_PAGE) for n in batch.kv_lens)
+        table = np.full((len(batch.kv_lens), width), -1, dtype=np.int32)
+        items, pages = [], 0
+        for b, (m, n) in enumerate(zip(batch.q_lens, batch.kv_lens)):
+            if -(-m * group // ROWS_PER_TILE) <= SPLIT_MAX_TILES:
+                continue
+            first = int(first_keys(n - m, window, None))
+            lo = first // UNPACK_PAGE
+            count = -(-n // UNPACK_PAGE) - lo
+            table[b, lo : lo + count] = np.arange(pages, pages + count)
+            keys = np.arange(first // UNPACK_KEYS * UNPACK_KEYS, n, UNPACK_KEYS)
+            items.append(np.stack([np.full_like(keys, b), keys, pages + keys // UNPACK_PAGE - lo], axis=1))
+            pages += count
+        rows = np.concatenate(items).astype(np.int32)
+        host = torch.from_numpy(np.concatenate([rows.reshape(-1), table.reshape(-1)]))
+        dev = host.pin_memory().to(device, non_blocking=True)
+        held = batch.scratch[key] = (dev, rows.shape[0], width, pages)
+    return held
+
+
 def quant_paged_attention(
     q: torch.Tensor,
     cache: torch.Tensor,
@@ -231,7 +268,7 @@ def quant_paged_attention(
     call: `q` [T, Hq, hd] (float32 or bfloat16, rotated), `batch` the step's `StepBatch`, `window` the keys a query reads, its
     own included (None: all).  Returns [T, Hq * hd] in q's type.  A query one of whose keys has no page gets NaN."""
     KernelError, _check, _code = _base()
-    from . import _attention_plan, _check_mask
+    from . import _attention_plan, _check_mask, _half_blocks_built, _three_blocks_a_unit
 
     _check_device(q, cache, block_table, batch.cu_q, batch.kv_len)
     _check_mask(window, None, None)
@@ -254,19 +291,45 @@ def quant_paged_attention(
     out = torch.empty((n_tokens, n_q * hd), dtype=dtype, device=q.device)
     if n_tokens == 0:
         return out
-    plan = _attention_plan(batch, n_q // n_kv, n_kv, hd, window, q.device)
-    partial = None
+    group = n_q // n_kv
+    # bfloat16 queries of many rows: their keys and values are unpacked once and read by the attention over a bfloat16 cache
+    plan = _attention_plan(batch, group, n_kv, hd, window, q.device, None, dtype == torch.bfloat16 and _half_blocks_built(n_kv, hd, UNPACK_PAGE))
+    unpacks = plan.n_wide > 0 and dtype == torch.bfloat16
+    partials = partial = None
     if plan.n_partials:
-        partial = torch.empty(plan.n_partials * n_kv * 16 * (hd + 4), dtype=torch.float32, device=q.device)
-    function, lib = _entry("attention_quant", "cwm_attention_quant", hd)
-    status = function(
-        q.data_ptr(), token, code, out.data_ptr(), n_q * hd, cache.data_ptr(), block_table.data_ptr(), block_table.shape[1],
-        batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), plan.work.data_ptr(), plan.n_work, plan.wide.data_ptr(), plan.n_wide, plan.item_tiles,
-        plan.merge.data_ptr(), plan.n_merge, None if partial is None else partial.data_ptr(), n_q, n_kv, hd, page_size, pages,
-        -1 if window is None else window - 1, scale, bits, _stream(),
+        partials = torch.empty(plan.n_partials * n_kv * 16 * (hd + 4), dtype=torch.float32, device=q.device)  # held until the last launch
+        partial = partials.data_ptr()
+    table, width = block_table.data_ptr(), block_table.shape[1]
+    first, lengths, work, wide, merge, stream = (
+        batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), plan.work.data_ptr(), plan.wide.data_ptr(), plan.merge.data_ptr(), _stream()
     )
-    if status:
-        _check(lib, status)
+    if plan.n_work or not unpacks:
+        function, lib = _entry("attention_quant", "cwm_attention_quant", hd)
+        status = function(
+            q.data_ptr(), token, code, out.data_ptr(), n_q * hd, cache.data_ptr(), table, width, first, lengths, work, plan.n_work, wide,
+            0 if unpacks else plan.n_wide, plan.item_tiles, merge, 0 if unpacks else plan.n_merge, partial, n_q, n_kv, hd, page_size, pages,
+            -1 if window is None else window - 1, scale, bits, stream,
+        )
+        if status:
+            _check(lib, status)
+    if unpacks:
+        listed, n_items, wide_width, n_pages = _unpack_list(batch, group, window, q.device)
+        unpacked = torch.empty((n_pages, 2, n_kv, UNPACK_PAGE * hd), dtype=dtype, device=q.device)
+        function, lib = _entry("quant_cache", "cwm_quant_unpack")
+        status = function(
+            unpacked.data_ptr(), UNPACK_PAGE, listed.data_ptr(), n_items, cache.data_ptr(), table, width, page_size, pages, lengths, n_kv, hd, bits, stream,
+        )
+        if status:
+            _check(lib, status)
+        function, lib = _entry("attention_mfma", "cwm_attention_mfma", hd)
+        status = function(
+            q.data_ptr(), token, out.data_ptr(), n_q * hd, unpacked.data_ptr(), listed.data_ptr() + 12 * n_items, wide_width, first, lengths,
+            work, 0, 0, wide, plan.n_wide, plan.item_tiles, _three_blocks_a_unit(plan.n_wide * n_kv, plan.wide_shape, q.device),
+            merge, plan.n_merge, plan.n_merge_mid, plan.n_merge_wide, partial, n_q, n_kv, hd, UNPACK_PAGE, n_pages,
+            -1 if window is None else window - 1, 0, scale, 0.0, None, None, None, None, 0, stream,
+        )
+        if status:
+            _check(lib, status)
     return out
 
 

@@ -171,7 +171,9 @@ def attention(step, q, keys, values, bits, window, scale):
     s (143 + 136) |q| and |z| |q| with an offset of the codes (bfloat16 queries, 4 bits; 8 bits: 255 + 128), s 2 H |q| without.
     A score that is off by d moves the result by at most 2 d sum p |v|.  bfloat16: the weights p s are rounded to half a step
     and multiply codes less H, and the result is rounded; the sums with the codes' offset, s (OFF' + c), are float32 sums of one
-    term for 32 keys."""
+    term for 32 keys.  bfloat16 portions of more than 128 rows read keys and values unpacked to bfloat16: a score is off by the
+    sum of dim independent roundings of up to half a step, 2^-8 |q k| each, whose deviation is that over sqrt(3) (six of them are
+    allowed), and a value by half a step; the weights p are rounded and multiply whole values."""
     T, heads_q, dim = q.shape
     heads = keys[0].shape[1]
     group = heads_q // heads
@@ -200,7 +202,11 @@ def attention(step, q, keys, values, bits, window, scale):
                 off = 2.0 * 2.0 ** -24 * (dim + 40) * scale * torch.where(seen, size, torch.zeros_like(size)).amax(1)
                 spread = p @ (sv[:, None] * reach + zv[:, None].abs())
                 err = 2 * off[:, None] * (p @ v.abs()) + 2.0 * 2.0 ** -24 * (n / 32 + 40) * spread
-                if not fine:
+                if not fine and m * group > 128:
+                    off = off + 6 / 3 ** 0.5 * HALF_STEP[q.dtype] * scale * torch.where(seen, (x * x) @ (k * k).t(), torch.zeros_like(size)).sqrt().amax(1)
+                    err = 2 * off[:, None] * (p @ v.abs()) + 2.0 * 2.0 ** -24 * (n / 32 + 40) * spread
+                    err = err + 2.01 * HALF_STEP[q.dtype] * (p @ v.abs()) + HALF_STEP[q.dtype] * o.abs() * 1.01
+                elif not fine:
                     err = err + HALF_STEP[q.dtype] * (p @ (sv[:, None] * (cv - half).abs().double())) + HALF_STEP[q.dtype] * o.abs() * 1.01
                 else:
                     err = err + 2.0 ** -23 * o.abs()

@@ -239,6 +239,31 @@ def test_a_key_that_is_not_finite_reaches_its_readers_only():
     assert torch.equal(bad, want) and torch.isfinite(got[~want.to(DEV)]).all()
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+def test_portions_of_many_rows_and_what_is_not_finite(bits):
+    """Portions whose keys are unpacked first: a window that has passed pages, pages of 24 and of 512 tokens, a key and a value that are
+    not finite, and a page that is missing, beside decoded tokens."""
+    for page in (24, 512):
+        dim, group, heads, window = 64, 4, 2, 300
+        new, kv = [100, 1, 200], [1500, 40, 200]
+        step, cache, q, keys, values = _case(new, kv, page, group * heads, heads, dim, bits, torch.bfloat16, window, 31 + page)
+        for lp in range((1400 - window + 1) // page):
+            step.table[0, lp] = -1  # given back: the window has passed them
+        _close(_attend(step, cache, q, bits, window, 0.125), step, q, keys, values, bits, window, 0.125)
+        keys[0][1440, 0, 40], values[2][150, 1, 7] = math.inf, math.nan
+        for b, key in ((0, 1440), (2, 150)):
+            place = step.table[b, key // page].long().reshape(1), torch.tensor([key % page])
+            held.put_tokens(cache, *place, keys[b][key : key + 1], values[b][key : key + 1], bits)
+        got = torch.isnan(_attend(step, cache, q, bits, window, 0.125)).reshape(301, 2, group, dim).all(-1).all(-1).cpu()
+        want = torch.zeros(301, 2, dtype=torch.bool)
+        want[40:100, 0] = True  # the tokens at 1440 .. 1499
+        want[101 + 150 :, 1] = True
+        assert torch.equal(got, want)
+    step.table[2, 0] = 10 ** 6
+    got = torch.isnan(_attend(step, cache, q, bits, window, 0.125)).all(-1)
+    assert got[101:].all() and not got[:40].any()
+
+
 def test_a_missing_page_is_seen():
     new, kv, dim, bits = [1, 1], [60, 60], 64, 4
     step, cache, q, keys, values = _case(new, kv, 16, 4, 2, dim, bits, torch.bfloat16, 20, 12)
