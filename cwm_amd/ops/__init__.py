@@ -1146,24 +1146,24 @@ class StaticPlans:
     def __init__(self, device: torch.device, max_keys: int) -> None:
         self.device = device
         self.max_keys = max_keys  # the most keys a sequence may hold while the capture is in use
-        self.homes: dict = {}  # (group, key/value heads, window, chunk, whether keys are cut finer) -> (capacity, device vector, uploaded plan)
+        self.homes: dict = {}  # (group, key/value heads, window, chunk, whether keys are cut finer, whether they are packed) -> (capacity, device vector, uploaded plan)
 
-    def _padded(self, batch, group: int, n_kv: int, window: Optional[int], capacity, chunk: Optional[int], finer: bool):
+    def _padded(self, batch, group: int, n_kv: int, window: Optional[int], capacity, chunk: Optional[int], finer: bool, packed: bool):
         from .attention_plan import build_plan, capacity_until, pad_plan
 
         wide_cut_below = -(-2 * _compute_units(self.device) // n_kv)
         if capacity is None:
-            plan, capacity = capacity_until(batch.q_lens, batch.kv_lens, group, window, wide_cut_below, self.max_keys, chunk, finer)
+            plan, capacity = capacity_until(batch.q_lens, batch.kv_lens, group, window, wide_cut_below, self.max_keys, chunk, finer, packed)
         else:
-            plan = build_plan(batch.q_lens, batch.kv_lens, group, window, wide_cut_below, chunk, finer)
+            plan = build_plan(batch.q_lens, batch.kv_lens, group, window, wide_cut_below, chunk, finer, packed=packed)
         flat = pad_plan(plan, capacity)
         return plan, capacity, flat
 
-    def plan(self, batch, group: int, n_kv: int, window: Optional[int], chunk: Optional[int], finer: bool) -> "_UploadedPlan":
-        key = (group, n_kv, window, chunk, finer)
+    def plan(self, batch, group: int, n_kv: int, window: Optional[int], chunk: Optional[int], finer: bool, packed: bool = False) -> "_UploadedPlan":
+        key = (group, n_kv, window, chunk, finer, packed)
         home = self.homes.get(key)
         if home is None:
-            plan, capacity, flat = self._padded(batch, group, n_kv, window, None, chunk, finer)
+            plan, capacity, flat = self._padded(batch, group, n_kv, window, None, chunk, finer, packed)
             if flat is None:
                 raise KernelError("this step's attention work has items that a captured step does not take")
             dev = torch.from_numpy(flat).pin_memory().to(self.device, non_blocking=True)
@@ -1178,8 +1178,8 @@ class StaticPlans:
 
     def refresh(self, batch) -> bool:
         """Fill every home with the lists of `batch`; False if one of them has outgrown its home."""
-        for (group, n_kv, window, chunk, finer), (capacity, dev, _) in self.homes.items():
-            _, _, flat = self._padded(batch, group, n_kv, window, capacity, chunk, finer)
+        for (group, n_kv, window, chunk, finer, packed), (capacity, dev, _) in self.homes.items():
+            _, _, flat = self._padded(batch, group, n_kv, window, capacity, chunk, finer, packed)
             if flat is None:
                 return False
             dev.copy_(torch.from_numpy(flat).pin_memory(), non_blocking=True)
@@ -1188,25 +1188,26 @@ class StaticPlans:
 
 def _attention_plan(
     batch, group: int, n_kv: int, head_dim: int, window: Optional[int], device: torch.device, chunk: Optional[int] = None, halves: bool = False,
+    packed: bool = False,
 ) -> _UploadedPlan:
     """The step's work list for this (group size, key/value heads and their size, window or block of keys), uploaded once per step.
-    `halves`: whether blocks of 64 rows are built for what the layer has (`_half_blocks_built`)."""
+    `halves`: whether blocks of 64 rows are built for what the layer has (`_half_blocks_built`).  `packed`: whether its cache holds 4 or 8 bits."""
     from .attention_plan import build_plan, cuts_finer, wide_item_tiles
 
     finer = cuts_finer(n_kv, head_dim)
     static = getattr(batch, "static", None)
     if static is not None:
-        return static.plan(batch, group, n_kv, window, chunk, finer)
+        return static.plan(batch, group, n_kv, window, chunk, finer, packed)
     # with such blocks the list depends on the head size, by which they are chosen; layers of other sizes have lists of their own
-    key = ("attention_plan", group, n_kv, window, chunk, finer, head_dim if halves else None)
+    key = ("attention_plan", group, n_kv, window, chunk, finer, head_dim if halves else None, packed)
     cached = batch.scratch.get(key)
     if cached is None:
         # a sequence whose blocks of 128 rows, over all key/value heads, would not give every compute unit two
         wide_cut_below = -(-2 * _compute_units(device) // n_kv) if device.type == "cuda" else 0
         item_tiles = WIDE_TILES
         if device.type == "cuda" and halves:
-            item_tiles = wide_item_tiles(batch.q_lens, batch.kv_lens, group, n_kv, head_dim, wide_cut_below, _compute_units(device))
-        plan = build_plan(batch.q_lens, batch.kv_lens, group, window, wide_cut_below, chunk, finer, item_tiles)
+            item_tiles = wide_item_tiles(batch.q_lens, batch.kv_lens, group, n_kv, head_dim, wide_cut_below, _compute_units(device), packed)
+        plan = build_plan(batch.q_lens, batch.kv_lens, group, window, wide_cut_below, chunk, finer, item_tiles, packed)
         flat = np.concatenate([plan.work.reshape(-1), plan.work_wide.reshape(-1), plan.merge.reshape(-1)]).astype(np.int32)
         host = torch.from_numpy(flat)
         if device.type == "cuda":

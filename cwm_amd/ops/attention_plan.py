@@ -20,6 +20,10 @@ SPLIT_MAX_TILES = 8  # sequences with more row tiles than this are not split
 WIDE_TILES = 8  # row tiles (128 rows) of one block of the kernel that shares keys and values through LDS
 WIDE_CHUNK = 8192  # keys after which such a block's range is cut (at fixed absolute positions, like the others)
 WIDE_CHUNK_FINE = 2048  # the same for a sequence with very few such blocks
+# Both, for a step whose cache holds 4 or 8 bits (`packed`).  us with 8,192 and 2,048 keys / 1,024 (32 query heads on 8 of 128): 513 tokens to
+# 3,585 keys 96 / 74, 100 to 6,000 96 / 58, 64 to 30,000 95 / 87, 300 to 1,300, 2,300, 300 and 800 65 / 65; chunks of 512 make the
+# last but one 117.
+PACKED_WIDE_CHUNK = 1024
 # Most blocks of WIDE_TILES row tiles a compute unit, by the head size, of a launch that takes half as high ones instead.  Such a
 # block walks its keys alone, so with few blocks the longest one's walk is the launch: a tile of 32 keys costs it 1.4 us with 128
 # rows and 0.9 with 64, and twice as many blocks read keys from LDS.  Blocks of 128 rows, us with them and with 64 rows: heads of
@@ -28,7 +32,7 @@ WIDE_CHUNK_FINE = 2048  # the same for a sequence with very few such blocks
 WIDE_HALF_BLOCKS = {64: 3.75, 128: 2.7, 256: float("inf")}
 
 
-def chunk_keys(n_keys, few_heads: bool = False):
+def chunk_keys(n_keys, few_heads: bool = False, packed: bool = False):
     """Keys per chunk (a multiple of 128: four wavefronts take a chunk's tiles of 32 keys in turn) for a row tile
     that reads `n_keys` keys (a number or an array of them).  Up to 2,048 keys are not cut: a block of four
     wavefronts reads them and leaves no partial result (64 sequences of 1,024 keys: 45 us a layer of the 32B
@@ -36,8 +40,13 @@ def chunk_keys(n_keys, few_heads: bool = False):
     in chunks of 256).  Longer ranges are cut so that a few sequences still spread over the chip: 512 keys up
     to 8,192 (eight sequences in a window of 8,192 keys: 54 us against 58 us in chunks of 1,024), 1,024 up to
     65,536, then 2,048 (eight sequences of 131,072 keys: 647 us against 665 us in chunks of 4,096).
-    `few_heads` (see `cuts_finer`): chunks of 256 keys, of 512 beyond 8,192 and 1,024 beyond 65,536 keys."""
+    `few_heads` (see `cuts_finer`): chunks of 256 keys, of 512 beyond 8,192 and 1,024 beyond 65,536 keys.
+    `packed`: a cache of 4 or 8 bits, whose keys are fewer bytes and no less work before and after a block's loop: 1,024
+    up to 8,192 keys, then 2,048 (48 query heads on 8 of 128 and 4 bits, us in chunks of 512 / 1,024 / 2,048 / 4,096: eight sequences of
+    32,768 keys 95 / 74 / 63 / 59, one 18 / 18 / 21 / 32, eight of 8,192 28 / 23 / 23 / 34, 32 of 4,096 50 / 40 / 35 / 33)."""
     n = np.asarray(n_keys)
+    if packed:
+        return np.where(n <= 2048, 2048, np.where(n <= 8192, 1024, 2048))
     if few_heads:
         return np.where(n <= 8192, 256, np.where(n <= 65536, 512, 1024))
     return np.where(n <= 2048, 2048, np.where(n <= 8192, 512, np.where(n <= 65536, 1024, 2048)))
@@ -82,13 +91,15 @@ def first_keys(last_key, window: Optional[int], chunk: Optional[int]):
 
 def build_plan(
     q_lens: Sequence[int], kv_lens: Sequence[int], group: int, window: Optional[int], wide_cut_below: int = 0,
-    chunk: Optional[int] = None, few_heads: bool = False, wide_tiles: int = WIDE_TILES,
+    chunk: Optional[int] = None, few_heads: bool = False, wide_tiles: int = WIDE_TILES, packed: bool = False,
 ) -> AttentionPlan:
     """`window` or `chunk` (at most one): which keys a query reads, see `first_keys`.  `wide_cut_below`: a sequence with fewer wide items than this has their keys cut at multiples of
     WIDE_CHUNK (its blocks alone would leave compute units idle), with fewer than an eighth of it at
     multiples of WIDE_CHUNK_FINE; the caller derives the number from the model's heads and the chip,
     so that it is the same whatever else the batch holds.  `few_heads`: see `chunk_keys`.  `wide_tiles`: row tiles of a wide
-    item, WIDE_TILES or what `wide_item_tiles` answers (a sequence's items are counted in the former where that decides on a cut)."""
+    item, WIDE_TILES or what `wide_item_tiles` answers (a sequence's items are counted in the former where that decides on a cut).
+    `packed`: the step's cache holds 4 or 8 bits, see `chunk_keys` and PACKED_WIDE_CHUNK."""
+    wide_chunk, wide_chunk_fine = wide_chunks(packed)
     q = np.asarray(q_lens, dtype=np.int64)
     kv = np.asarray(kv_lens, dtype=np.int64)
     n_rows = q * group
@@ -108,7 +119,7 @@ def build_plan(
         wide_lo.append(lo[first])
         wide_hi.append(hi[last])
         wide_n_tiles.append(last - first + 1)
-        wide_cut.append(np.full(n_items, 0 if n_wide >= wide_cut_below else (WIDE_CHUNK if 8 * n_wide >= wide_cut_below else WIDE_CHUNK_FINE)))
+        wide_cut.append(np.full(n_items, 0 if n_wide >= wide_cut_below else (wide_chunk if 8 * n_wide >= wide_cut_below else wide_chunk_fine)))
 
     # ---- all tiles of the other sequences at once, in the order (sequence, tile, chunk)
     small = np.nonzero(~is_wide)[0]
@@ -122,7 +133,7 @@ def build_plan(
     last_tok = np.minimum(row0 + ROWS_PER_TILE - 1, n_rows[seq] - 1) // group
     hi = n_old + last_tok + 1  # exclusive
     lo = first_keys(n_old + first_tok, window, chunk)
-    cut = chunk_keys(hi - lo, few_heads)
+    cut = chunk_keys(hi - lo, few_heads, packed)
     c0 = lo // cut
     n_chunks = (hi - 1) // cut - c0 + 1
     split = n_chunks > 1
@@ -197,18 +208,26 @@ def build_plan(
     )
 
 
-def wide_item_tiles(q_lens: Sequence[int], kv_lens: Sequence[int], group: int, n_kv: int, head_dim: int, wide_cut_below: int, units: int) -> int:
+def wide_chunks(packed: bool) -> "tuple[int, int]":
+    """Keys after which a block of many rows is cut where its sequence has few such blocks, and where it has very few."""
+    return (PACKED_WIDE_CHUNK, PACKED_WIDE_CHUNK) if packed else (WIDE_CHUNK, WIDE_CHUNK_FINE)
+
+
+def wide_item_tiles(
+    q_lens: Sequence[int], kv_lens: Sequence[int], group: int, n_kv: int, head_dim: int, wide_cut_below: int, units: int, packed: bool = False
+) -> int:
     """Row tiles of a wide item for a step of these lengths on `units` compute units: half of WIDE_TILES where blocks of
     WIDE_TILES are few (`WIDE_HALF_BLOCKS`; other head sizes have no such blocks).  A row's bits are the same either way unless
     its keys are cut, so a step with a cut sequence keeps the whole size, or first keys are kept beside a window, for which the
     caller does not ask."""
     blocks, most = 0, WIDE_HALF_BLOCKS.get(head_dim, 0) * units
+    wide_chunk, wide_chunk_fine = wide_chunks(packed)
     for q, kv in zip(q_lens, kv_lens):
         n_tiles = -(-q * group // ROWS_PER_TILE)
         if n_tiles <= SPLIT_MAX_TILES:
             continue
         n_wide = -(-n_tiles // WIDE_TILES)
-        if n_wide < wide_cut_below and kv > (WIDE_CHUNK if 8 * n_wide >= wide_cut_below else WIDE_CHUNK_FINE):
+        if n_wide < wide_cut_below and kv > (wide_chunk if 8 * n_wide >= wide_cut_below else wide_chunk_fine):
             return WIDE_TILES
         blocks += n_wide * n_kv
     return WIDE_TILES // 2 if 0 < blocks <= most else WIDE_TILES
@@ -270,17 +289,17 @@ CHUNK_RULE_ENDS = (2048, 8192, 65536)
 
 def capacity_until(
     q_lens: Sequence[int], kv_lens: Sequence[int], group: int, window: Optional[int], wide_cut_below: int, max_keys: int,
-    chunk: Optional[int] = None, few_heads: bool = False,
+    chunk: Optional[int] = None, few_heads: bool = False, packed: bool = False,
 ) -> "tuple[AttentionPlan, PlanCapacity]":
     """The step's plan, and the sizes of its lists for as long as no sequence holds more than `max_keys` keys
     (every sequence growing by a token a step): the sequences as they are, all of them grown to `max_keys`, and
     grown to each length in between at which the rule for cutting the keys changes."""
-    plan = build_plan(q_lens, kv_lens, group, window, wide_cut_below, chunk, few_heads)
+    plan = build_plan(q_lens, kv_lens, group, window, wide_cut_below, chunk, few_heads, packed=packed)
     plans = [plan]
     for length in sorted({max_keys, *(n + d for n in CHUNK_RULE_ENDS for d in (0, 1) if n + d < max_keys)}):
         grown = [min(max(kv, length), max(kv, max_keys)) for kv in kv_lens]
         if grown != list(kv_lens):
-            plans.append(build_plan(q_lens, grown, group, window, wide_cut_below, chunk, few_heads))
+            plans.append(build_plan(q_lens, grown, group, window, wide_cut_below, chunk, few_heads, packed=packed))
     capacity = PlanCapacity.covering(plans)
     span = window if chunk is None else chunk
     if span is not None and max(max(kv_lens), max_keys) > span:
@@ -290,7 +309,7 @@ def capacity_until(
         # Where a range of the window's length may be cut into more than MERGE_MID_MAX parts, one cut more or less moves a tile
         # from one list of merges to the other (a window of 8,192 keys in chunks of 256: 32 parts from an aligned start, else 33).
         tiles = int((plan.work[:, 4] < 0).sum()) + plan.merge.shape[0]
-        most_parts = (span - 2) // int(chunk_keys(span, few_heads)) + 2
+        most_parts = (span - 2) // int(chunk_keys(span, few_heads, packed)) + 2
         capacity = PlanCapacity(
             work=capacity.work + tiles,
             merge_many=max(capacity.merge_many, tiles if most_parts > MERGE_MID_MAX else 0),

@@ -293,7 +293,7 @@ def quant_paged_attention(
         return out
     group = n_q // n_kv
     # bfloat16 queries of many rows: their keys and values are unpacked once and read by the attention over a bfloat16 cache
-    plan = _attention_plan(batch, group, n_kv, hd, window, q.device, None, dtype == torch.bfloat16 and _half_blocks_built(n_kv, hd, UNPACK_PAGE))
+    plan = _attention_plan(batch, group, n_kv, hd, window, q.device, None, dtype == torch.bfloat16 and _half_blocks_built(n_kv, hd, UNPACK_PAGE), packed=True)
     unpacks = plan.n_wide > 0 and dtype == torch.bfloat16
     partials = partial = None
     if plan.n_partials:
