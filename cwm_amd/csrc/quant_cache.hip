@@ -301,95 +301,110 @@ quant_kv_write_kernel(const T* __restrict__ k, long k_stride, const T* __restric
   if (j == 0) put_words<G>((uint32_t*)(to + at.key_words) + (size_t)p.slot * G, words);
 }
 
-// Reads the tokens of a list: grid (chunks of eight tokens, groups of eight heads: keys, then values), blocks as above.
+// Reads the tokens of a list: grid (chunks of eight tokens, groups of eight heads: keys, then values).  Bound by memory, most of it the
+// written rows: neighbouring lanes write neighbouring pieces, whole cache lines an instruction.
 template <typename T, int G, int BITS>
 __global__ void __launch_bounds__(256)
 quant_kv_read_kernel(T* __restrict__ k, T* __restrict__ v, const int* __restrict__ positions, const int* __restrict__ seq_of_token,
                      const uint8_t* __restrict__ cache, const int* __restrict__ block_table, int n_seqs, int table_width, int page_size,
                      int num_pages, int n_tokens, int n_kv_heads, int kv_groups) {
   constexpr int D = 32 * G;
-  constexpr int UNITS = BITS == 4 ? D / 2 : D;
   constexpr int H = 1 << (BITS - 1);
   constexpr int WORDS = BITS / 4;
+  __shared__ const uint8_t* src_page[CHUNK];
+  __shared__ int src_slot[CHUNK];
+  __shared__ uint32_t value_words[HEADS_A_BLOCK][CHUNK];
   const int t0 = blockIdx.x * CHUNK;
   const bool values = blockIdx.y >= kv_groups;
   const int head0 = (blockIdx.y - (values ? kv_groups : 0)) * HEADS_A_BLOCK;
+  const int heads = min(HEADS_A_BLOCK, n_kv_heads - head0);
   const int tid = threadIdx.x;
+  const int last = min(CHUNK, n_tokens - t0) - 1;
   const QuantHead at = quant_head(page_size, D, BITS);
+  if (tid < HEADS_A_BLOCK * CHUNK) {
+    const int tk = tid & 7, hb = tid >> 3;
+    Place p = {nullptr, 0};
+    if (tk <= last)
+      p = place_of((uint8_t*)cache, at.bytes * n_kv_heads, positions[t0 + tk], seq_of_token[t0 + tk], block_table, n_seqs, table_width, page_size, num_pages);
+    if (hb == 0) {
+      src_page[tk] = p.page;
+      src_slot[tk] = p.slot;
+    }
+    // a token without a page reads as zeros
+    if (values && hb < heads) value_words[hb][tk] = p.page ? *(const uint32_t*)(p.page + (size_t)(head0 + hb) * at.bytes + at.value_words + (size_t)p.slot * 4) : 0u;
+  }
+  __syncthreads();
 
   if (!values) {
-    const int t = t0 + ((tid >> 2) & 7), j = tid & 3, head = head0 + (tid >> 5);
-    if (t >= n_tokens || head >= n_kv_heads) return;
-    const Place p = place_of((uint8_t*)cache, at.bytes * n_kv_heads, positions[t], seq_of_token[t], block_table, n_seqs, table_width, page_size, num_pages);
-    uint32_t codes[G * WORDS] = {}, words[G] = {};  // a token without a page reads as zeros
-    if (p.page) {
-      const uint8_t* from = p.page + (size_t)head * at.bytes;
-      get_words<G * WORDS>((const uint32_t*)from + ((size_t)p.slot * 4 + j) * G * WORDS, codes);
-      get_words<G>((const uint32_t*)(from + at.key_words) + (size_t)p.slot * G, words);
-    }
-    T* out = k + ((size_t)t * n_kv_heads + head) * D + 8 * j;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float s = word_step(words[g]), z = word_offset(words[g]);
+    constexpr int PIECES = D / 8;  // of a token's key; piece 4 g + j holds the codes [j][g]
+    for (int i = tid; i < (last + 1) * heads * PIECES; i += blockDim.x) {
+      const int piece = i % PIECES, th = i / PIECES, tk = th / heads, head = head0 + th - tk * heads;
+      const int g = piece >> 2, j = piece & 3;
+      const uint8_t* page = src_page[tk];
+      uint32_t codes[WORDS] = {}, word = 0;
+      if (page) {
+        const uint8_t* from = page + (size_t)head * at.bytes;
+        get_words<WORDS>((const uint32_t*)from + (((size_t)src_slot[tk] * 4 + j) * G + g) * WORDS, codes);
+        word = *(const uint32_t*)(from + at.key_words + ((size_t)src_slot[tk] * G + g) * 4);
+      }
+      const float s = word_step(word), z = word_offset(word);
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int c = BITS == 4 ? (codes[g] >> (4 * (e / 2 + 4 * (e % 2)))) & 15 : (codes[(2 * g + e / 4) % (G * WORDS)] >> (8 * (e & 3))) & 255;
+        const int c = BITS == 4 ? (codes[0] >> (4 * (e / 2 + 4 * (e % 2)))) & 15 : (codes[e / 4 % WORDS] >> (8 * (e & 3))) & 255;
         x[e] = fmaf(s, (float)(c - H), z);
       }
-      store8(out + 32 * g, true, x);
+      store8(k + ((size_t)(t0 + tk) * n_kv_heads + head) * D + 8 * piece, true, x);
     }
     return;
   }
 
-  __shared__ const uint8_t* src_page[CHUNK];
-  __shared__ int src_slot[CHUNK];
-  if (tid < CHUNK) {
-    Place p = {nullptr, 0};
-    if (t0 + tid < n_tokens)
-      p = place_of((uint8_t*)cache, at.bytes * n_kv_heads, positions[t0 + tid], seq_of_token[t0 + tid], block_table, n_seqs, table_width, page_size, num_pages);
-    src_page[tid] = p.page;
-    src_slot[tid] = p.slot;
-  }
-  __syncthreads();
-  // Tokens that follow one another lie in at most two value blocks, of which a thread reads its eight bytes each.
-  const int lead = src_slot[0] & 7, last = min(CHUNK, n_tokens - t0) - 1, second = min(8 - lead, last);
+  // Tokens that follow one another lie in at most two value blocks, of which a thread reads its sixteen bytes each.
+  const int lead = src_slot[0] & 7, second = min(8 - lead, last);
   bool run = src_page[0] != nullptr && src_page[second] != nullptr;
   for (int i = 1; i <= last; ++i) {
     const int first = i < 8 - lead ? 0 : second;
     run = run && src_page[i] == src_page[first] && src_slot[i] == src_slot[first] + i - first;
   }
   run = run && (second < 8 - lead || (src_slot[second] & 7) == 0);
-  const int units = min(HEADS_A_BLOCK, n_kv_heads - head0) * UNITS;
-  for (int i = tid; i < units; i += blockDim.x) {
+  constexpr int DIMS = BITS == 4 ? 4 : 2;  // of a thread: sixteen bytes of a value block
+  constexpr int UNITS = D / DIMS;
+  for (int i = tid; i < heads * UNITS; i += blockDim.x) {
     const int hb = i / UNITS, u = i - hb * UNITS, head = head0 + hb;
-    const size_t unit = (size_t)head * at.bytes + at.values + (size_t)u * 8;
-    unsigned long long a = 0, b = 0;
+    const size_t unit = (size_t)head * at.bytes + at.values + (size_t)u * 16;
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
     if (run) {
-      a = *(const unsigned long long*)(src_page[0] + unit + (size_t)(src_slot[0] >> 3) * UNITS * 8);
-      b = *(const unsigned long long*)(src_page[second] + unit + (size_t)(src_slot[second] >> 3) * UNITS * 8);
+      a = b = *(const uint4*)(src_page[0] + unit + (size_t)(src_slot[0] >> 3) * (D * BITS));
+      if (lead) b = *(const uint4*)(src_page[second] + unit + (size_t)(src_slot[second] >> 3) * (D * BITS));
     }
 #pragma unroll
     for (int e = 0; e < CHUNK; ++e) {
       if (e > last) break;
       const uint8_t* page = src_page[e];
       const int slot = src_slot[e], place = BITS == 4 ? quant_place(slot & 7) : slot & 7;
-      uint32_t byte = 0, word = 0;
-      if (page) {
-        byte = run ? (uint32_t)((e < 8 - lead ? a : b) >> (8 * place)) & 255u : page[unit + (size_t)(slot >> 3) * UNITS * 8 + place];
-        word = *(const uint32_t*)(page + (size_t)head * at.bytes + at.value_words + (size_t)slot * 4);
+      uint32_t byte[2] = {};
+      if (run) {
+        const bool in_a = e < 8 - lead;
+        byte[0] = (place < 4 ? (in_a ? a.x : b.x) : (in_a ? a.y : b.y)) >> (8 * (place & 3)) & 255u;
+        byte[1] = (place < 4 ? (in_a ? a.z : b.z) : (in_a ? a.w : b.w)) >> (8 * (place & 3)) & 255u;
+      } else if (page) {
+        const uint8_t* p = page + unit + (size_t)(slot >> 3) * (D * BITS) + place;
+        byte[0] = p[0], byte[1] = p[8];
       }
+      const uint32_t word = value_words[hb][e];
       const float s = word_step(word), z = word_offset(word);
-      T* out = v + ((size_t)(t0 + e) * n_kv_heads + head) * D;
-      if constexpr (BITS == 4) {
-        const float x0 = fmaf(s, (float)((int)(byte & 15) - H), z), x1 = fmaf(s, (float)((int)(byte >> 4) - H), z);
-        if constexpr (sizeof(T) == 2)
-          *(uint32_t*)(out + 2 * u) = pack2_bf16(x0, x1);
-        else
-          *(float2*)(out + 2 * u) = make_float2(x0, x1);
-      } else {
-        Elem<T>::store(out + u, fmaf(s, (float)((int)byte - H), z));
-      }
+      float x[DIMS];
+#pragma unroll
+      for (int d = 0; d < DIMS; ++d) x[d] = fmaf(s, (float)((int)(BITS == 4 ? (byte[d / 2] >> (4 * (d & 1))) & 15u : byte[d % 2]) - H), z);
+      T* out = v + ((size_t)(t0 + e) * n_kv_heads + head) * D + DIMS * u;
+      if constexpr (sizeof(T) == 2 && DIMS == 4)
+        *(uint2*)out = make_uint2(pack2_bf16(x[0], x[1]), pack2_bf16(x[2 % DIMS], x[3 % DIMS]));
+      else if constexpr (sizeof(T) == 2)
+        *(uint32_t*)out = pack2_bf16(x[0], x[1]);
+      else if constexpr (DIMS == 4)
+        *(float4*)out = make_float4(x[0], x[1], x[2 % DIMS], x[3 % DIMS]);
+      else
+        *(float2*)out = make_float2(x[0], x[1]);
     }
   }
 }
@@ -519,7 +534,7 @@ extern "C" int cwm_quant_kv_read(void* k, void* v, int dtype, const int* positio
   CWM_REQUIRE(((uintptr_t)cache % 16) == 0 && ((uintptr_t)k % 16) == 0 && ((uintptr_t)v % 16) == 0, "quant_kv_read: tensors must be 16-byte aligned");
   const int kv_groups = (n_kv_heads + HEADS_A_BLOCK - 1) / HEADS_A_BLOCK;
   CWM_REQUIRE(2 * kv_groups <= 65535, "quant_kv_read: too many heads");
-  const dim3 grid((n_tokens + CHUNK - 1) / CHUNK, 2 * kv_groups), block(64 * (((n_kv_heads < HEADS_A_BLOCK ? n_kv_heads : HEADS_A_BLOCK) + 1) / 2));
+  const dim3 grid((n_tokens + CHUNK - 1) / CHUNK, 2 * kv_groups), block(256);
 #define CALL_READ(G, BITS)                                                                                                                         if (dtype == CWM_BF16)                                                                                                                             hipLaunchKernelGGL((quant_kv_read_kernel<bf16_t, G, BITS>), grid, block, 0, stream, (bf16_t*)k, (bf16_t*)v, positions, seq_of_token,                                 (const uint8_t*)cache, block_table, n_seqs, table_width, page_size, num_pages, n_tokens, n_kv_heads, kv_groups);            else                                                                                                                                               hipLaunchKernelGGL((quant_kv_read_kernel<float, G, BITS>), grid, block, 0, stream, (float*)k, (float*)v, positions, seq_of_token,                                    (const uint8_t*)cache, block_table, n_seqs, table_width, page_size, num_pages, n_tokens, n_kv_heads, kv_groups)
   if (bits == 4) {
     FOR_GROUPS(CALL_READ, 4)
