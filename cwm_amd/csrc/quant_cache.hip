@@ -516,7 +516,17 @@ quant_unpack_kernel(bf16_t* __restrict__ out, int out_page, const int* __restric
 }
 
 // ---- entry points ------------------------------------------------------------------------ //
-#define FOR_GROUPS(CALL, BITS)                                    switch (head_dim / 32) {                                          case 1: CALL(1, BITS); break;                                   case 2: CALL(2, BITS); break;                                   case 3: CALL(3, BITS); break;                                   case 4: CALL(4, BITS); break;                                   case 5: CALL(5, BITS); break;                                   case 6: CALL(6, BITS); break;                                   case 7: CALL(7, BITS); break;                                   default: CALL(8, BITS); break;                                }
+#define FOR_GROUPS(CALL, BITS)     \
+  switch (head_dim / 32) {         \
+    case 1: CALL(1, BITS); break;  \
+    case 2: CALL(2, BITS); break;  \
+    case 3: CALL(3, BITS); break;  \
+    case 4: CALL(4, BITS); break;  \
+    case 5: CALL(5, BITS); break;  \
+    case 6: CALL(6, BITS); break;  \
+    case 7: CALL(7, BITS); break;  \
+    default: CALL(8, BITS); break; \
+  }
 
 extern "C" int cwm_quant_kv_write(const void* k, long k_stride, const void* v, long v_stride, void* q, long q_stride, int dtype, const int* positions,
                                   const int* seq_of_token, const float* inv_freq, void* cache, const int* block_table, int n_seqs, int table_width,
@@ -536,7 +546,15 @@ extern "C" int cwm_quant_kv_write(const void* k, long k_stride, const void* v, l
   const int piece = dtype == CWM_BF16 ? 8 : 4;
   const bool ka = k_stride % piece == 0 && (uintptr_t)k % 16 == 0, va = v_stride % piece == 0 && (uintptr_t)v % 16 == 0;
   const bool qa = q_stride % piece == 0 && (uintptr_t)q % 16 == 0;
-#define CALL_WRITE(G, BITS)                                                                                                                       if (dtype == CWM_BF16)                                                                                                                            hipLaunchKernelGGL((quant_kv_write_kernel<bf16_t, G, BITS>), grid, block, 0, stream, (const bf16_t*)k, k_stride, (const bf16_t*)v, v_stride,                        (bf16_t*)q, q_stride, positions, seq_of_token, inv_freq, (uint8_t*)cache, block_table, n_seqs, table_width, page_size,                          num_pages, n_tokens, n_kv_heads, n_q_heads, kv_groups, ka, va, qa);                                                        else                                                                                                                                              hipLaunchKernelGGL((quant_kv_write_kernel<float, G, BITS>), grid, block, 0, stream, (const float*)k, k_stride, (const float*)v, v_stride,                          (float*)q, q_stride, positions, seq_of_token, inv_freq, (uint8_t*)cache, block_table, n_seqs, table_width, page_size,                           num_pages, n_tokens, n_kv_heads, n_q_heads, kv_groups, ka, va, qa)
+#define CALL_WRITE(G, BITS)                                                                                                                      \
+  if (dtype == CWM_BF16)                                                                                                                         \
+    hipLaunchKernelGGL((quant_kv_write_kernel<bf16_t, G, BITS>), grid, block, 0, stream, (const bf16_t*)k, k_stride, (const bf16_t*)v, v_stride, \
+      (bf16_t*)q, q_stride, positions, seq_of_token, inv_freq, (uint8_t*)cache, block_table, n_seqs, table_width, page_size,                     \
+      num_pages, n_tokens, n_kv_heads, n_q_heads, kv_groups, ka, va, qa);                                                                        \
+  else                                                                                                                                           \
+    hipLaunchKernelGGL((quant_kv_write_kernel<float, G, BITS>), grid, block, 0, stream, (const float*)k, k_stride, (const float*)v, v_stride,    \
+      (float*)q, q_stride, positions, seq_of_token, inv_freq, (uint8_t*)cache, block_table, n_seqs, table_width, page_size,                      \
+      num_pages, n_tokens, n_kv_heads, n_q_heads, kv_groups, ka, va, qa)
   if (bits == 4) {
     FOR_GROUPS(CALL_WRITE, 4)
   } else {
@@ -556,7 +574,13 @@ extern "C" int cwm_quant_kv_read(void* k, void* v, int dtype, const int* positio
   const int kv_groups = (n_kv_heads + HEADS_A_BLOCK - 1) / HEADS_A_BLOCK;
   CWM_REQUIRE(2 * kv_groups <= 65535, "quant_kv_read: too many heads");
   const dim3 grid((n_tokens + CHUNK - 1) / CHUNK, 2 * kv_groups), block(256);
-#define CALL_READ(G, BITS)                                                                                                                         if (dtype == CWM_BF16)                                                                                                                             hipLaunchKernelGGL((quant_kv_read_kernel<bf16_t, G, BITS>), grid, block, 0, stream, (bf16_t*)k, (bf16_t*)v, positions, seq_of_token,                                 (const uint8_t*)cache, block_table, n_seqs, table_width, page_size, num_pages, n_tokens, n_kv_heads, kv_groups);            else                                                                                                                                               hipLaunchKernelGGL((quant_kv_read_kernel<float, G, BITS>), grid, block, 0, stream, (float*)k, (float*)v, positions, seq_of_token,                                    (const uint8_t*)cache, block_table, n_seqs, table_width, page_size, num_pages, n_tokens, n_kv_heads, kv_groups)
+#define CALL_READ(G, BITS)                                                                                                               \
+  if (dtype == CWM_BF16)                                                                                                                 \
+    hipLaunchKernelGGL((quant_kv_read_kernel<bf16_t, G, BITS>), grid, block, 0, stream, (bf16_t*)k, (bf16_t*)v, positions, seq_of_token, \
+      (const uint8_t*)cache, block_table, n_seqs, table_width, page_size, num_pages, n_tokens, n_kv_heads, kv_groups);                   \
+  else                                                                                                                                   \
+    hipLaunchKernelGGL((quant_kv_read_kernel<float, G, BITS>), grid, block, 0, stream, (float*)k, (float*)v, positions, seq_of_token,    \
+      (const uint8_t*)cache, block_table, n_seqs, table_width, page_size, num_pages, n_tokens, n_kv_heads, kv_groups)
   if (bits == 4) {
     FOR_GROUPS(CALL_READ, 4)
   } else {
