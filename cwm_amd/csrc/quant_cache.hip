@@ -1,9 +1,8 @@
 // Writes keys and values into the cache of 4 or 8 bits (layout and formulas: quant_cache.h) and reads them back.
 //
 // Both kernels take eight tokens of the list at a time, the tokens of one value block where the list follows a sequence.
-// Four lanes share a token's head, lane j with the elements 32 g + 8 j .. + 7 of every group g: a lane's codes of a key are
-// one piece of memory, the largest and smallest of a group are two exchanges between lanes, and the two elements that a
-// rotation turns are the lane's own.
+// Writing, four lanes share a group, lane j with its elements 8 j .. + 7: a lane's codes of a key are one piece of memory, the
+// largest and smallest of a group are two exchanges between lanes, and the two elements that a rotation turns are the lane's own.
 #include "quant_cache.h"
 
 CWM_DEFINE_ERROR_API
@@ -116,41 +115,59 @@ template <int N> __device__ __forceinline__ void stream_out(float* p, const floa
 
 // Largest and smallest of eight values; a value that is not finite makes the largest infinite.
 __device__ __forceinline__ void extremes(const float (&x)[8], float& hi, float& lo) {
+  float rest = 0.f;  // NaN where a value is not finite
+  hi = lo = x[0];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool finite = (__float_as_uint(x[e]) & 0x7f800000u) != 0x7f800000u;
-    hi = fmaxf(hi, finite ? x[e] : __builtin_inff());
-    lo = fminf(lo, finite ? x[e] : hi);
-  }
+  for (int e = 0; e < 8; ++e) rest = fmaf(x[e], 0.f, rest), hi = fmaxf(hi, x[e]), lo = fminf(lo, x[e]);
+  if (rest != 0.f) hi = __builtin_inff();
 }
-__device__ __forceinline__ void over_lanes(float& hi, float& lo) {  // of the four lanes of a token's head
-#pragma unroll
-  for (int off = 1; off < 4; off <<= 1) {
-    hi = fmaxf(hi, __shfl_xor(hi, off, 64));
-    lo = fminf(lo, __shfl_xor(lo, off, 64));
-  }
+template <int QUAD_PERM> __device__ __forceinline__ float of_quad(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), QUAD_PERM, 15, 15, true));
+}
+__device__ __forceinline__ void over_lanes(float& hi, float& lo) {  // of the four lanes of a group
+  hi = fmaxf(hi, of_quad<0xb1>(hi)), lo = fminf(lo, of_quad<0xb1>(lo));
+  hi = fmaxf(hi, of_quad<0x4e>(hi)), lo = fminf(lo, of_quad<0x4e>(lo));
+}
+
+// a / d in 64 bits for d of 7, 15, 127 and 255: the product with the reciprocal and its remainder give the rounded quotient
+// (Markstein's theorem: the reciprocals lie within 0.3 steps).
+template <int d> __device__ __forceinline__ double over(double a) {
+  constexpr double inv = 1. / d;
+  const double q = a * inv;
+  return fma(fma(-q, (double)d, a), inv, q);
 }
 
 // Step and offset of a group, in 64 bits: a step that just fits (a quotient without a remainder) is common among bfloat16
 // numbers and must not be taken for the next larger one.
 template <int BITS> __device__ __forceinline__ uint32_t group_word(float hi, float lo) {
-  constexpr double H = 1 << (BITS - 1);
+  constexpr int H = 1 << (BITS - 1);
   if (hi == __builtin_inff()) return 0x7fc07fc0u;
-  uint32_t z = f32_to_bf16(to_float((H * hi + (H - 1) * lo) / (2 * H - 1)));
+  uint32_t z = f32_to_bf16(to_float(over<2 * H - 1>((double)H * hi + (double)(H - 1) * lo)));
   if ((z & 0x7fffu) == 0x7f80u) z -= 1;  // float32 values next to the largest one: the largest of bfloat16
   const double zd = word_offset(z);
-  const float need = (float)fmax((hi - zd) / (H - 1), (zd - lo) / H);
+  const float need = (float)fmax(over<H - 1>(hi - zd), (zd - lo) * (1. / H));
   return ((__float_as_uint(need) + 0xffffu) & 0xffff0000u) | z;
 }
 
-// The code of x.  float32 arithmetic decides it except next to a tie, where it may be off by its own rounding (the
-// quotient is at most 2^7 and three roundings of 2^-24 make it, 2.3e-5 in all): there it is the quotient of 64 bits.
-template <int BITS> __device__ __forceinline__ int code_of(float x, float s, float inv, float z) {
+// The codes of eight numbers, less H.  float32 arithmetic decides one except next to a tie, where it may be off by its own
+// rounding (the quotient is at most 2^7; a reciprocal off by 2^-23 and two roundings of 2^-24 make it, 3.1e-5 in all): there it is the quotient of 64 bits.
+template <int BITS> __device__ __forceinline__ void codes_of(const float (&x)[8], uint32_t word, int (&c)[8]) {
   constexpr int H = 1 << (BITS - 1);
-  const float t = (x - z) * inv;
-  float r = rintf(t);
-  if (!(fabsf(t - r) < 0.4999f)) r = s > 0.f ? (float)rint(((double)x - (double)z) / (double)s) : 0.f;
-  return (int)fminf(fmaxf(r, -(float)H), (float)(H - 1)) + H;  // a NaN gives H
+  const float s = word_step(word), z = word_offset(word);
+  const float inv = s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;  // a step of 0 or NaN: codes of H
+  float r[8], off = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = (x[e] - z) * inv;
+    r[e] = rintf(t);
+    off = fmaxf(off, fabsf(t - r[e]));
+  }
+  if (off >= 0.4999f || inv == __builtin_inff()) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = s > 0.f ? (float)rint(((double)x[e] - (double)z) / (double)s) : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = min(max((int)r[e], -H), H - 1);  // a NaN gives 0
 }
 
 // A token's place in the cache: the first byte of its page and its slot, or no page.
@@ -170,84 +187,84 @@ __device__ __forceinline__ Place place_of(uint8_t* cache, long page_bytes, int p
   return p;
 }
 
-// grid: (chunks of eight tokens, groups of eight heads: those of the keys, of the values, then of the queries)
-// block: 32 lanes a head: 8 tokens x 4
-// Bound by memory for prompts (2 bytes in and half a byte out a value) and by its latency for decoded tokens.
+// Heads of a writing block: up to 512 lanes (4,096 tokens of 8 heads of 128 take 16.6 us, with 256 lanes 17.9, with 1,024 19.0).
+__host__ __device__ constexpr int write_heads(int groups) { return 16 / groups < HEADS_A_BLOCK ? 16 / groups : HEADS_A_BLOCK; }
+
+// grid: (chunks of eight tokens, groups of `heads_a_block` heads: those of the keys, of the values, then of the queries)
+// block: a lane for eight elements: 8 tokens x heads x G groups x 4
+// Prompts are bound by their arithmetic (300 instructions a lane, the turns and the rounding in 64 bits the most of them: 4,096
+// tokens of 8 heads of 128 in 16.6 us, whose bytes take 5), decoded tokens by what waits for what, which the fetching of the code itself
+// belongs to: with a lane for all groups of a head, four times the code, eight tokens took 7.1 us, now 5.1.
 template <typename T, int G, int BITS>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
 quant_kv_write_kernel(const T* __restrict__ k, long k_stride, const T* __restrict__ v, long v_stride, T* __restrict__ q, long q_stride,
                       const int* __restrict__ positions, const int* __restrict__ seq_of_token, const float* __restrict__ inv_freq,
                       uint8_t* __restrict__ cache, const int* __restrict__ block_table, int n_seqs, int table_width, int page_size, int num_pages,
-                      int n_tokens, int n_kv_heads, int n_q_heads, int kv_groups, bool k_aligned, bool v_aligned, bool q_aligned) {
+                      int n_tokens, int n_kv_heads, int n_q_heads, int heads_a_block, int kv_groups, bool k_aligned, bool v_aligned, bool q_aligned) {
   constexpr int D = 32 * G;
+  constexpr int MOST_HEADS = write_heads(G);
   constexpr int UNITS = BITS == 4 ? D / 2 : D;  // rows of eight bytes of a value block
+  constexpr int WORDS = BITS / 4;               // of a group's eight codes
   __shared__ double turn_s[CHUNK][D / 2], turn_c[CHUNK][D / 2];
-  __shared__ __attribute__((aligned(8))) uint8_t block_codes[HEADS_A_BLOCK][UNITS][8];
+  __shared__ __attribute__((aligned(8))) uint8_t block_codes[MOST_HEADS][UNITS][8];
+  __shared__ float2 block_extremes[CHUNK][MOST_HEADS][G];
   __shared__ uint8_t* dst_page[CHUNK];
   __shared__ int dst_slot[CHUNK];
 
   const int t0 = blockIdx.x * CHUNK;
   const int kind = blockIdx.y < kv_groups ? 0 : (blockIdx.y < 2 * kv_groups ? 1 : 2);  // keys, values, queries
-  const int head0 = (blockIdx.y - kind * kv_groups) * HEADS_A_BLOCK;
+  const int head0 = (blockIdx.y - kind * kv_groups) * heads_a_block;
   const int tid = threadIdx.x;
-  const int head_in_block = tid >> 5, tk = (tid >> 2) & 7, j = tid & 3;
+  const int j = tid & 3, g = (tid >> 2) % G, pair = tid / (4 * G), tk = pair / heads_a_block, head_in_block = pair - tk * heads_a_block;
   const int t = t0 + tk;
-  const int heads = kind == 2 ? n_q_heads : n_kv_heads;
   const int head = head0 + head_in_block;
+  const int heads = kind == 2 ? n_q_heads : n_kv_heads;
   const bool mine = t < n_tokens && head < heads;
   const QuantHead at = quant_head(page_size, D, BITS);
 
-  if (kind != 1 && inv_freq) {
-    // the turns of the eight tokens, once for all heads of the block; in 64 bits, so that a turned key is what the formula
-    // gives, rounded once
-    for (int i = tid; i < CHUNK * (D / 2); i += blockDim.x) {
-      const int tt = i / (D / 2), f = i - tt * (D / 2);
-      if (t0 + tt < n_tokens) {
-        const double turns = (double)positions[t0 + tt] * (double)inv_freq[f] * 0.15915494309189535;
-        sincospi(2.0 * (turns - rint(turns)), &turn_s[tt][f], &turn_c[tt][f]);
-      }
-    }
-  }
-  if (kind == 1 && tid < CHUNK) {
+  // The loads of the row and of the tokens' places are under way while the turns are computed.  A lane without a row takes the last one.
+  const size_t at_row = (size_t)min(t, n_tokens - 1), column = (size_t)min(head, heads - 1) * D + 32 * g + 8 * j;
+  float x[8];
+  load8((kind == 0 ? k + at_row * k_stride : kind == 1 ? v + at_row * v_stride : q + at_row * q_stride) + column,
+        kind == 0 ? k_aligned : kind == 1 ? v_aligned : q_aligned, x);
+  if (kind != 2 && tid < CHUNK) {
     Place p = {nullptr, 0};
     if (t0 + tid < n_tokens)
       p = place_of(cache, at.bytes * n_kv_heads, positions[t0 + tid], seq_of_token[t0 + tid], block_table, n_seqs, table_width, page_size, num_pages);
     dst_page[tid] = p.page;
     dst_slot[tid] = p.slot;
   }
-  __syncthreads();
 
   if (kind == 1) {
-    if (mine) {
-      float x[G][8];
-      float hi = -__builtin_inff(), lo = __builtin_inff();
-      const T* row = v + (size_t)t * v_stride + (size_t)head * D + 8 * j;
+    float hi, lo;
+    extremes(x, hi, lo);
+    over_lanes(hi, lo);
+    if (j == 0) block_extremes[tk][head_in_block][g] = make_float2(hi, lo);
+    __syncthreads();
 #pragma unroll
-      for (int g = 0; g < G; ++g) load8(row + 32 * g, v_aligned, x[g]);
-#pragma unroll
-      for (int g = 0; g < G; ++g) extremes(x[g], hi, lo);
-      over_lanes(hi, lo);
-      const uint32_t word = group_word<BITS>(hi, lo);
-      const float s = word_step(word), z = word_offset(word), inv = 1.f / s;
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int e = 0; e < 8; e += BITS == 4 ? 2 : 1) {
-          const int d = 32 * g + 8 * j + e;
-          const int c = code_of<BITS>(x[g][e], s, inv, z);
-          if constexpr (BITS == 4)
-            block_codes[head_in_block][d / 2][tk] = (uint8_t)(c | (code_of<BITS>(x[g][e + 1], s, inv, z) << 4));
-          else
-            block_codes[head_in_block][d][tk] = (uint8_t)c;
-        }
-      if (j == 0 && dst_page[tk]) *(uint32_t*)(dst_page[tk] + (size_t)head * at.bytes + at.value_words + (size_t)dst_slot[tk] * 4) = word;
+    for (int i = 0; i < G; ++i) {
+      const float2 of = block_extremes[tk][head_in_block][i];
+      hi = fmaxf(hi, of.x);
+      lo = fminf(lo, of.y);
     }
+    const uint32_t word = group_word<BITS>(hi, lo);
+    int c[8];
+    codes_of<BITS>(x, word, c);
+#pragma unroll
+    for (int e = 0; e < 8; e += BITS == 4 ? 2 : 1) {
+      const int d = 32 * g + 8 * j + e;
+      if constexpr (BITS == 4)
+        block_codes[head_in_block][d / 2][tk] = (uint8_t)(c[e] + 16 * c[e + 1] + 0x88);
+      else
+        block_codes[head_in_block][d][tk] = (uint8_t)(c[e] + 0x80);
+    }
+    if (mine && j == 0 && g == 0 && dst_page[tk]) *(uint32_t*)(dst_page[tk] + (size_t)head * at.bytes + at.value_words + (size_t)dst_slot[tk] * 4) = word;
     __syncthreads();
     // Eight tokens that fill a value block are stored eight bytes at a time; tokens that do not follow one another, or that
     // begin inside a block, byte by byte.
     bool whole = dst_page[0] != nullptr && (dst_slot[0] & 7) == 0;
     for (int i = 1; i < CHUNK; ++i) whole = whole && dst_page[i] == dst_page[0] && dst_slot[i] == dst_slot[0] + i;
-    const int units = min(HEADS_A_BLOCK, n_kv_heads - head0) * UNITS;
+    const int units = min(heads_a_block, n_kv_heads - head0) * UNITS;
     if (whole) {
       uint8_t* block = dst_page[0] + (size_t)head0 * at.bytes + at.values + (size_t)(dst_slot[0] >> 3) * UNITS * 8;
       for (int i = tid; i < units; i += blockDim.x) {
@@ -264,62 +281,59 @@ quant_kv_write_kernel(const T* __restrict__ k, long k_stride, const T* __restric
         for (int e = 0; e < CHUNK; ++e) {
           uint8_t* page = dst_page[e];
           if (!page) continue;
-          const int slot = dst_slot[e], place = BITS == 4 ? quant_place(slot & 7) : slot & 7;
-          page[(size_t)(head0 + hb) * at.bytes + at.values + ((size_t)(slot >> 3) * UNITS + u) * 8 + place] = (uint8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
+          const int slot = dst_slot[e], byte = BITS == 4 ? quant_place(slot & 7) : slot & 7;
+          page[(size_t)(head0 + hb) * at.bytes + at.values + ((size_t)(slot >> 3) * UNITS + u) * 8 + byte] = (uint8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
         }
       }
     }
     return;
   }
 
-  if (!mine) return;
-  const bool is_key = kind == 0;
-  const T* row = (is_key ? k + (size_t)t * k_stride : q + (size_t)t * q_stride) + (size_t)head * D + 8 * j;
-  const bool aligned = is_key ? k_aligned : q_aligned;
-  float x[G][8];
-#pragma unroll
-  for (int g = 0; g < G; ++g) load8(row + 32 * g, aligned, x[g]);
   if (inv_freq) {
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const int f = 16 * g + 4 * j + e / 2;
-        const double re = x[g][e], im = x[g][e + 1], c = turn_c[tk][f], s = turn_s[tk][f];
-        x[g][e] = as_stored<T>(to_float(re * c - im * s));
-        x[g][e + 1] = as_stored<T>(to_float(im * c + re * s));
+    // the turns of the eight tokens, once for all heads of the block; in 64 bits, so that a turned key is what the formula
+    // gives, rounded once
+    for (int i = tid; i < CHUNK * (D / 2); i += blockDim.x) {
+      const int tt = i / (D / 2), f = i - tt * (D / 2);
+      if (t0 + tt < n_tokens) {
+        const double turns = (double)positions[t0 + tt] * (double)inv_freq[f] * 0.15915494309189535;
+        sincospi(2.0 * (turns - rint(turns)), &turn_s[tt][f], &turn_c[tt][f]);
       }
-  }
-  if (!is_key) {
-    T* out = q + (size_t)t * q_stride + (size_t)head * D + 8 * j;
-#pragma unroll
-    for (int g = 0; g < G; ++g) store8(out + 32 * g, aligned, x[g]);
-    return;
-  }
-  constexpr int WORDS = BITS / 4;  // of a group's eight codes
-  uint32_t codes[G * WORDS], words[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    float hi = -__builtin_inff(), lo = __builtin_inff();
-    extremes(x[g], hi, lo);
-    over_lanes(hi, lo);
-    words[g] = group_word<BITS>(hi, lo);
-    const float s = word_step(words[g]), z = word_offset(words[g]), inv = 1.f / s;
-    int c[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = code_of<BITS>(x[g][e], s, inv, z);
-    if constexpr (BITS == 4) {
-      codes[g] = c[0] | (c[2] << 4) | (c[4] << 8) | (c[6] << 12) | (c[1] << 16) | (c[3] << 20) | (c[5] << 24) | ((uint32_t)c[7] << 28);
-    } else {
-      codes[2 * g] = c[0] | (c[1] << 8) | (c[2] << 16) | ((uint32_t)c[3] << 24);
-      codes[2 * g + 1] = c[4] | (c[5] << 8) | (c[6] << 16) | ((uint32_t)c[7] << 24);
     }
   }
-  const Place p = place_of(cache, at.bytes * n_kv_heads, positions[t], seq_of_token[t], block_table, n_seqs, table_width, page_size, num_pages);
-  if (!p.page) return;
-  uint8_t* to = p.page + (size_t)head * at.bytes;
-  put_words<G * WORDS>((uint32_t*)to + ((size_t)p.slot * 4 + j) * G * WORDS, codes);
-  if (j == 0) put_words<G>((uint32_t*)(to + at.key_words) + (size_t)p.slot * G, words);
+  __syncthreads();
+  if (inv_freq) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const int f = 16 * g + 4 * j + e / 2;
+      const double re = x[e], im = x[e + 1], c = turn_c[tk][f], s = turn_s[tk][f];
+      x[e] = as_stored<T>(to_float(re * c - im * s));
+      x[e + 1] = as_stored<T>(to_float(im * c + re * s));
+    }
+  }
+  if (kind == 2) {
+    if (mine) store8(q + at_row * q_stride + column, q_aligned, x);
+    return;
+  }
+  float hi, lo;
+  extremes(x, hi, lo);
+  over_lanes(hi, lo);
+  const uint32_t word = group_word<BITS>(hi, lo);
+  int c[8];
+  codes_of<BITS>(x, word, c);
+  uint8_t* const page = dst_page[tk];
+  if (!mine || !page) return;
+  // sums of signed codes, and H on every one of them at the end: nothing is carried over
+  uint32_t codes[WORDS];
+  if constexpr (BITS == 4) {
+    codes[0] = ((((((c[7] * 16 + c[5]) * 16 + c[3]) * 16 + c[1]) * 16 + c[6]) * 16 + c[4]) * 16 + c[2]) * 16 + c[0] + 0x88888888u;
+  } else {
+    codes[0] = ((c[3] * 256 + c[2]) * 256 + c[1]) * 256 + c[0] + 0x80808080u;
+    codes[WORDS - 1] = ((c[7] * 256 + c[6]) * 256 + c[5]) * 256 + c[4] + 0x80808080u;
+  }
+  uint8_t* const to = page + (size_t)head * at.bytes;
+  const int slot = dst_slot[tk];
+  put_words<WORDS>((uint32_t*)to + (((size_t)slot * 4 + j) * G + g) * WORDS, codes);
+  if (j == 0) *(uint32_t*)(to + at.key_words + ((size_t)slot * G + g) * 4) = word;
 }
 
 // Reads the tokens of a list: grid (chunks of eight tokens, groups of eight heads: keys, then values).  Bound by memory, most of it the
@@ -538,11 +552,12 @@ extern "C" int cwm_quant_kv_write(const void* k, long k_stride, const void* v, l
   CWM_REQUIRE(k && v && cache && block_table && positions && seq_of_token, "quant_kv_write: a tensor is missing");
   CWM_REQUIRE(q || n_q_heads == 0, "quant_kv_write: queries missing");
   CWM_REQUIRE(((uintptr_t)cache % 16) == 0, "quant_kv_write: the cache must be 16-byte aligned");
-  const int kv_groups = (n_kv_heads + HEADS_A_BLOCK - 1) / HEADS_A_BLOCK;
-  const int q_groups = q && inv_freq ? (n_q_heads + HEADS_A_BLOCK - 1) / HEADS_A_BLOCK : 0;
+  const int groups = head_dim / 32, chunks = (n_tokens + CHUNK - 1) / CHUNK;
+  const int heads = q && n_q_heads > n_kv_heads ? n_q_heads : n_kv_heads, heads_a_block = write_heads(groups) < heads ? write_heads(groups) : heads;
+  const int kv_groups = (n_kv_heads + heads_a_block - 1) / heads_a_block;
+  const int q_groups = q && inv_freq ? (n_q_heads + heads_a_block - 1) / heads_a_block : 0;
   CWM_REQUIRE(2 * kv_groups + q_groups <= 65535, "quant_kv_write: too many heads");
-  const int most_heads = q_groups ? HEADS_A_BLOCK : (n_kv_heads < HEADS_A_BLOCK ? n_kv_heads : HEADS_A_BLOCK);
-  const dim3 grid((n_tokens + CHUNK - 1) / CHUNK, 2 * kv_groups + q_groups), block(64 * ((most_heads + 1) / 2));
+  const dim3 grid(chunks, 2 * kv_groups + q_groups), block(32 * groups * heads_a_block);
   const int piece = dtype == CWM_BF16 ? 8 : 4;
   const bool ka = k_stride % piece == 0 && (uintptr_t)k % 16 == 0, va = v_stride % piece == 0 && (uintptr_t)v % 16 == 0;
   const bool qa = q_stride % piece == 0 && (uintptr_t)q % 16 == 0;
@@ -550,11 +565,11 @@ extern "C" int cwm_quant_kv_write(const void* k, long k_stride, const void* v, l
   if (dtype == CWM_BF16)                                                                                                                         \
     hipLaunchKernelGGL((quant_kv_write_kernel<bf16_t, G, BITS>), grid, block, 0, stream, (const bf16_t*)k, k_stride, (const bf16_t*)v, v_stride, \
       (bf16_t*)q, q_stride, positions, seq_of_token, inv_freq, (uint8_t*)cache, block_table, n_seqs, table_width, page_size,                     \
-      num_pages, n_tokens, n_kv_heads, n_q_heads, kv_groups, ka, va, qa);                                                                        \
+      num_pages, n_tokens, n_kv_heads, n_q_heads, heads_a_block, kv_groups, ka, va, qa);                                                                        \
   else                                                                                                                                           \
     hipLaunchKernelGGL((quant_kv_write_kernel<float, G, BITS>), grid, block, 0, stream, (const float*)k, k_stride, (const float*)v, v_stride,    \
       (float*)q, q_stride, positions, seq_of_token, inv_freq, (uint8_t*)cache, block_table, n_seqs, table_width, page_size,                      \
-      num_pages, n_tokens, n_kv_heads, n_q_heads, kv_groups, ka, va, qa)
+      num_pages, n_tokens, n_kv_heads, n_q_heads, heads_a_block, kv_groups, ka, va, qa)
   if (bits == 4) {
     FOR_GROUPS(CALL_WRITE, 4)
   } else {
