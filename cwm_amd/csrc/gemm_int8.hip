@@ -275,9 +275,10 @@ template <int WM, int WN>
 struct Int8Source {
   const bf16_t *A, *W;
   long lda, ldw;  // in pairs of bytes
-  int M, N, w_last, lane, wave;
+  int M, N, w_last, steps, lane, wave;
   Int8Order order;
   const bf16_t *a, *w;
+  int first_step;
   uint32_t off[WideShape<WM, WN>::ND];
   static constexpr bool W_TILES = false;
   __device__ __forceinline__ const bf16_t* base(int p) const { return p < WideShape<WM, WN>::BM / 8 ? a : w; }
@@ -288,6 +289,7 @@ struct Int8Source {
     const int m0 = tm * BM, n0 = tn * BN;
     a = A + (size_t)m0 * lda;
     w = W + (size_t)n0 * ldw;
+    first_step = tn % steps;
 #pragma unroll
     for (int i = 0; i < WideShape<WM, WN>::ND; ++i) {
       const int p = min(wave + 8 * i, WideShape<WM, WN>::PIECES - 1);
@@ -381,7 +383,7 @@ gemm_int8_wide_kernel(const int8_t* __restrict__ X, long ldx, const float* __res
   const int first = xcd * per + min(xcd, rest), count = per + (xcd < rest ? 1 : 0);
   const int mine = (count - idx + blocks - 1) / blocks;
   const Int8Order order = {m_tiles, n_tiles};
-  Int8Source<WM, WN> src = {(const bf16_t*)X, (const bf16_t*)W, ldx / 2, ldw / 2, M, N, (K - 128) / 2, lane, wave, order};
+  Int8Source<WM, WN> src = {(const bf16_t*)X, (const bf16_t*)W, ldx / 2, ldw / 2, M, N, (K - 128) / 2, (K + 127) / 128, lane, wave, order};
   Int8Sink<WM, WN, T> sink = {y, ldy, a, w_scale, bias, M, N, lane, wave, vector, order};
   wide_loop<WM, WN, Int8Sink<WM, WN, T>::STORES, WideInt8<ONCE>>(lds, src, sink, first + idx, blocks, mine, (K + 127) / 128);
 }

@@ -50,6 +50,7 @@ struct WideBf16 {
   static constexpr bool W_ONCE = false;  // whether the rows of W go past the caches: with one tile of rows each is read once
   // where a step of W's rows begins
   template <typename SOURCE> static __device__ __forceinline__ size_t w_step(const SOURCE&, int step, int length) { return (size_t)step * length; }
+  template <typename SOURCE> static __device__ __forceinline__ int at(const SOURCE&, int step, int) { return step; }  // the step of K that comes in turn
   static __device__ __forceinline__ Sums run(const Frag8& w, const Frag8& a, const Sums& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v, a.v, c, 0, 0, 0); }
 };
 typedef int int4v __attribute__((ext_vector_type(4)));
@@ -60,6 +61,12 @@ template <bool ONCE> struct WideInt8 {  // K goes in steps of 128
   // it reads a second time.
   template <typename SOURCE> static __device__ __forceinline__ size_t w_step(const SOURCE& src, int step, int length) {
     return min(step * length, src.w_last);
+  }
+  // Sums of integers may be made in any order: with rows of W that are read once, every tile begins at another step of K, so that the
+  // blocks' reads of rows of one stride spread over the memory's channels.
+  template <typename SOURCE> static __device__ __forceinline__ int at(const SOURCE& src, int step, int steps) {
+    const int turned = step + src.first_step;
+    return !ONCE ? step : turned < steps ? turned : turned - steps;
   }
   static __device__ __forceinline__ Sums run(const Frag8& w, const Frag8& a, const Sums& c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4v, w.u), __builtin_bit_cast(int4v, a.u), c, 0, 0, 0);
@@ -90,7 +97,8 @@ __device__ __forceinline__ void wide_loop(unsigned char* lds, SOURCE& src, SINK&
   src.enter(i_tile);
   auto issue_one = [&](int i, uint32_t stage) __attribute__((always_inline)) {
     const int p = min(wave + 8 * i, PIECES - 1);
-    const bf16_t* from = src.base(p) + (p >= BM / 8 ? MMA::w_step(src, i_step, SOURCE::W_TILES ? 1024 : WIDE_BK) : (size_t)i_step * WIDE_BK);
+    const int step = MMA::at(src, i_step, steps);
+    const bf16_t* from = src.base(p) + (p >= BM / 8 ? MMA::w_step(src, step, SOURCE::W_TILES ? 1024 : WIDE_BK) : (size_t)step * WIDE_BK);
     if (MMA::W_ONCE && p >= BM / 8)
       dma16_once(from, src.off[i], lds0 + stage + p * 1024);
     else
