@@ -6,6 +6,8 @@
 //
 // Few rows: every byte of W is read once, straight into the matrix instruction's operand, and the product is bound by that
 // reading.  More rows: gemm_wide.h's loop.
+#include <type_traits>
+
 #include "gemm_wide.h"
 
 CWM_DEFINE_ERROR_API
@@ -275,7 +277,7 @@ template <int WM, int WN>
 struct Int8Source {
   const bf16_t *A, *W;
   long lda, ldw;  // in pairs of bytes
-  int M, N, w_last, steps, lane, wave;
+  int M, N, w_last, begin, steps, lane, wave;  // the steps of K from `begin` on
   Int8Order order;
   const bf16_t *a, *w;
   int first_step;
@@ -320,80 +322,125 @@ struct Int8Sink {
     const int r = lane & 15, j = lane >> 4, wm = wave >> 2, wn = wave & 3;
     const int m0 = tm * BM + wm * WM * 16 + r;
     const int n0 = tn * BN + wn * WN * 16 + 4 * WN * j;
-    float am[WM], ws[WN][4], bs[WN][4];
+    if constexpr (std::is_same<T, int>::value) {  // sums of a part of K: rows of whole tiles
 #pragma unroll
-    for (int i = 0; i < WM; ++i) am[i] = a[min(m0 + 16 * i, M - 1)];
+      for (int i = 0; i < WM; ++i)
 #pragma unroll
-    for (int b = 0; b < WN; ++b)
+        for (int b = 0; b < WN; ++b)
+          if (m0 + 16 * i < M) *(int4v*)(C + (size_t)(m0 + 16 * i) * ldc + n0 + 4 * b) = acc[i][b];
+      return false;
+    } else {
+      float am[WM], ws[WN][4], bs[WN][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int n = min(n0 + 4 * b + e, N - 1);
-        ws[b][e] = w_scale[n];
-        bs[b][e] = bias ? bias[n] : 0.f;
-      }
-    // Waited for here, by an instruction that the compiler knows of: loads that it takes to be under way at the loop's head
-    // make it wait for all of the loop's own loads in every step (2,048 x 43,008 x 6,144 663 us, 1.24 us a step).
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    const bool full = vector && (tm + 1) * BM <= M && (tn + 1) * BN <= N;
-#pragma unroll
-    for (int i = 0; i < WM; ++i) {
-      const int m = m0 + 16 * i;
-      if (m >= M) continue;
-      T* row = C + (size_t)m * ldc + n0;
-      float v[WN][4];
+      for (int i = 0; i < WM; ++i) am[i] = a[min(m0 + 16 * i, M - 1)];
 #pragma unroll
       for (int b = 0; b < WN; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[b][e] = (float)acc[i][b][e] * am[i] * ws[b][e] + bs[b][e];
+        for (int e = 0; e < 4; ++e) {
+          const int n = min(n0 + 4 * b + e, N - 1);
+          ws[b][e] = w_scale[n];
+          bs[b][e] = bias ? bias[n] : 0.f;
+        }
+      // Waited for here, by an instruction that the compiler knows of: loads that it takes to be under way at the loop's head
+      // make it wait for all of the loop's own loads in every step (2,048 x 43,008 x 6,144 663 us, 1.24 us a step).
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+      const bool full = vector && (tm + 1) * BM <= M && (tn + 1) * BN <= N;
 #pragma unroll
-      for (int b = 0; b < WN; b += 2) {
-        if (vector && n0 + 4 * b + 7 < N) {
-          if constexpr (sizeof(T) == 4) {
-            *(float4*)(row + 4 * b) = make_float4(v[b][0], v[b][1], v[b][2], v[b][3]);
-            *(float4*)(row + 4 * b + 4) = make_float4(v[b + 1][0], v[b + 1][1], v[b + 1][2], v[b + 1][3]);
+      for (int i = 0; i < WM; ++i) {
+        const int m = m0 + 16 * i;
+        if (m >= M) continue;
+        T* row = C + (size_t)m * ldc + n0;
+        float v[WN][4];
+#pragma unroll
+        for (int b = 0; b < WN; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[b][e] = (float)acc[i][b][e] * am[i] * ws[b][e] + bs[b][e];
+#pragma unroll
+        for (int b = 0; b < WN; b += 2) {
+          if (vector && n0 + 4 * b + 7 < N) {
+            if constexpr (sizeof(T) == 4) {
+              *(float4*)(row + 4 * b) = make_float4(v[b][0], v[b][1], v[b][2], v[b][3]);
+              *(float4*)(row + 4 * b + 4) = make_float4(v[b + 1][0], v[b + 1][1], v[b + 1][2], v[b + 1][3]);
+            } else {
+              *(uint4*)(row + 4 * b) = make_uint4(pack2_bf16(v[b][0], v[b][1]), pack2_bf16(v[b][2], v[b][3]), pack2_bf16(v[b + 1][0], v[b + 1][1]),
+                                                  pack2_bf16(v[b + 1][2], v[b + 1][3]));
+            }
           } else {
-            *(uint4*)(row + 4 * b) = make_uint4(pack2_bf16(v[b][0], v[b][1]), pack2_bf16(v[b][2], v[b][3]), pack2_bf16(v[b + 1][0], v[b + 1][1]),
-                                                pack2_bf16(v[b + 1][2], v[b + 1][3]));
-          }
-        } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (n0 + 4 * b + e < N) Elem<T>::store(row + 4 * b + e, v[b + e / 4][e % 4]);
+            for (int e = 0; e < 8; ++e)
+              if (n0 + 4 * b + e < N) Elem<T>::store(row + 4 * b + e, v[b + e / 4][e % 4]);
+          }
         }
       }
+      return full;
     }
-    return full;
   }
 };
 
+// T int: the sums of `parts` parts of K are written to y, [parts][M][ldy], a block a tile of one part.
 template <int WM, int WN, typename T, bool ONCE>
 __global__ void __launch_bounds__(512, 2)
 gemm_int8_wide_kernel(const int8_t* __restrict__ X, long ldx, const float* __restrict__ a, const int8_t* __restrict__ W, long ldw,
                       const float* __restrict__ w_scale, const float* __restrict__ bias, T* __restrict__ y, long ldy, bool vector, int M, int N,
-                      int K, int m_tiles, int n_tiles) {
+                      int K, int m_tiles, int n_tiles, int parts) {
   typedef WideShape<WM, WN> Shape;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[Shape::S * Shape::STAGE];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // the XCDs (block number modulo 8) take consecutive runs of tiles, their blocks in turn
-  const int total = m_tiles * n_tiles, groups = min(8, (int)gridDim.x);
+  const int tiles = m_tiles * n_tiles, total = tiles * parts, groups = min(8, (int)gridDim.x);
   const int xcd = blockIdx.x % groups, idx = blockIdx.x / groups;
   const int blocks = ((int)gridDim.x + groups - 1 - xcd) / groups;
   const int per = total / groups, rest = total % groups;
   const int first = xcd * per + min(xcd, rest), count = per + (xcd < rest ? 1 : 0);
   const int mine = (count - idx + blocks - 1) / blocks;
   const Int8Order order = {m_tiles, n_tiles};
-  Int8Source<WM, WN> src = {(const bf16_t*)X, (const bf16_t*)W, ldx / 2, ldw / 2, M, N, (K - 128) / 2, (K + 127) / 128, lane, wave, order};
-  Int8Sink<WM, WN, T> sink = {y, ldy, a, w_scale, bias, M, N, lane, wave, vector, order};
-  wide_loop<WM, WN, Int8Sink<WM, WN, T>::STORES, WideInt8<ONCE>>(lds, src, sink, first + idx, blocks, mine, (K + 127) / 128);
+  constexpr bool PARTS = std::is_same<T, int>::value;
+  const int all = (K + 127) / 128, part = PARTS ? (first + idx) / tiles : 0;
+  const int begin = PARTS ? part * all / parts : 0, steps = PARTS ? (part + 1) * all / parts - begin : all;
+  Int8Source<WM, WN> src = {(const bf16_t*)X, (const bf16_t*)W, ldx / 2, ldw / 2, M, N, (K - 128) / 2, begin, steps, lane, wave, order};
+  Int8Sink<WM, WN, T> sink = {y + (size_t)part * M * ldy, ldy, a, w_scale, bias, M, N, lane, wave, vector, order};
+  wide_loop<WM, WN, Int8Sink<WM, WN, T>::STORES, WideInt8<ONCE>>(lds, src, sink, first + idx - part * tiles, blocks, mine, steps);
+}
+
+// The parts' sums, [parts][M][ldp], added, scaled and rounded.  A thread has four columns of a row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+gemm_int8_join_kernel(const int* __restrict__ sums, long ldp, int parts, const float* __restrict__ a, const float* __restrict__ w_scale,
+                      const float* __restrict__ bias, T* __restrict__ y, long ldy, bool vector, int M, int N) {
+  const int n = 4 * (blockIdx.x * 256 + threadIdx.x), m = blockIdx.y;
+  if (n >= N) return;
+  int4v sum = *(const int4v*)(sums + (size_t)m * ldp + n);
+  for (int p = 1; p < parts; ++p) sum += *(const int4v*)(sums + ((size_t)p * M + m) * ldp + n);
+  const float am = a[m];
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int at = min(n + e, N - 1);
+    const float ws = w_scale[at], bs = bias ? bias[at] : 0.f;
+    v[e] = (float)sum[e] * am * ws + bs;
+  }
+  T* row = y + (size_t)m * ldy + n;
+  if (vector && n + 3 < N) {
+    if constexpr (sizeof(T) == 4)
+      *(float4*)row = make_float4(v[0], v[1], v[2], v[3]);
+    else
+      *(uint2*)row = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < N) Elem<T>::store(row + e, v[e]);
+  }
 }
 
 // y = x W^T (+ bias): x [M][x_stride] of x_dtype; W int8 [N][ldw] with its float32 scales [N]; y of y_dtype.  `codes`, `a`: room
 // for the integers of x, [M][K rounded up to 128] bytes, and their scales, M floats (neither with tile -1).
 // `tile`: -1 few rows whose integers every block makes itself (M <= 4); 0 few rows; 1 to 4 the tiles of many rows (256 x 128,
-// 128 x 256, 64 x 128, 128 x 128), which need a K of 128 at least.
+// 128 x 256, 64 x 128, 128 x 128), which need a K of 128 at least.  `parts` > 1 (tiles 3 and 4): K in that many parts, whose sums go to
+// `sums`, [parts][M][N rounded up to 128] 32-bit integers, and are joined by a last launch.
 extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* codes, float* a, const void* W, long ldw, const float* w_scale,
-                               const float* bias, void* y, int dtype, long ldy, int M, int N, int K, int units, int tile, hipStream_t stream) {
+                               const float* bias, void* y, int dtype, long ldy, int M, int N, int K, int units, int tile, int parts, int* sums,
+                               hipStream_t stream) {
   CWM_REQUIRE(M >= 0 && N > 0 && K > 0 && K % 16 == 0 && K <= INT8_MAX_K && units > 0, "linear_int8: bad sizes M=%d N=%d K=%d units=%d", M, N, K, units);
   if (M == 0) return 0;
   CWM_REQUIRE(x && W && w_scale && y, "linear_int8: a tensor is missing");
@@ -476,9 +523,34 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
   CWM_REQUIRE(ldx < (1L << 23) && ldw < (1L << 23), "linear_int8: row strides too long for 32-bit offsets");
   CWM_REQUIRE(tile >= 1 && tile <= 4, "linear_int8: no tile %d", tile);
   const bool vector = ldy % 8 == 0 && (uintptr_t)y % 16 == 0;
+  CWM_REQUIRE(parts >= 1 && parts <= Kp / 128 && (parts == 1 || ((tile == 3 || tile == 4) && sums && (uintptr_t)sums % 16 == 0)),
+              "linear_int8: K in %d parts with tile %d", parts, tile);
+  if (parts > 1) {
+    const long m_tiles = tile == 3 ? (M + 63) / 64 : (M + 127) / 128, n_tiles = (N + 127) / 128, ldp = n_tiles * 128;
+    CWM_REQUIRE(m_tiles * n_tiles * parts <= 65536 && M <= 65535, "linear_int8: too many tiles to take K in parts");
+    const dim3 grid((unsigned)(m_tiles * n_tiles * parts));
+#define INT8_PARTS_RUN(WM, ONCE)                                                                                                              \
+  hipLaunchKernelGGL((gemm_int8_wide_kernel<WM, 2, int, ONCE>), grid, dim3(512), 0, stream, (const int8_t*)X, ldx, a, (const int8_t*)W, ldw, \
+                     w_scale, bias, sums, ldp, true, M, N, K, (int)m_tiles, (int)n_tiles, parts)
+    if (tile == 3 && m_tiles == 1)
+      INT8_PARTS_RUN(2, true);
+    else if (tile == 3)
+      INT8_PARTS_RUN(2, false);
+    else if (m_tiles == 1)
+      INT8_PARTS_RUN(4, true);
+    else
+      INT8_PARTS_RUN(4, false);
+    if (int status = cwm_launch_status("linear_int8 (K in parts)")) return status;
+    const dim3 join((unsigned)((N + 1023) / 1024), (unsigned)M);
+    if (dtype == CWM_BF16)
+      hipLaunchKernelGGL((gemm_int8_join_kernel<bf16_t>), join, dim3(256), 0, stream, sums, ldp, parts, a, w_scale, bias, (bf16_t*)y, ldy, vector, M, N);
+    else
+      hipLaunchKernelGGL((gemm_int8_join_kernel<float>), join, dim3(256), 0, stream, sums, ldp, parts, a, w_scale, bias, (float*)y, ldy, vector, M, N);
+    return cwm_launch_status("linear_int8 (joining parts)");
+  }
 #define INT8_WIDE_RUN(WM, WN, T, ONCE)                                                                                                      \
   hipLaunchKernelGGL((gemm_int8_wide_kernel<WM, WN, T, ONCE>), grid, dim3(512), 0, stream, (const int8_t*)X, ldx, a, (const int8_t*)W, ldw,  \
-                     w_scale, bias, (T*)y, ldy, vector, M, N, K, (int)m_tiles, (int)n_tiles)
+                     w_scale, bias, (T*)y, ldy, vector, M, N, K, (int)m_tiles, (int)n_tiles, 1)
 #define INT8_WIDE(WM, WN)                                                                                          \
   {                                                                                                                \
     const long m_tiles = (M + 32 * WM - 1) / (32 * WM), n_tiles = (N + 64 * WN - 1) / (64 * WN);                   \

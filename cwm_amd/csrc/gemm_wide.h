@@ -65,8 +65,8 @@ template <bool ONCE> struct WideInt8 {  // K goes in steps of 128
   // Sums of integers may be made in any order: with rows of W that are read once, every tile begins at another step of K, so that the
   // blocks' reads of rows of one stride spread over the memory's channels.
   template <typename SOURCE> static __device__ __forceinline__ int at(const SOURCE& src, int step, int steps) {
-    const int turned = step + src.first_step;
-    return !ONCE ? step : turned < steps ? turned : turned - steps;
+    const int turned = step + (ONCE ? src.first_step : 0);
+    return src.begin + (turned < steps ? turned : turned - steps);
   }
   static __device__ __forceinline__ Sums run(const Frag8& w, const Frag8& a, const Sums& c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4v, w.u), __builtin_bit_cast(int4v, a.u), c, 0, 0, 0);

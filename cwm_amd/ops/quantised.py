@@ -29,7 +29,7 @@ _ARGTYPES = {
         _P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P, _P, _I, _P,
     ),
     "cwm_quantize_rows": (_P, _L, _I, _P, _L, _P, _I, _I, _I, _P),
-    "cwm_linear_int8": (_P, _L, _I, _P, _P, _P, _L, _P, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P),
+    "cwm_linear_int8": (_P, _L, _I, _P, _P, _P, _L, _P, _P, _P, _I, _L, _I, _I, _I, _I, _I, _I, _P, _P),
 }
 _entries: dict = {}
 
@@ -374,11 +374,13 @@ def linear_int8(
     bias: Optional[torch.Tensor] = None,
     out_dtype: Optional[torch.dtype] = None,
     tile: Optional[int] = None,
+    parts: int = 1,
 ) -> torch.Tensor:
     """y = x W^T (+ bias) in 8-bit integers: the rows of `x` [M, K] (float32 or bfloat16) are quantised as by `quantize_rows`,
     multiplied with the int8 `weight` [N, K] with exact 32-bit sums, and scaled by the rows' scales and the float32
     `weight_scale` [N] (`quantize_rows` of the weight); `bias` float32 [N].  K a multiple of 16, rows of the weight 16-byte
-    aligned.  Returns [M, N] in `out_dtype` (default: x's).  `tile` (tests) names one of the kernels."""
+    aligned.  Returns [M, N] in `out_dtype` (default: x's).  `tile` (tests) names one of the kernels and
+    `parts` in how many pieces it takes K."""
     KernelError, _check, _code = _base()
     from . import _compute_units
 
@@ -404,17 +406,20 @@ def linear_int8(
     if m == 0:
         return y
     if tile is None:
-        tile = _int8_tile(m, n, k, _compute_units(x.device))
-    codes = scale = None
+        tile, parts = _int8_tile(m, n, k, _compute_units(x.device))
+    codes = scale = sums = joined = None
     if tile >= 0:
         padded = -(-k // 128) * 128
         room = torch.empty(m * (padded + 4), dtype=torch.uint8, device=x.device)  # the integers of x, then their scales
         codes = room.data_ptr()
         scale = codes + m * padded
+    if parts > 1:
+        sums = torch.empty((parts, m, -(-n // 128) * 128), dtype=torch.int32, device=x.device)  # held until the last launch
+        joined = sums.data_ptr()
     function, lib = _entry("gemm_int8", "cwm_linear_int8")
     status = function(
         x.data_ptr(), x.stride(0), x_code, codes, scale, weight.data_ptr(), weight.stride(0) if n > 1 else max(k, weight.stride(0)),
-        weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), code, n, m, n, k, _compute_units(x.device), tile, _stream(),
+        weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), code, n, m, n, k, _compute_units(x.device), tile, parts, joined, _stream(),
     )
     if status:
         _check(lib, status)
@@ -427,13 +432,27 @@ def linear_int8(
 _INT8_TILES = ((1, 256, 128, 2.9, 0.98), (2, 128, 256, 5.6, 0.85), (3, 64, 128, 1.6, 0.38), (4, 128, 128, 3.2, 0.52))
 
 
+_INT8_PARTS_US, _INT8_PARTS_BYTES = 5.0, 4e6  # of joining the parts of K: a launch, and the bytes of their sums a us
+
+
 @functools.lru_cache(maxsize=1024)
-def _int8_tile(m: int, n: int, k: int, units: int) -> int:
-    """The kernel for a product's sizes.  Up to four rows one launch does all (1 x 6,144 x 6,144 14.5 us, in two launches 16.2);
-    up to 16 W is read straight into the matrix instruction (16 x 6,144 x 6,144 20.3 us, tiles of 64 rows 27.2; 16 x 28,672 x 4,096 41.5
-    and 32.1: there the tiles' loads, further ahead, are the faster ones); more rows take the tile of least cost."""
+def _int8_tile(m: int, n: int, k: int, units: int) -> Tuple[int, int]:
+    """The kernel for a product's sizes, and the parts it takes K in.  Up to four rows one launch does all (1 x 6,144 x 6,144 14.5 us, in
+    two launches 16.2); up to 16 W is read straight into the matrix instruction (8 x 6,144 x 6,144 18.4 us, tiles of 64 rows 27.1, with
+    K in parts 20.3; 16 x 28,672 x 4,096 42.1 and 27.1: there the tiles' loads, further ahead, are the faster ones); more rows take the
+    tile of least cost.  Where its tiles are fewer than the compute units, K is taken in parts (33 x 6,144 x 6,144 29.3 us, in five
+    parts 21.2; 64 x 4,096 x 14,336 64.0 and, in eight, 31.7; 64 x 8,192 x 1,024 15.3 and, in two, 20.3, which stays whole)."""
     if m <= INT8_FUSED_ROWS and k <= INT8_FUSED_K // (m if m <= 2 else 4):
-        return -1
+        return -1, 1
     if k < 128 or (m <= INT8_FEW_ROWS and n * k < 1 << 26):
-        return 0
-    return min(_INT8_TILES, key=lambda t: -(-(-(-m // t[1]) * -(-n // t[2])) // units) * (t[3] + -(-k // 128) * t[4]))[0]
+        return 0, 1
+    steps, best = -(-k // 128), None
+    for tile, rows, columns, start, step in _INT8_TILES:
+        tiles = -(-m // rows) * -(-n // columns)
+        for parts in range(1, max(1, min(units // tiles, steps)) + 1 if tile in (3, 4) else 2):
+            cost = -(-tiles * parts // units) * (start + -(-steps // parts) * step)
+            if parts > 1:
+                cost += _INT8_PARTS_US + 8 * parts * m * n / _INT8_PARTS_BYTES
+            if best is None or cost < best[0]:
+                best = (cost, tile, parts)
+    return best[1:]

@@ -86,6 +86,25 @@ def test_products_of_few_rows(dtype):
         _check(x, w, s, None, torch.float32, 0)
 
 
+@pytest.mark.parametrize("tile", [3, 4])
+def test_products_with_k_in_parts(tile):
+    """The parts' sums are whole numbers: whatever the parts, the result is the same."""
+    for i, (m, n, k, parts) in enumerate([(1, 1, 256, 2), (5, 130, 272, 3), (17, 33, 1040, 4), (64, 129, 1168, 9), (65, 70, 2048, 16), (130, 260, 640, 3)]):
+        for dtype in (torch.bfloat16, torch.float32):
+            x = _rows(m, k, dtype, 40 + i)
+            w, s = _weight(n, k, 40 + i, stride=k + 16 * (i % 2))
+            bias = torch.randn(n) if i % 2 else None
+            given = (x.to(DEV), w.to(DEV), s.to(DEV), None if bias is None else bias.to(DEV))
+            for out in (torch.bfloat16, torch.float32):
+                _check(x, w, s, bias, out, tile)
+                assert torch.equal(ops.linear_int8(*given, out, tile, parts), ops.linear_int8(*given, out, tile))
+                assert torch.equal(ops.linear_int8(*given, out), ops.linear_int8(*given, out, tile))
+    with pytest.raises(ops.KernelError, match="parts"):
+        ops.linear_int8(*given, tile=tile, parts=6)
+    with pytest.raises(ops.KernelError, match="parts"):
+        ops.linear_int8(*given, tile=2, parts=2)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_products_of_one_launch(dtype):
     """Up to four rows, whose integers every block makes itself."""
