@@ -52,6 +52,20 @@ def _base():
     return KernelError, _check, _code
 
 
+@functools.cache
+def _planning():
+    from . import _attention_plan, _check_mask, _half_blocks_built, _three_blocks_a_unit
+
+    return _attention_plan, _check_mask, _half_blocks_built, _three_blocks_a_unit
+
+
+@functools.cache
+def _units(device: torch.device) -> int:
+    from . import _compute_units
+
+    return _compute_units(device)
+
+
 def _stream() -> int:
     """The current HIP stream of the current device, as a plain handle."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
@@ -268,8 +282,7 @@ def quant_paged_attention(
     call: `q` [T, Hq, hd] (float32 or bfloat16, rotated), `batch` the step's `StepBatch`, `window` the keys a query reads, its
     own included (None: all).  Returns [T, Hq * hd] in q's type.  A query one of whose keys has no page gets NaN."""
     KernelError, _check, _code = _base()
-    from . import _attention_plan, _check_mask, _half_blocks_built, _three_blocks_a_unit
-
+    _attention_plan, _check_mask, _half_blocks_built, _three_blocks_a_unit = _planning()
     _check_device(q, cache, block_table, batch.cu_q, batch.kv_len)
     _check_mask(window, None, None)
     if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
@@ -382,8 +395,6 @@ def linear_int8(
     aligned.  Returns [M, N] in `out_dtype` (default: x's).  `tile` (tests) names one of the kernels and
     `parts` in how many pieces it takes K."""
     KernelError, _check, _code = _base()
-    from . import _compute_units
-
     _check_device(x, weight, weight_scale, bias)
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise KernelError(f"linear_int8: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
@@ -406,7 +417,7 @@ def linear_int8(
     if m == 0:
         return y
     if tile is None:
-        tile, parts = _int8_tile(m, n, k, _compute_units(x.device))
+        tile, parts = _int8_tile(m, n, k, _units(x.device))
     codes = scale = sums = joined = None
     if tile >= 0:
         padded = -(-k // 128) * 128
@@ -419,7 +430,7 @@ def linear_int8(
     function, lib = _entry("gemm_int8", "cwm_linear_int8")
     status = function(
         x.data_ptr(), x.stride(0), x_code, codes, scale, weight.data_ptr(), weight.stride(0) if n > 1 else max(k, weight.stride(0)),
-        weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), code, n, m, n, k, _compute_units(x.device), tile, parts, joined, _stream(),
+        weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), code, n, m, n, k, _units(x.device), tile, parts, joined, _stream(),
     )
     if status:
         _check(lib, status)
