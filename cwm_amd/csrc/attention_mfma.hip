@@ -53,6 +53,31 @@ CWM_DEFINE_ERROR_API
 #define PARTIAL_STRIDE (HEAD_DIM + 4)  // max and sum after the output; keeps rows 16-byte aligned
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { return pack2_bf16(lo, hi); }
+
+// A library built with -DHALF_INPUTS=1 has the portions' kernel alone, over keys and values in float16 that were unpacked from a
+// cache of fewer bits, with exponents (half_parts.h) for every 32 keys: `exponents` [pages][heads][page size / 32][2], the keys'
+// and the values'.  Queries (bfloat16 as ever) are turned into float16 with an exponent a row, probabilities are float16: what was
+// held in few bits is rounded to 2^-12 of itself where bfloat16 would take 2^-9, and the result to bfloat16 once.
+// A score's exponent is part of its row's scale, or multiplied into a tile's scores where the keys have one; values with another
+// exponent than the sums have rescale the sums, in float32, as a new reference does.  That no tile of an item has exponents is the
+// rule, and found out once an item.
+#ifdef HALF_INPUTS
+#include "half_parts.h"
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+#define PACK_P pack2_f16
+#define WIDE_MFMA(A, B, C) __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, (A).u), __builtin_bit_cast(half8, (B).u), C, 0, 0, 0)
+#define HALF_PARAMS , const int* __restrict__ exponents
+#define LOOK_FOR_EXPONENTS look_for_exponents();
+#define HALF_ENTRY_PARAMS , const int* exponents
+#define HALF_ARGS , exponents
+#else
+#define PACK_P pack_bf16
+#define WIDE_MFMA(A, B, C) __builtin_amdgcn_mfma_f32_16x16x32_bf16((A).v, (B).v, C, 0, 0, 0)
+#define HALF_PARAMS
+#define LOOK_FOR_EXPONENTS
+#define HALF_ENTRY_PARAMS
+#define HALF_ARGS
+#endif
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // One row's share of a 32-key tile of scores: masks (only where a tile reaches past some
@@ -145,7 +170,7 @@ __device__ __forceinline__ float tanh_of(float x) {
       psum += pv[e];                                                                                         \
     }                                                                                                        \
     L_RUN += psum;                                                                                           \
-    PF.u = make_uint4(pack_bf16(pv[0], pv[1]), pack_bf16(pv[2], pv[3]), pack_bf16(pv[4], pv[5]), pack_bf16(pv[6], pv[7])); \
+    PF.u = make_uint4(PACK_P(pv[0], pv[1]), PACK_P(pv[2], pv[3]), PACK_P(pv[4], pv[5]), PACK_P(pv[6], pv[7]));             \
   }
 
 extern "C" int cwm_attention_mfma_head_dim() { return HEAD_DIM; }
@@ -511,7 +536,7 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
                      const int* __restrict__ cu_q, const int* __restrict__ kv_len, const int* __restrict__ work,
                      float* __restrict__ partial, int n_kv_heads_grid, int n_q_heads, int n_kv_heads, int page_size,
                      int page_shift, int num_pages, int window_left, int chunk, float scale_log2e, float cap_raw,
-                      const float* __restrict__ sink, const float* __restrict__ out_scale BIAS_PARAMS KEPT_PARAMS) {
+                      const float* __restrict__ sink, const float* __restrict__ out_scale BIAS_PARAMS KEPT_PARAMS HALF_PARAMS) {
   constexpr bool FAST = MODE != LDS_PLAIN;
   constexpr int DMA_AHEAD = DMA_BUFFERS - 1;
   __shared__ __attribute__((aligned(16))) bf16_t lds_k[MODE == LDS_DMA ? 1 : 2][MODE == LDS_DMA ? 8 : 32 * LDS_K_STRIDE];
@@ -550,7 +575,11 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
   float slope_raw[RT], rate[RT];
 #endif
   const float neg_inf = -__builtin_inff();
+#ifdef HALF_INPUTS
+  float row_scale[RT], row_lazy[RT];
+#else
   const float lazy_raw = 8.0f / scale_log2e;  // 8 binary orders, in units of the raw scores
+#endif
   const float inv_cap_raw = cap_raw > 0.f ? 1.0f / cap_raw : 0.f;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -573,6 +602,26 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
       else
         qf[rt][s].u = make_uint4(0, 0, 0, 0);
     }
+#ifdef HALF_INPUTS
+    float most = 0.f;
+#pragma unroll
+    for (int s = 0; s < K32_STEPS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(bf16_to_f32(qf[rt][s].h[e])));
+    most = fmaxf(most, __shfl_xor(most, 16, 64));
+    most = fmaxf(most, __shfl_xor(most, 32, 64));
+    const int of_row = half_exponent(most);
+    const float down = power_of_two(-of_row);
+    row_scale[rt] = scale_log2e * power_of_two(of_row);
+    row_lazy[rt] = 8.0f / row_scale[rt];
+#pragma unroll
+    for (int s = 0; s < K32_STEPS; ++s) {
+      uint32_t pair[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pair[e] = pack2_f16(bf16_to_f32(qf[rt][s].h[2 * e]) * down, bf16_to_f32(qf[rt][s].h[2 * e + 1]) * down);
+      qf[rt][s].u = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+    }
+#endif
 #pragma unroll
     for (int dt = 0; dt < D_TILES; ++dt) acc[rt][dt] = (float4v){0.f, 0.f, 0.f, 0.f};
     m_run[rt] = neg_inf;
@@ -732,6 +781,26 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
       span_lacks_page(table, table_width, num_pages, page_size, page_shift, max(lo_w, key_begin), min(hi_w, key_end - 1), lane) ||
       (kept_end > 0 && hi_w >= 0 && span_lacks_page(table, table_width, num_pages, page_size, page_shift, 0, kept_end - 1, lane));
 
+#ifdef HALF_INPUTS
+  // the exponents of the keys and of the values of the tile from `kt` on
+  auto exponents_of = [&](int kt) -> int2 {
+    const int lp = page_shift >= 0 ? (kt >> page_shift) : (kt / page_size);
+    const int page = lp < table_width ? table[lp] : -1;
+    if ((unsigned)page >= (unsigned)num_pages) return make_int2(0, 0);
+    return *(const int2*)(exponents + (((size_t)page * n_kv_heads + g) * (page_size / 32) + (kt - lp * page_size) / 32) * 2);
+  };
+  bool with_exponents = false;
+  auto look_for_exponents = [&]() {  // over the item's tiles; called with the first tiles' loads under way
+    bool seen = false;
+    for (int kt = (key_begin & ~31) + 32 * lane; kt < key_end; kt += 32 * 64) {
+      const int2 e = exponents_of(kt);
+      seen = seen || (e.x | e.y) != 0;
+    }
+    with_exponents = __any(seen);
+  };
+  int acc_exponent = 0;  // of the sums of values
+#endif
+
   // one 32-key tile from LDS buffer `buf`: scores, running softmax, weighted values
   auto compute = [&](int kt, bool kept, const bf16_t* kbuf, const bf16_t* vbuf) {
     // a wavefront whose rows all end before this tile, or start after it, has nothing to add
@@ -753,9 +822,22 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
           kf.u = filled ? *(const uint4*)(krow + 8 * j + 32 * s) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
-          st[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.v, qf[rt][s].v, st[rt][t], 0, 0, 0);
+          st[rt][t] = WIDE_MFMA(kf, qf[rt][s], st[rt][t]);
       }
     }
+#ifdef HALF_INPUTS
+    float down = 1.f;  // of the sums of values, to the tile's exponent
+    if (with_exponents) {
+      const int2 of_tile = exponents_of(kt);
+      const float up = power_of_two(of_tile.x);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) st[rt][t] *= up;
+      down = power_of_two(acc_exponent - of_tile.y);
+      acc_exponent = of_tile.y;
+    }
+#endif
     // ---- mask, running maximum, probabilities ------------------------------------------------ //
     const bool need_mask = kept || kt < lo_all || kt + 31 > hi_all;
     float alpha[RT];
@@ -763,9 +845,15 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
     bool moved = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+#ifdef HALF_INPUTS
+      const float scale_log2e = row_scale[rt], lazy_raw = row_lazy[rt];
+#endif
       SOFTMAX_TILE(true, st[rt][0], st[rt][1], need_mask,
                    row_valid[rt] && key <= row_end[rt] && (kept ? key < kept_end : key >= row_start[rt] || (IS_KEPT(key) && key >= key_begin)), m_run[rt],
                    neg_mc_run[rt], l_run[rt], alpha[rt], pf[rt], slope_raw[rt], rate[rt], row_end[rt] - (kt + 8 * j))
+#ifdef HALF_INPUTS
+      alpha[rt] *= down;
+#endif
       moved = moved || alpha[rt] != 1.0f;
     }
     if (__any(moved)) {  // seldom after the first tiles
@@ -788,7 +876,7 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
       vf.u = *(const uint4*)(vrow + dt * 16 * 8);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        acc[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[rt].v, acc[rt][dt], 0, 0, 0);
+        acc[rt][dt] = WIDE_MFMA(vf, pf[rt], acc[rt][dt]);
       }
     }
   };
@@ -881,6 +969,7 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
     };
 #pragma unroll
     for (int t = 0; t < DMA_AHEAD; ++t) dma_next_tile(t);
+    LOOK_FOR_EXPONENTS
     for (int it = 0; it < n_tiles; it += DMA_BUFFERS) {
 #pragma unroll
       for (int u = 0; u < DMA_BUFFERS; ++u) {
@@ -913,6 +1002,7 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
     stash(sa, first_key(0), is_kept(0), 0);
     fetch(sa, first_key(2), is_kept(2), page_next);
     page_next = tile_page(first_key(3));
+    LOOK_FOR_EXPONENTS
     __syncthreads();
     for (int it = 0; it < n_tiles; it += 2) {
       compute(first_key(it), is_kept(it), lds_k[0], lds_v[0]);
@@ -931,6 +1021,7 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
     fetch(sa, first_key(0), 0 < kept_tiles, 0);
     stash(sa, first_key(0), 0 < kept_tiles, 0);
     if (n_tiles > 1) fetch(sa, first_key(1), 1 < kept_tiles, 0);
+    LOOK_FOR_EXPONENTS
     __syncthreads();
     for (int it = 0; it < n_tiles; ++it) {
       const int buf = it & 1;
@@ -949,6 +1040,12 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
     l_row += __shfl_xor(l_row, 16, 64);
     l_row += __shfl_xor(l_row, 32, 64);
     if (!row_valid[rt]) continue;
+#ifdef HALF_INPUTS
+    const float scale_log2e = row_scale[rt];
+    const float up = power_of_two(acc_exponent);
+#pragma unroll
+    for (int dt = 0; dt < D_TILES; ++dt) acc[rt][dt] *= up;
+#endif
     if (w[4] >= 0) {
       // the item's keys are cut into w[5] chunks and this block had one of them: its row tile t
       // leaves what it has at slot w[4] + t * w[5], in the form of the split kernel's partial results
@@ -1069,9 +1166,12 @@ extern "C" int cwm_attention_mfma(const void* q, long q_stride, void* out, long 
                                   int wide_three_blocks, const int* merge,
                                   int n_merge, int n_merge_mid, int n_merge_few, float* partial, int n_q_heads, int n_kv_heads, int head_dim,
                                   int page_size, int num_pages, int window_left, int chunk, float scale, float softcap,
-                                  const float* sink, const float* bias_slope, const float* bias_rate, const float* out_scale, int keep_first,
+                                  const float* sink, const float* bias_slope, const float* bias_rate, const float* out_scale, int keep_first HALF_ENTRY_PARAMS,
                                   hipStream_t stream) {
   // `out_scale`: null, or float32 [tokens][n_q_heads], a factor on a head's finished row
+#ifdef HALF_INPUTS
+  CWM_REQUIRE(n_work == 0 && exponents && page_size % 32 == 0, "attention_mfma: this library has the portions of many rows over keys in float16 alone");
+#endif
 #ifdef KEPT_KEYS
   CWM_REQUIRE(keep_first >= 0 && chunk == 0, "attention_mfma: kept first keys go with a window, not with blocks of keys");
 #define KEPT_ARGS , keep_first
@@ -1108,6 +1208,7 @@ extern "C" int cwm_attention_mfma(const void* q, long q_stride, void* out, long 
     while ((1 << page_shift) < page_size) ++page_shift;
   }
   int status = 0;
+#ifndef HALF_INPUTS
   if (n_work > 0) {
     // a block of four wavefronts per (item, key/value head)
     const long long blocks = (long long)n_work * n_kv_heads;
@@ -1126,6 +1227,7 @@ extern "C" int cwm_attention_mfma(const void* q, long q_stride, void* out, long 
     status = cwm_launch_status("attention_mfma");
     if (status) return status;
   }
+#endif
   if (n_work_wide > 0) {
     const long long blocks = (long long)n_work_wide * n_kv_heads;
     CWM_REQUIRE(blocks <= 0x7fffffffLL, "attention_mfma: too many work items");
@@ -1133,7 +1235,7 @@ extern "C" int cwm_attention_mfma(const void* q, long q_stride, void* out, long 
   hipLaunchKernelGGL((attention_lds_kernel<RT, MODE, BUFFERS, MIN_BLOCKS>), dim3((unsigned)blocks), dim3(256), 0, stream,     \
                      (const bf16_t*)q, q_stride,                                                                          \
                      (bf16_t*)out, out_stride, (const bf16_t*)cache, block_table, table_width, cu_q, kv_len, work_wide,   \
-                     partial, n_kv_heads, n_q_heads, n_kv_heads, page_size, page_shift, num_pages, window_left, chunk, scale_log2e, cap_raw, sink, out_scale BIAS_ARGS KEPT_ARGS)
+                     partial, n_kv_heads, n_q_heads, n_kv_heads, page_size, page_shift, num_pages, window_left, chunk, scale_log2e, cap_raw, sink, out_scale BIAS_ARGS KEPT_ARGS HALF_ARGS)
     if (wide_tiles == 4) {
 #if DMA_HEAD_DIM_OK
       CWM_REQUIRE(page_size % 32 == 0 && (unsigned long long)n_kv_heads * page_size * HEAD_DIM * 2 < (1ull << 31),

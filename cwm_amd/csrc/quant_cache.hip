@@ -3,6 +3,7 @@
 // Both kernels take eight tokens of the list at a time, the tokens of one value block where the list follows a sequence.
 // Writing, four lanes share a group, lane j with its elements 8 j .. + 7: a lane's codes of a key are one piece of memory, the
 // largest and smallest of a group are two exchanges between lanes, and the two elements that a rotation turns are the lane's own.
+#include "half_parts.h"
 #include "quant_cache.h"
 
 CWM_DEFINE_ERROR_API
@@ -444,60 +445,97 @@ quant_kv_read_kernel(T* __restrict__ k, T* __restrict__ v, const int* __restrict
   }
 }
 
-// Unpacks keys and values of whole sequences to bfloat16 in the layout of a cache of that type, [pages][2][heads][PAGE * D], keys
+// Unpacks keys and values of whole sequences to float16 in the layout of a cache of that type, [pages][2][heads][PAGE * D], keys
 // [slot][D], values [slot / 8][D][8], for an attention of many rows: its blocks would each unpack the same keys (a prompt of 2,048
-// tokens with 6 query heads to a key/value head is 96 blocks a head).  List item: {sequence, first key (a multiple of UNPACK_KEYS),
-// page of the unpacked cache}; grid (items, heads, keys and values).  What a query must not read without a NaN (a key without a page, a
-// value held as NaN) becomes a key of NaN with a value of zeros: a masked score takes no part, where zero times NaN would.
+// tokens with 6 query heads to a key/value head is 96 blocks a head).  `exponents` [pages][heads][PAGE / 32][2] has those of the
+// keys and of the values of every 32 tokens (half_parts.h), by the bounds that their words set.  List item: {sequence, first key (a
+// multiple of UNPACK_KEYS), page of the unpacked cache}; grid (items, heads, keys and values).  What a query must not read without a
+// NaN (a key without a page, a value held as NaN) becomes a key of NaN with a value of zeros: a masked score takes no part, where
+// zero times NaN would.
 #define UNPACK_KEYS 64
+// the largest magnitude that a word lets its group have; a NaN counts for nothing (fmaxf)
+template <int BITS> __device__ __forceinline__ float word_bound(uint32_t word) {
+  constexpr float H = 1 << (BITS - 1);
+  const float s = word_step(word), z = word_offset(word);
+  return fmaxf(fmaxf(fabsf(fmaf(-H, s, z)), fabsf(fmaf(H - 1, s, z))), 0.f);
+}
 template <int G, int BITS>
 __global__ void __launch_bounds__(256)
-quant_unpack_kernel(bf16_t* __restrict__ out, int out_page, const int* __restrict__ list, const uint8_t* __restrict__ cache,
+quant_unpack_kernel(uint16_t* __restrict__ out, int* __restrict__ exponents, int out_page, const int* __restrict__ list, const uint8_t* __restrict__ cache,
                     const int* __restrict__ block_table, int table_width, int page_size, int num_pages, const int* __restrict__ kv_len, int n_kv_heads) {
   constexpr int D = 32 * G;
   constexpr int UNITS = BITS == 4 ? D / 2 : D;
   constexpr int H = 1 << (BITS - 1);
   constexpr int WORDS = BITS / 4;
+  __shared__ float tops[UNPACK_KEYS / 16];
   const int* item = list + (size_t)blockIdx.x * 3;
   const int b = item[0], key0 = item[1], head = blockIdx.y;
   const int end = kv_len[b];
   const QuantHead at = quant_head(page_size, D, BITS);
   const size_t plane = (size_t)n_kv_heads * out_page * D;
-  bf16_t* to = out + (size_t)item[2] * 2 * plane + (size_t)head * out_page * D;
+  uint16_t* to = out + (size_t)item[2] * 2 * plane + (size_t)head * out_page * D;
   const int slot0 = key0 % out_page;
+  int* exponents_to = exponents + (((size_t)item[2] * n_kv_heads + head) * (out_page / 32) + slot0 / 32) * 2;
   auto page_of = [&](int key, int& slot) -> const uint8_t* {  // the head's first byte in the key's page
     const int lp = key / page_size;
     slot = key - lp * page_size;
     const int page = lp < table_width ? block_table[(size_t)b * table_width + lp] : -1;
     return page >= 0 && page < num_pages ? cache + ((size_t)page * n_kv_heads + head) * at.bytes : nullptr;
   };
+  auto put8 = [](uint16_t* p, const float(&x)[8]) {
+    *(uint4*)p = make_uint4(pack2_f16(x[0], x[1]), pack2_f16(x[2], x[3]), pack2_f16(x[4], x[5]), pack2_f16(x[6], x[7]));
+  };
+  const int wave = threadIdx.x >> 6;
   if (blockIdx.z == 0) {
     const int key = key0 + (threadIdx.x >> 2), j = threadIdx.x & 3;
-    if (key >= end) return;
     int slot;
-    const uint8_t* from = page_of(key, slot);
+    const uint8_t* from = key < end ? page_of(key, slot) : nullptr;
     uint32_t codes[G * WORDS] = {}, words[G];
-    bool bad = from == nullptr;
-    if (!bad) {
+    const bool held = from != nullptr;
+    bool bad = !held;
+    float most = 0.f;
+    if (held) {
       get_words<G * WORDS>((const uint32_t*)from + ((size_t)slot * 4 + j) * G * WORDS, codes);
       get_words<G>((const uint32_t*)(from + at.key_words) + (size_t)slot * G, words);
       const float vs = word_step(*(const uint32_t*)(from + at.value_words + (size_t)slot * 4));
       bad = vs != vs;
+#pragma unroll
+      for (int g = 0; g < G; ++g) most = fmaxf(most, word_bound<BITS>(words[g]));
     }
-    bf16_t* row = to + (size_t)(slot0 + (threadIdx.x >> 2)) * D + 8 * j;
+    most = wave_max(most);
+    if ((threadIdx.x & 63) == 0) tops[wave] = most;
+    __syncthreads();
+    const int e = half_exponent(fmaxf(tops[wave & ~1], tops[wave | 1]));  // 16 keys a wavefront
+    if ((threadIdx.x & 127) == 0) exponents_to[(threadIdx.x >> 7) * 2] = e;
+    if (key >= end) return;
+    const float down = power_of_two(-e);
+    uint16_t* row = to + (size_t)(slot0 + (threadIdx.x >> 2)) * D + 8 * j;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const float s = bad ? __uint_as_float(0x7fc00000u) : word_step(words[g]), z = bad ? s : word_offset(words[g]);
       float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = BITS == 4 ? (codes[g] >> (4 * (e / 2 + 4 * (e % 2)))) & 15 : (codes[(2 * g + e / 4) % (G * WORDS)] >> (8 * (e & 3))) & 255;
-        x[e] = fmaf(s, (float)(c - H), z);
+      for (int i = 0; i < 8; ++i) {
+        const int c = BITS == 4 ? (codes[g] >> (4 * (i / 2 + 4 * (i % 2)))) & 15 : (codes[(2 * g + i / 4) % (G * WORDS)] >> (8 * (i & 3))) & 255;
+        x[i] = fmaf(s, (float)(c - H), z) * down;
       }
-      store8(row + 32 * g, true, x);
+      put8(row + 32 * g, x);
     }
     return;
   }
+  if (threadIdx.x < UNPACK_KEYS) {
+    const int key = key0 + threadIdx.x;
+    int slot;
+    const uint8_t* from = key < end ? page_of(key, slot) : nullptr;
+    float most = from ? word_bound<BITS>(*(const uint32_t*)(from + at.value_words + (size_t)slot * 4)) : 0.f;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+    if ((threadIdx.x & 31) == 0) {
+      tops[threadIdx.x >> 5] = most;
+      exponents_to[(threadIdx.x >> 5) * 2 + 1] = half_exponent(most);
+    }
+  }
+  __syncthreads();
   for (int i = threadIdx.x; i < UNPACK_KEYS / 8 * UNITS; i += 256) {
     const int block = i / UNITS, u = i - block * UNITS, key = key0 + 8 * block;
     if (key >= end) return;
@@ -509,6 +547,7 @@ quant_unpack_kernel(bf16_t* __restrict__ out, int out_page, const int* __restric
       codes = *(const uint2*)(from + at.values + ((size_t)(slot >> 3) * UNITS + u) * 8);
       get_words<8>((const uint32_t*)(from + at.value_words) + slot, words);
     }
+    const float down = power_of_two(-half_exponent(tops[block >> 2]));
     float x[BITS == 4 ? 2 : 1][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -517,15 +556,15 @@ quant_unpack_kernel(bf16_t* __restrict__ out, int out_page, const int* __restric
       const float s = word_step(words[e]), z = word_offset(words[e]);
       const bool nan = s != s;
       if constexpr (BITS == 4) {
-        x[0][e] = nan ? 0.f : fmaf(s, (float)((c & 15) - H), z);
-        x[1][e] = nan ? 0.f : fmaf(s, (float)((c >> 4) - H), z);
+        x[0][e] = nan ? 0.f : fmaf(s, (float)((c & 15) - H), z) * down;
+        x[1][e] = nan ? 0.f : fmaf(s, (float)((c >> 4) - H), z) * down;
       } else {
-        x[0][e] = nan ? 0.f : fmaf(s, (float)(c - H), z);
+        x[0][e] = nan ? 0.f : fmaf(s, (float)(c - H), z) * down;
       }
     }
-    bf16_t* row = to + plane + ((size_t)((slot0 >> 3) + block) * D + (BITS == 4 ? 2 * u : u)) * 8;
-    store8(row, true, x[0]);
-    if constexpr (BITS == 4) store8(row + 8, true, x[BITS == 4 ? 1 : 0]);
+    uint16_t* row = to + plane + ((size_t)((slot0 >> 3) + block) * D + (BITS == 4 ? 2 * u : u)) * 8;
+    put8(row, x[0]);
+    if constexpr (BITS == 4) put8(row + 8, x[BITS == 4 ? 1 : 0]);
   }
 }
 
@@ -606,17 +645,17 @@ extern "C" int cwm_quant_kv_read(void* k, void* v, int dtype, const int* positio
 
 extern "C" int cwm_quant_unpack_keys() { return UNPACK_KEYS; }
 
-extern "C" int cwm_quant_unpack(void* out, int out_page, const int* list, int n_items, const void* cache, const int* block_table, int table_width,
+extern "C" int cwm_quant_unpack(void* out, int* exponents, int out_page, const int* list, int n_items, const void* cache, const int* block_table, int table_width,
                                 int page_size, int num_pages, const int* kv_len, int n_kv_heads, int head_dim, int bits, hipStream_t stream) {
   QUANT_REQUIRE_SIZES("quant_unpack");
   CWM_REQUIRE(n_items >= 0 && n_kv_heads <= 65535 && out_page > 0 && out_page % UNPACK_KEYS == 0, "quant_unpack: bad sizes");
   if (n_items == 0) return 0;
-  CWM_REQUIRE(out && list && cache && block_table && kv_len, "quant_unpack: a tensor is missing");
+  CWM_REQUIRE(out && exponents && list && cache && block_table && kv_len, "quant_unpack: a tensor is missing");
   CWM_REQUIRE((uintptr_t)cache % 16 == 0 && (uintptr_t)out % 16 == 0, "quant_unpack: tensors must be 16-byte aligned");
   const dim3 grid(n_items, n_kv_heads, 2);
 #define CALL_UNPACK(G, BITS)                                                                                                                   \
-  hipLaunchKernelGGL((quant_unpack_kernel<G, BITS>), grid, dim3(256), 0, stream, (bf16_t*)out, out_page, list, (const uint8_t*)cache, block_table, \
-                     table_width, page_size, num_pages, kv_len, n_kv_heads)
+  hipLaunchKernelGGL((quant_unpack_kernel<G, BITS>), grid, dim3(256), 0, stream, (uint16_t*)out, exponents, out_page, list, (const uint8_t*)cache, \
+                     block_table, table_width, page_size, num_pages, kv_len, n_kv_heads)
   if (bits == 4) {
     FOR_GROUPS(CALL_UNPACK, 4)
   } else {

@@ -75,7 +75,7 @@ SOURCES: Dict[str, Tuple[Mapping[str, int], ...]] = {
     "quant_cache": ({},),
     "gemm_int8": ({},),
     "attention_quant": tuple({"HEAD_DIM": hd} for hd in (32, 64, 96, 128, 160, 192, 224, 256)),
-    "attention_mfma": tuple({"HEAD_DIM": hd} for hd in (16, 32, 48, 64, 80, 96, 128, 160, 192, 224, 256)) + tuple({"DISTANCE_BIAS": 1, "HEAD_DIM": hd} for hd in (32, 48, 64, 128))
+    "attention_mfma": tuple({"HEAD_DIM": hd} for hd in (16, 32, 48, 64, 80, 96, 128, 256)) + tuple({"HALF_INPUTS": 1, "HEAD_DIM": hd} for hd in (32, 64, 96, 128, 160, 192, 224, 256)) + tuple({"DISTANCE_BIAS": 1, "HEAD_DIM": hd} for hd in (32, 48, 64, 128))
     + tuple({"HEAD_DIM": hd, "KEPT_KEYS": 1} for hd in (16, 32, 48, 64, 80, 96, 128, 192)),
 }
 

@@ -24,9 +24,9 @@ _ARGTYPES = {
     "cwm_quant_kv_write": (_P, _L, _P, _L, _P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P),
     "cwm_quant_kv_read": (_P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P),
     "cwm_attention_quant": (_P, _L, _I, _P, _L, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P),
-    "cwm_quant_unpack": (_P, _I, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _I, _P),
+    "cwm_quant_unpack": (_P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _I, _P),
     "cwm_attention_mfma": (
-        _P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P, _P, _I, _P,
+        _P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P, _P, _I, _P, _P,
     ),
     "cwm_quantize_rows": (_P, _L, _I, _P, _L, _P, _I, _I, _I, _P),
     "cwm_linear_int8": (_P, _L, _I, _P, _P, _P, _L, _P, _P, _P, _I, _L, _I, _I, _I, _I, _I, _I, _P, _P),
@@ -34,11 +34,11 @@ _ARGTYPES = {
 _entries: dict = {}
 
 
-def _entry(library: str, name: str, head_dim: Optional[int] = None):
-    """The entry point `name` of a library, and the library (for its error message)."""
+def _entry(library: str, name: str, head_dim: Optional[int] = None, *switches: str):
+    """The entry point `name` of a library built for a head size with the named switches, and the library (for its error message)."""
     found = _entries.get((name, head_dim))
     if found is None:
-        lib = _build.load(library, None if head_dim is None else {"HEAD_DIM": head_dim})
+        lib = _build.load(library, None if head_dim is None else {"HEAD_DIM": head_dim, **dict.fromkeys(switches, 1)})
         function = lib[name]  # an object of its own: other callers of the library hand in objects of ctypes
         function.argtypes = _ARGTYPES[name]
         found = _entries[(name, head_dim)] = (function, lib)
@@ -305,7 +305,7 @@ def quant_paged_attention(
     if n_tokens == 0:
         return out
     group = n_q // n_kv
-    # bfloat16 queries of many rows: their keys and values are unpacked once and read by the attention over a bfloat16 cache
+    # bfloat16 queries of many rows: their keys and values are unpacked once, to float16, and read by the attention over a cache of 16 bits
     plan = _attention_plan(batch, group, n_kv, hd, window, q.device, None, dtype == torch.bfloat16 and _half_blocks_built(n_kv, hd, UNPACK_PAGE), packed=True)
     unpacks = plan.n_wide > 0 and dtype == torch.bfloat16
     partials = partial = None
@@ -327,19 +327,21 @@ def quant_paged_attention(
             _check(lib, status)
     if unpacks:
         listed, n_items, wide_width, n_pages = _unpack_list(batch, group, window, q.device)
-        unpacked = torch.empty((n_pages, 2, n_kv, UNPACK_PAGE * hd), dtype=dtype, device=q.device)
+        held = n_pages * 2 * n_kv * UNPACK_PAGE * hd * 2  # bytes; behind them two exponents for every 32 keys of a head
+        unpacked = torch.empty(held + n_pages * n_kv * (UNPACK_PAGE // 32) * 8, dtype=torch.uint8, device=q.device)
+        exponents = unpacked.data_ptr() + held
         function, lib = _entry("quant_cache", "cwm_quant_unpack")
         status = function(
-            unpacked.data_ptr(), UNPACK_PAGE, listed.data_ptr(), n_items, cache.data_ptr(), table, width, page_size, pages, lengths, n_kv, hd, bits, stream,
+            unpacked.data_ptr(), exponents, UNPACK_PAGE, listed.data_ptr(), n_items, cache.data_ptr(), table, width, page_size, pages, lengths, n_kv, hd, bits, stream,
         )
         if status:
             _check(lib, status)
-        function, lib = _entry("attention_mfma", "cwm_attention_mfma", hd)
+        function, lib = _entry("attention_mfma", "cwm_attention_mfma", hd, "HALF_INPUTS")
         status = function(
             q.data_ptr(), token, out.data_ptr(), n_q * hd, unpacked.data_ptr(), listed.data_ptr() + 12 * n_items, wide_width, first, lengths,
             work, 0, 0, wide, plan.n_wide, plan.item_tiles, _three_blocks_a_unit(plan.n_wide * n_kv, plan.wide_shape, q.device),
             merge, plan.n_merge, plan.n_merge_mid, plan.n_merge_wide, partial, n_q, n_kv, hd, UNPACK_PAGE, n_pages,
-            -1 if window is None else window - 1, 0, scale, 0.0, None, None, None, None, 0, stream,
+            -1 if window is None else window - 1, 0, scale, 0.0, None, None, None, None, 0, exponents, stream,
         )
         if status:
             _check(lib, status)

@@ -163,6 +163,12 @@ class Step:
         )
 
 
+def _most_of_tile(x):
+    """[n, dim] -> [n]: the largest magnitude among the 32 tokens that a token belongs to."""
+    most = torch.nn.functional.pad(x.abs().amax(1), (0, -x.shape[0] % 32)).reshape(-1, 32).amax(1)
+    return most.repeat_interleave(32)[: x.shape[0]]
+
+
 def attention(step, q, keys, values, bits, window, scale):
     """Float64 result [T, Hq * dim] over what the cache holds of `keys` and `values`, and how far a kernel may be off it.
 
@@ -171,9 +177,11 @@ def attention(step, q, keys, values, bits, window, scale):
     s (143 + 136) |q| and |z| |q| with an offset of the codes (bfloat16 queries, 4 bits; 8 bits: 255 + 128), s 2 H |q| without.
     A score that is off by d moves the result by at most 2 d sum p |v|.  bfloat16: the weights p s are rounded to half a step
     and multiply codes less H, and the result is rounded; the sums with the codes' offset, s (OFF' + c), are float32 sums of one
-    term for 32 keys.  bfloat16 portions of more than 128 rows read keys and values unpacked to bfloat16: a score is off by the
-    sum of dim independent roundings of up to half a step, 2^-8 |q k| each, whose deviation is that over sqrt(3) (six of them are
-    allowed), and a value by half a step; the weights p are rounded and multiply whole values."""
+    term for 32 keys.  bfloat16 portions of more than 128 rows read queries, keys and values as float16 with a power of two beside them: a
+    score is off by the sum of dim independent roundings of up to half a step, 2^-11 |q k| each, whose deviation is that over sqrt(3)
+    (six of them are allowed), and a value by half a step; the weights p are rounded and multiply whole values.  What is smaller than
+    2^-14 beside its power of two is off by 2^-25 at most: 2^-17 of the largest query of its row, the largest key or value of its
+    32, and 2^-25 of a weight whose row has one of at least 1."""
     T, heads_q, dim = q.shape
     heads = keys[0].shape[1]
     group = heads_q // heads
@@ -203,9 +211,13 @@ def attention(step, q, keys, values, bits, window, scale):
                 spread = p @ (sv[:, None] * reach + zv[:, None].abs())
                 err = 2 * off[:, None] * (p @ v.abs()) + 2.0 * 2.0 ** -24 * (n / 32 + 40) * spread
                 if not fine and m * group > 128:
-                    off = off + 6 / 3 ** 0.5 * HALF_STEP[q.dtype] * scale * torch.where(seen, (x * x) @ (k * k).t(), torch.zeros_like(size)).sqrt().amax(1)
+                    half_step, least = 2.0 ** -11, 2.0 ** -17
+                    off = off + 6 / 3 ** 0.5 * half_step * scale * torch.where(seen, (x * x) @ (k * k).t(), torch.zeros_like(size)).sqrt().amax(1)
+                    small = x.abs().amax(1)[:, None] * k.abs().sum(1) + x.abs().sum(1)[:, None] * _most_of_tile(k)
+                    off = off + least * scale * torch.where(seen, small, torch.zeros_like(size)).amax(1)
                     err = 2 * off[:, None] * (p @ v.abs()) + 2.0 * 2.0 ** -24 * (n / 32 + 40) * spread
-                    err = err + 2.01 * HALF_STEP[q.dtype] * (p @ v.abs()) + HALF_STEP[q.dtype] * o.abs() * 1.01
+                    err = err + 2.01 * half_step * (p @ v.abs()) + least * (p @ _most_of_tile(v))[:, None] + 2.0 ** -25 * (seen.double() @ v.abs())
+                    err = err + HALF_STEP[q.dtype] * (o.abs() + err)
                 elif not fine:
                     err = err + HALF_STEP[q.dtype] * (p @ (sv[:, None] * (cv - half).abs().double())) + HALF_STEP[q.dtype] * o.abs() * 1.01
                 else:

@@ -226,6 +226,24 @@ def test_scores_that_outgrow_their_reference(bits):
     _close(_attend(step, cache, q, bits, None, 0.125), step, q, keys, values, bits, None, 0.125)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [64, 96, 192])
+def test_portions_whose_numbers_do_not_fit_16_bits(dim, bits):
+    """Queries, keys and values from 2^-60 to 2^60, by row and by some of the tokens."""
+    new, kv, group = [80, 50], [333, 50], 4
+    for i, (of_q, of_k, of_v) in enumerate([(0, 0, 40), (0, 0, -40), (-25, 25, 0), (25, -25, 12), (-60, 60, -30), (3, -14, 60)]):
+        step, cache, q, keys, values = _case(new, kv, 32, group, 1, dim, bits, torch.bfloat16, None, 60 + i)
+        for j, (k, v) in enumerate(zip(keys, values)):
+            k *= 2.0 ** of_k
+            some = torch.arange(v.shape[0]) // 40 % 3 == j
+            v *= torch.where(some, 2.0 ** of_v, 2.0 ** (of_v // 2))[:, None, None].to(v.dtype)
+        keys[0][70:90] *= 2.0 ** -9
+        q *= 2.0 ** of_q
+        q[3:60:7] *= 2.0 ** -8
+        held.put_all(cache, step.table, kv, keys, values, bits)
+        _close(_attend(step, cache, q, bits, None, dim ** -0.5), step, q, keys, values, bits, None, dim ** -0.5)
+
+
 def test_a_key_that_is_not_finite_reaches_its_readers_only():
     new, kv, dim, bits = [12, 1], [60, 300], 64, 4
     step, cache, q, keys, values = _case(new, kv, 16, 4, 2, dim, bits, torch.bfloat16, 20, 11)
