@@ -131,7 +131,10 @@ class Model:
         if bits != 8:
             raise ValueError(f"matrices are held in 8 bits or in the activations' type, not in {bits} bits")
         for block in self.blocks:
-            for part in getattr(block, "parts", {}).values():
+            parts = getattr(block, "parts", None)
+            if parts is None:
+                raise ValueError(f"{type(block).__name__} keeps its parts itself: which of them would hold their matrices in {bits} bits is not known")
+            for part in parts.values():
                 if isinstance(part, (Mixer, FeedForward)) and not part.takes_weight_bits:
                     raise ValueError(f"{type(part).__name__} holds its matrices in the activations' type only, not in {bits} bits")
 

@@ -62,6 +62,8 @@ class LinearWeights:
     def rows(self, start: int, stop: int) -> "LinearWeights":
         """The rows start .. stop - 1 of a joined matrix as a matrix of their own that shares its memory (its streaming
         copy only where both ends fall on a tile of 16 rows or the matrix's end)."""
+        if self.codes is not None:
+            raise ValueError("a matrix of 8-bit integers is not divided: divide it before it is quantised")
         part = LinearWeights(self.weight[start:stop], self.bias[start:stop] if self.bias is not None else None)
         if self.streamed is not None and start % 16 == 0 and (stop % 16 == 0 or stop == self.weight.shape[0]):
             part.streamed = self.streamed[start // 16 : -(-stop // 16)]

@@ -8,6 +8,7 @@ from cwm_amd.config.registry import parse_config
 from cwm_amd.engine import Engine, GenArgs
 from cwm_amd.models.model import Model
 from cwm_amd.parts.base import PagedKVSpec, QuantKVSpec, Runtime
+from cwm_amd.parts.linear import LinearWeights
 from helpers import configs, lapevik
 
 
@@ -56,6 +57,17 @@ def test_models_that_cannot():
         Model(other).bind({}, Runtime(torch.device("cpu"), torch.float32, weight_bits=8))
     with pytest.raises(ValueError, match="8 bits"):
         Model(_plan(configs.get("tiny_b"))).bind({}, Runtime(torch.device("cpu"), torch.float32, weight_bits=4))
+
+
+def test_what_8_bits_are_refused():
+    model = Model(_plan(configs.get("tiny_b")))
+    model.blocks = [object()]
+    with pytest.raises(ValueError, match="keeps its parts itself"):
+        model.bind({}, Runtime(torch.device("cpu"), torch.float32, weight_bits=8))
+    matrix = LinearWeights(torch.randn(32, 64))
+    matrix.codes = torch.zeros(32, 64, dtype=torch.int8)
+    with pytest.raises(ValueError, match="not divided"):
+        matrix.rows(0, 16)
 
 
 def test_an_engine_asks_for_what_its_model_has():
