@@ -29,26 +29,59 @@ __device__ __forceinline__ int int8_of(float x, float a) {
   return (int)rintf(x / a);  // a true quotient: ties are common among short numbers, and a product with 1 / a would decide them otherwise
 }
 
+// The integers of N numbers.  A product with 1 / a decides one except next to a tie, where it may be off by its own rounding (the
+// quotient is at most 127, a reciprocal off by 2^-23 and a product by 2^-24 make it 2.3e-5): there it is the quotient.
+template <int N> __device__ __forceinline__ void int8_all(const float (&x)[N], float a, int (&c)[N]) {
+  const float inv = __builtin_amdgcn_rcpf(a);  // an infinity for the smallest scales
+  float r[N], off = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float t = x[e] * inv;
+    r[e] = rintf(t);
+    off = fmaxf(off, fabsf(t - r[e]));
+  }
+  if (off >= 0.4999f || inv == __builtin_inff()) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) c[e] = int8_of(x[e], a);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) c[e] = (int)r[e];
+  }
+}
+__device__ __forceinline__ uint32_t four_bytes(int a, int b, int c, int d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+}
+
 // One block a row: the largest magnitude, then the integers in a row of Kp.  Zeros fill it up, from K on, or (`shift`, Kp - K) ahead of
 // the integers from the last multiple of 128 on, which then end with the row.  A row with a NaN or an infinity in it has a NaN
 // for its scale (and zeros for its integers).
-template <typename T>
-__global__ void __launch_bounds__(256)
-quantize_rows_kernel(const T* __restrict__ x, long x_stride, int8_t* __restrict__ codes, long c_stride, float* __restrict__ scale, int K, int Kp,
-                     int shift, bool aligned) {
+// PIECES > 0 (rows of whole pieces of eight, 16-byte aligned, up to 4,096 PIECES columns): a thread keeps that many pieces of eight
+// in registers, all loaded at once: few rows are bound by that latency, many by the memory.
+#define ROW_THREADS 512
+template <typename T, int PIECES>
+__global__ void __launch_bounds__(ROW_THREADS)
+quantize_rows_kernel(const T* __restrict__ x, long x_stride, int8_t* __restrict__ codes, long c_stride, float* __restrict__ scale, int K, int Kp, int shift) {
   __shared__ float scratch[16];
   const T* row = x + (size_t)blockIdx.x * x_stride;
   int8_t* out = codes + (size_t)blockIdx.x * c_stride;
+  const int tail = K / 128 * 128;  // from here on the integers move on by `shift`
   uint32_t top = 0;  // magnitudes as integers: an infinity and a NaN are larger than every number
-  if (aligned) {
-    for (int k = 4 * threadIdx.x; k < K; k += 1024) {
-      float v[4];
-      load4(row + k, v);
+  float v[PIECES > 0 ? PIECES : 1][8];
+  if constexpr (PIECES > 0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    for (int i = 0; i < PIECES; ++i) {
+      const int k = min(8 * (int)(threadIdx.x + ROW_THREADS * i), K - 8);  // past the row its last piece again
+      float lo[4], hi[4];
+      load4(row + k, lo), load4(row + k + 4, hi);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] = lo[e], v[i][4 + e] = hi[e];
     }
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
   } else {
-    for (int k = threadIdx.x; k < K; k += 256) top = max(top, __float_as_uint(Elem<T>::load(row + k)) & 0x7fffffffu);
+    for (int k = threadIdx.x; k < K; k += ROW_THREADS) top = max(top, __float_as_uint(Elem<T>::load(row + k)) & 0x7fffffffu);
   }
   // the order of these floats is that of their bits; a NaN becomes an infinity
   const float most = block_max(top >= 0x7f800000u ? __builtin_inff() : __uint_as_float(top), scratch);
@@ -56,24 +89,20 @@ quantize_rows_kernel(const T* __restrict__ x, long x_stride, int8_t* __restrict_
   const float a = most / 127.f;
   if (threadIdx.x == 0) scale[blockIdx.x] = finite ? a : __uint_as_float(0x7fc00000u);
   const bool none = !finite || a == 0.f;
-  const int tail = shift > 0 ? K / 128 * 128 : Kp;  // where the integers move on by `shift`
-  if (aligned) {
-    for (int at = 4 * threadIdx.x; at < Kp; at += 1024) {
-      const int k = at >= tail ? at - shift : at;
-      uint32_t w = 0;
-      if (k < K && (at < tail || k >= tail) && !none) {
-        float v[4];
-        load4(row + k, v);
+  if constexpr (PIECES > 0) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w |= ((uint32_t)int8_of(v[e], a) & 255u) << (8 * e);
-      }
-      *(uint32_t*)(out + at) = w;
+    for (int i = 0; i < PIECES; ++i) {
+      const int k = 8 * (threadIdx.x + ROW_THREADS * i);
+      if (k >= K) break;
+      int c[8] = {};
+      if (!none) int8_all(v[i], a, c);
+      *(uint2*)(out + k + (k >= tail ? shift : 0)) = make_uint2(four_bytes(c[0], c[1], c[2], c[3]), four_bytes(c[4], c[5], c[6], c[7]));
     }
+    const int at = (shift > 0 ? tail : K) + 8 * threadIdx.x;
+    if (8 * threadIdx.x < Kp - K) *(uint2*)(out + at) = make_uint2(0, 0);
   } else {
-    for (int at = threadIdx.x; at < Kp; at += 256) {
-      const int k = at >= tail ? at - shift : at;
-      out[at] = k < K && (at < tail || k >= tail) && !none ? (int8_t)int8_of(Elem<T>::load(row + k), a) : 0;
-    }
+    for (int k = threadIdx.x; k < K; k += ROW_THREADS) out[k + (k >= tail ? shift : 0)] = none ? 0 : (int8_t)int8_of(Elem<T>::load(row + k), a);
+    for (int i = threadIdx.x; i < Kp - K; i += ROW_THREADS) out[(shift > 0 ? tail : K) + i] = 0;
   }
 }
 
@@ -83,11 +112,25 @@ static int quantize_rows(const void* x, long x_stride, int dtype, void* codes, l
   if (M == 0) return 0;
   CWM_REQUIRE(x && codes && scale, "quantize_rows: a tensor is missing");
   const int size = dtype == CWM_BF16 ? 2 : 4;
-  const bool aligned = K % 4 == 0 && Kp % 4 == 0 && x_stride % 4 == 0 && c_stride % 4 == 0 && (uintptr_t)x % (4 * size) == 0 && (uintptr_t)codes % 4 == 0;
-  if (dtype == CWM_BF16)
-    hipLaunchKernelGGL(quantize_rows_kernel<bf16_t>, dim3(M), dim3(256), 0, stream, (const bf16_t*)x, x_stride, (int8_t*)codes, c_stride, scale, K, Kp, shift, aligned);
-  else
-    hipLaunchKernelGGL(quantize_rows_kernel<float>, dim3(M), dim3(256), 0, stream, (const float*)x, x_stride, (int8_t*)codes, c_stride, scale, K, Kp, shift, aligned);
+  const bool whole = K % 8 == 0 && Kp % 8 == 0 && x_stride * size % 16 == 0 && c_stride % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)codes % 8 == 0;
+  const int pieces = !whole || K > 32 * ROW_THREADS ? 0 : K <= 8 * ROW_THREADS ? 1 : K <= 16 * ROW_THREADS ? 2 : 4;
+  CWM_REQUIRE(shift == 0 || shift == Kp - K, "quantize_rows: integers move on to the end of their row or not at all");
+#define QUANTIZE_ROWS(T, PIECES) \
+  hipLaunchKernelGGL((quantize_rows_kernel<T, PIECES>), dim3(M), dim3(ROW_THREADS), 0, stream, (const T*)x, x_stride, (int8_t*)codes, c_stride, scale, K, Kp, shift)
+#define QUANTIZE_PIECES(T)    \
+  if (pieces == 0)            \
+    QUANTIZE_ROWS(T, 0);      \
+  else if (pieces == 1)       \
+    QUANTIZE_ROWS(T, 1);      \
+  else if (pieces == 2)       \
+    QUANTIZE_ROWS(T, 2);      \
+  else                        \
+    QUANTIZE_ROWS(T, 4)
+  if (dtype == CWM_BF16) {
+    QUANTIZE_PIECES(bf16_t);
+  } else {
+    QUANTIZE_PIECES(float);
+  }
   return cwm_launch_status("quantize_rows");
 }
 
@@ -180,12 +223,9 @@ gemm_int8_few_kernel(const int8_t* __restrict__ X, long ldx, const float* __rest
     for (int i = 0; i < FUSED_SLOTS; ++i) {
       const int m = i / A_ROW, k = i % A_ROW * FUSED_SLOT + 4 * threadIdx.x;
       if (m >= M || k >= Kp) continue;
-      uint32_t c = 0;
-      if (scale_row[m] > 0.f) {  // not of a row of zeros, nor where it is a NaN
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c |= ((uint32_t)int8_of(v[i][e], scale_row[m]) & 255u) << (8 * e);
-      }
-      *(uint32_t*)(codes + (size_t)m * Kp + k) = c;
+      int c[4] = {};
+      if (scale_row[m] > 0.f) int8_all(v[i], scale_row[m], c);  // not of a row of zeros, nor where it is a NaN
+      *(uint32_t*)(codes + (size_t)m * Kp + k) = four_bytes(c[0], c[1], c[2], c[3]);
     }
     __syncthreads();
   } else {
@@ -400,7 +440,7 @@ gemm_int8_wide_kernel(const int8_t* __restrict__ X, long ldx, const float* __res
   const int begin = PARTS ? part * all / parts : 0, steps = PARTS ? (part + 1) * all / parts - begin : all;
   Int8Source<WM, WN> src = {(const bf16_t*)X, (const bf16_t*)W, ldx / 2, ldw / 2, M, N, (K - 128) / 2, begin, steps, lane, wave, order};
   Int8Sink<WM, WN, T> sink = {y + (size_t)part * M * ldy, ldy, a, w_scale, bias, M, N, lane, wave, vector, order};
-  wide_loop<WM, WN, Int8Sink<WM, WN, T>::STORES, WideInt8<ONCE>>(lds, src, sink, first + idx - part * tiles, blocks, mine, steps);
+  wide_loop<WM, WN, Int8Sink<WM, WN, T>::STORES, WideInt8<ONCE, PARTS>>(lds, src, sink, first + idx - part * tiles, blocks, mine, steps);
 }
 
 // The parts' sums, [parts][M][ldp], added, scaled and rounded.  A thread has four columns of a row.

@@ -54,7 +54,7 @@ struct WideBf16 {
   static __device__ __forceinline__ Sums run(const Frag8& w, const Frag8& a, const Sums& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v, a.v, c, 0, 0, 0); }
 };
 typedef int int4v __attribute__((ext_vector_type(4)));
-template <bool ONCE> struct WideInt8 {  // K goes in steps of 128
+template <bool ONCE, bool PARTS> struct WideInt8 {  // K goes in steps of 128; PARTS: from the source's step `begin` on
   typedef int4v Sums;
   static constexpr bool W_ONCE = ONCE;
   // A last step that reaches past K begins earlier instead, at the row's end less a step: A's row has zeros in the place of what
@@ -65,8 +65,11 @@ template <bool ONCE> struct WideInt8 {  // K goes in steps of 128
   // Sums of integers may be made in any order: with rows of W that are read once, every tile begins at another step of K, so that the
   // blocks' reads of rows of one stride spread over the memory's channels.
   template <typename SOURCE> static __device__ __forceinline__ int at(const SOURCE& src, int step, int steps) {
-    const int turned = step + (ONCE ? src.first_step : 0);
-    return src.begin + (turned < steps ? turned : turned - steps);
+    if constexpr (ONCE) {
+      step += src.first_step;
+      step = step < steps ? step : step - steps;
+    }
+    return step + (PARTS ? src.begin : 0);
   }
   static __device__ __forceinline__ Sums run(const Frag8& w, const Frag8& a, const Sums& c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4v, w.u), __builtin_bit_cast(int4v, a.u), c, 0, 0, 0);
