@@ -5,7 +5,10 @@
 // 2^24), twice by the scales, and once to its type.
 //
 // Few rows: every byte of W is read once, straight into the matrix instruction's operand, and the product is bound by that
-// reading.  More rows: gemm_wide.h's loop.
+// reading (one row by 6,144 x 6,144: 13.2 us, 37.7 MB, of which a launch and the latencies of two reads are 5).
+// More rows: gemm_wide.h's loop.  Up to 64 rows it is bound by the reading of W (37 x 28,672 x 4,096: 23 us, 5.1 TB/s); 2,048 x
+// 43,008 x 6,144 runs at 2.2 POP/s in 490 us, bound by LDS and matrix cores in turn: by count a step's operands are read in 0.43 us and
+// multiplied in 0.43, and the step takes 0.85 (in bfloat16, with twice the products' time for as many bytes, the reads hide).
 #include <type_traits>
 
 #include "gemm_wide.h"
@@ -489,8 +492,8 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
   const int x_size = x_dtype == CWM_BF16 ? 2 : 4, Kp = (K + 127) / 128 * 128;
   const int a_wave = (K / 128 + FEW_WAVES - 1) / FEW_WAVES;  // pieces of a wavefront of few rows
   // Two blocks a compute unit stay, each with the same number of rows of W: what one unit can have in flight is limited, so with
-  // tiles dealt out one by one the units that get one more take that much longer (6,144 rows: 384 tiles 12.7 us, 512 blocks of 12
-  // rows 9).
+  // tiles dealt out one by one the units that get one more take that much longer (one row by 6,144 of 6,144: 384 tiles 14.6 us,
+  // 512 blocks of 12 rows 13.2).
   const int few_rows = (N + 2 * units - 1) / (2 * units) > 4 ? (N + 2 * units - 1) / (2 * units) : 4, few_blocks = (N + few_rows - 1) / few_rows;
   if (tile == -1) {
     const int rows = M <= 2 ? M : 4;
@@ -533,24 +536,20 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
   const int8_t* X = (const int8_t*)codes;
   const long ldx = Kp;
   if (tile == 0) {
-    const int row_tiles = (M + 15) / 16, rt = row_tiles >= 4 ? 4 : row_tiles >= 2 ? 2 : 1;
+    const int row_tiles = (M + 15) / 16, rt = row_tiles > 1 ? 4 : 1;  // more than one for a K below a tile's
     CWM_REQUIRE((row_tiles + rt - 1) / rt <= 65535, "linear_int8: too many rows");
     const dim3 grid(few_blocks, (row_tiles + rt - 1) / rt);
 #define INT8_FEW(T, RT, AHEAD)                                                                                                                       \
   hipLaunchKernelGGL((gemm_int8_few_kernel<float, T, RT, 0, AHEAD>), grid, dim3(64 * FEW_WAVES), 0, stream, X, ldx, a, (const float*)nullptr, 0l, \
                      false, (const int8_t*)W, ldw, w_scale, bias, (T*)y, ldy, M, N, K, few_rows)
-#define INT8_FEW_ROWS(T)          \
-  if (rt == 4)                    \
-    INT8_FEW(T, 4, 2);            \
-  else if (rt == 2 && a_wave <= 2) \
-    INT8_FEW(T, 2, 2);            \
-  else if (rt == 2)               \
-    INT8_FEW(T, 2, 4);            \
-  else if (a_wave <= 2)           \
-    INT8_FEW(T, 1, 2);            \
+#define INT8_FEW_ROWS(T)               \
+  if (rt == 4)                         \
+    INT8_FEW(T, 4, 2);                 \
+  else if (a_wave <= 2)                \
+    INT8_FEW(T, 1, 2);                 \
   else if (a_wave <= 4 || a_wave == 8) \
-    INT8_FEW(T, 1, 4);            \
-  else                            \
+    INT8_FEW(T, 1, 4);                 \
+  else                                 \
     INT8_FEW(T, 1, 6)
     if (dtype == CWM_BF16) {
       INT8_FEW_ROWS(bf16_t);

@@ -338,7 +338,8 @@ quant_kv_write_kernel(const T* __restrict__ k, long k_stride, const T* __restric
 }
 
 // Reads the tokens of a list: grid (chunks of eight tokens, groups of eight heads: keys, then values).  Bound by memory, most of it the
-// written rows: neighbouring lanes write neighbouring pieces, whole cache lines an instruction.
+// written rows: neighbouring lanes write neighbouring pieces, whole cache lines an instruction (131,072 tokens of 8 heads of 128 in 4
+// bits: 690 MB in 169 us, 4.1 TB/s where a plain copy has 4.85; with a lane for a token's eight elements of all groups 246).
 template <typename T, int G, int BITS>
 __global__ void __launch_bounds__(256)
 quant_kv_read_kernel(T* __restrict__ k, T* __restrict__ v, const int* __restrict__ positions, const int* __restrict__ seq_of_token,
@@ -447,7 +448,8 @@ quant_kv_read_kernel(T* __restrict__ k, T* __restrict__ v, const int* __restrict
 
 // Unpacks keys and values of whole sequences to float16 in the layout of a cache of that type, [pages][2][heads][PAGE * D], keys
 // [slot][D], values [slot / 8][D][8], for an attention of many rows: its blocks would each unpack the same keys (a prompt of 2,048
-// tokens with 6 query heads to a key/value head is 96 blocks a head).  `exponents` [pages][heads][PAGE / 32][2] has those of the
+// tokens with 6 query heads to a key/value head is 96 blocks a head: the two launches take 8 and 78 us, one whose blocks
+// unpacked for themselves took 197).  `exponents` [pages][heads][PAGE / 32][2] has those of the
 // keys and of the values of every 32 tokens (half_parts.h), by the bounds that their words set.  List item: {sequence, first key (a
 // multiple of UNPACK_KEYS), page of the unpacked cache}; grid (items, heads, keys and values).  What a query must not read without a
 // NaN (a key without a page, a value held as NaN) becomes a key of NaN with a value of zeros: a masked score takes no part, where
