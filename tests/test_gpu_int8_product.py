@@ -46,6 +46,23 @@ def test_integers_of_rows(m, k, dtype):
     assert torch.equal(codes.cpu(), want) and torch.equal(scale.cpu(), a)
 
 
+@pytest.mark.parametrize("k", [8, 120, 4104, 8200, 16392, 32768, 32776])
+def test_integers_of_long_rows_ties_and_the_ends_of_the_range(k):
+    """Rows of which a thread keeps one to eight pieces, or none; quotients that are ties; scales whose reciprocal is no float32."""
+    for dtype in (torch.bfloat16, torch.float32):
+        x = _rows(5, k, dtype, k)
+        x[1] = (torch.arange(k) % 255 - 127) / 2
+        x[1, 3] = 127.0  # a scale of 1: every second quotient is a tie
+        x[2] *= 1e-39
+        x[3] = 0
+        x[3, k // 2] = 3e38
+        x[4, k - 1] = 1000.0
+        codes, scale = ops.quantize_rows(x.to(DEV))
+        want, a = _quantised(x)
+        assert torch.equal(codes.cpu(), want) and torch.equal(scale.cpu(), a)
+        assert not codes._base[:, k:].any()
+
+
 def test_rows_that_are_not_finite():
     x = _rows(5, 64, torch.float32, 1)
     x[1, 3], x[2, 60], x[3, 0] = math.nan, math.inf, -math.inf
