@@ -11,14 +11,16 @@
 // where the second sum is one more matrix product, of the words (offset, step) of a key, which are already pairs of
 // bfloat16 numbers in a register, with the query's sums in three bfloat16 parts; and a product of the words with a column
 // that is 1 at one place brings a group's step to the lanes that hold its scores.  No vector instruction touches a word.
-//     o = sum_j p_j v_j = sum_j b_j (OFF' + c_j) - OFF sum_j b_j + sum_j p_j z_j,   b_j = p_j s_j rounded to bfloat16
+//     o = sum_j p_j v_j = sum_j b_j (OFF' + c_j) - OFF sum_j b_j + sum_j p_j z_j,   b_j = p_j s_j in two bfloat16 parts
 // The sum of the b_j is one more matrix product (a row of ones), so that it holds the same rounded numbers; the last sum is
-// kept in float32.  The rounding of b is that of p in the attention over a bfloat16 cache, and multiplies c - H, not c.
+// kept in float32.  One part would round the weights to 2^-8 of themselves, as much as the result is rounded; the second takes
+// that to 2^-16 for 2 us of 60 (the step below), since the matrix cores wait for the cache.
 // float32 queries: q and b in three bfloat16 parts each, codes without an offset (c - H is exact in bfloat16).
 //
 // Decoded tokens are bound by the reading of the cache: eight sequences of 32,768 tokens, 48 query heads on 8 of 128, 4 bits: 310 MB in
-// 60 us (5.2 TB/s; a plain read has 6.9) and 5 for joining the chunks; in bfloat16 the same step reads 1,074 MB in 178.  A wavefront's
-// loads run two tiles ahead of its arithmetic; eight wavefronts a block instead of four take 77 us.  A step of few keys is bound by its latencies (1,000 keys: 11.4 us).
+// 62 us (5.0 TB/s; a plain read has 6.9) and 5 for joining the chunks; in bfloat16 the same step reads 1,074 MB in 178.  A wavefront's
+// loads run two tiles ahead of its arithmetic; eight wavefronts a block instead of four take 77 us.  A step of few keys is bound by its
+// latencies (1,000 keys: 11.4 us).
 //
 // Lanes as in the attention over a bfloat16 cache (lane 16 j + n): S^T = K Q^T leaves lane (row n, j) the keys 8 j .. 8 j + 7
 // of 32, which is the operand of O^T = V^T P^T, so probabilities never move.
@@ -143,6 +145,7 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
                        int num_pages, int window_left, float scale_log2e) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int PARTS = EXACT ? 3 : 1;
+  constexpr int B_PARTS = EXACT ? 3 : 2;  // of a weight
   typedef Codes<BITS, EXACT> C;
   typedef KeyTile<BITS> Keys;
   const float neg_inf = -__builtin_inff();
@@ -350,7 +353,7 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
       }
     }
     const bool need_mask = kt < lo_all || kt + 31 > hi_all;
-    Frag8 bf[RT][PARTS];
+    Frag8 bf[RT][B_PARTS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float x[8] = {st[rt][0][0], st[rt][0][1], st[rt][0][2], st[rt][0][3], st[rt][1][0], st[rt][1][1], st[rt][1][2], st[rt][1][3]};
@@ -400,9 +403,18 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
       }
       l_run[rt] = l_even + l_odd, z_run[rt] = z_even + z_odd;
       if constexpr (EXACT) {
-        Frag8 part[3]; three_parts(bv, part); bf[rt][0] = part[0], bf[rt][1 % PARTS] = part[1], bf[rt][2 % PARTS] = part[2];
+        Frag8 part[3];
+        three_parts(bv, part);
+        bf[rt][0] = part[0], bf[rt][1] = part[1], bf[rt][2 % B_PARTS] = part[2];
       } else {
         bf[rt][0].u = make_uint4(pack2_bf16(bv[0], bv[1]), pack2_bf16(bv[2], bv[3]), pack2_bf16(bv[4], bv[5]), pack2_bf16(bv[6], bv[7]));
+        uint32_t rest[4];
+        const uint32_t whole[4] = {bf[rt][0].u.x, bf[rt][0].u.y, bf[rt][0].u.z, bf[rt][0].u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          rest[i] = pack2_bf16(bv[2 * i] - __uint_as_float(whole[i] << 16), bv[2 * i + 1] - __uint_as_float(whole[i] & 0xffff0000u));
+        bf[rt][1].u = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+        bsum[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones.v, bf[rt][1].v, bsum[rt], 0, 0, 0);
         bsum[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones.v, bf[rt][0].v, bsum[rt], 0, 0, 0);
       }
     }
@@ -421,7 +433,7 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int p = PARTS - 1; p >= 0; --p) acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, bf[rt][p].v, acc[rt][d], 0, 0, 0);
+        for (int p = B_PARTS - 1; p >= 0; --p) acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, bf[rt][p].v, acc[rt][d], 0, 0, 0);
     }
   };
 

@@ -175,8 +175,8 @@ def attention(step, q, keys, values, bits, window, scale):
     A kernel's scores are float32 sums of at most dim + 40 terms of the matrix instructions and of the groups, each rounded
     (2^-24 of the largest partial sum, twice for sums whose order is the instruction's): the terms are at most
     s (143 + 136) |q| and |z| |q| with an offset of the codes (bfloat16 queries, 4 bits; 8 bits: 255 + 128), s 2 H |q| without.
-    A score that is off by d moves the result by at most 2 d sum p |v|.  bfloat16: the weights p s are rounded to half a step
-    and multiply codes less H, and the result is rounded; the sums with the codes' offset, s (OFF' + c), are float32 sums of one
+    A score that is off by d moves the result by at most 2 d sum p |v|.  bfloat16: the weights p s are two parts of
+    half a step of half a step together and multiply codes less H, and the result is rounded; the sums with the codes' offset, s (OFF' + c), are float32 sums of one
     term for 32 keys.  bfloat16 portions of more than 128 rows read queries, keys and values as float16 with a power of two beside them: a
     score is off by the sum of dim independent roundings of up to half a step, 2^-11 |q k| each, whose deviation is that over sqrt(3)
     (six of them are allowed), and a value by half a step; the weights p are rounded and multiply whole values.  What is smaller than
@@ -219,7 +219,8 @@ def attention(step, q, keys, values, bits, window, scale):
                     err = err + 2.01 * half_step * (p @ v.abs()) + least * (p @ _most_of_tile(v))[:, None] + 2.0 ** -25 * (seen.double() @ v.abs())
                     err = err + HALF_STEP[q.dtype] * (o.abs() + err)
                 elif not fine:
-                    err = err + HALF_STEP[q.dtype] * (p @ (sv[:, None] * (cv - half).abs().double())) + HALF_STEP[q.dtype] * o.abs() * 1.01
+                    err = err + 2.0 ** -16 * (p @ (sv[:, None] * (cv - half).abs().double()))
+                    err = err + HALF_STEP[q.dtype] * (o.abs() + err)
                 else:
                     err = err + 2.0 ** -23 * o.abs()
                 limit[t0 : t0 + m, g] = err
