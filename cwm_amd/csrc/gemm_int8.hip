@@ -357,7 +357,6 @@ struct Int8Sink {
   long ldc;
   const float *a, *w_scale, *bias;
   int M, N, lane, wave;
-  bool vector;
   Int8Order order;
   static constexpr int STORES = sizeof(T) == 4 ? WM * WN : WM * WN / 2;
 
@@ -390,7 +389,7 @@ struct Int8Sink {
       // Waited for here, by an instruction that the compiler knows of: loads that it takes to be under way at the loop's head
       // make it wait for all of the loop's own loads in every step (2,048 x 43,008 x 6,144 663 us, 1.24 us a step).
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-      const bool full = vector && (tm + 1) * BM <= M && (tn + 1) * BN <= N;
+      const bool full = (tm + 1) * BM <= M && (tn + 1) * BN <= N;
 #pragma unroll
       for (int i = 0; i < WM; ++i) {
         const int m = m0 + 16 * i;
@@ -403,13 +402,14 @@ struct Int8Sink {
           for (int e = 0; e < 4; ++e) v[b][e] = (float)acc[i][b][e] * am[i] * ws[b][e] + bs[b][e];
 #pragma unroll
         for (int b = 0; b < WN; b += 2) {
-          if (vector && n0 + 4 * b + 7 < N) {
+          if (n0 + 4 * b + 7 < N) {  // a row may begin anywhere: 16 bytes to any address
             if constexpr (sizeof(T) == 4) {
-              *(float4*)(row + 4 * b) = make_float4(v[b][0], v[b][1], v[b][2], v[b][3]);
-              *(float4*)(row + 4 * b + 4) = make_float4(v[b + 1][0], v[b + 1][1], v[b + 1][2], v[b + 1][3]);
+              __builtin_memcpy(row + 4 * b, v[b], 16);
+              __builtin_memcpy(row + 4 * b + 4, v[b + 1], 16);
             } else {
-              *(uint4*)(row + 4 * b) = make_uint4(pack2_bf16(v[b][0], v[b][1]), pack2_bf16(v[b][2], v[b][3]), pack2_bf16(v[b + 1][0], v[b + 1][1]),
-                                                  pack2_bf16(v[b + 1][2], v[b + 1][3]));
+              const uint4 w = make_uint4(pack2_bf16(v[b][0], v[b][1]), pack2_bf16(v[b][2], v[b][3]), pack2_bf16(v[b + 1][0], v[b + 1][1]),
+                                         pack2_bf16(v[b + 1][2], v[b + 1][3]));
+              __builtin_memcpy(row + 4 * b, &w, 16);
             }
           } else {
 #pragma unroll
@@ -427,7 +427,7 @@ struct Int8Sink {
 template <int WM, int WN, typename T, bool ONCE>
 __global__ void __launch_bounds__(512, 2)
 gemm_int8_wide_kernel(const int8_t* __restrict__ X, long ldx, const float* __restrict__ a, const int8_t* __restrict__ W, long ldw,
-                      const float* __restrict__ w_scale, const float* __restrict__ bias, T* __restrict__ y, long ldy, bool vector, int M, int N,
+                      const float* __restrict__ w_scale, const float* __restrict__ bias, T* __restrict__ y, long ldy, int M, int N,
                       int K, int m_tiles, int n_tiles, int parts) {
   typedef WideShape<WM, WN> Shape;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[Shape::S * Shape::STAGE];
@@ -445,7 +445,7 @@ gemm_int8_wide_kernel(const int8_t* __restrict__ X, long ldx, const float* __res
   const int all = (K + 127) / 128, part = PARTS ? (first + idx) / tiles : 0;
   const int begin = PARTS ? part * all / parts : 0, steps = PARTS ? (part + 1) * all / parts - begin : all;
   Int8Source<WM, WN> src = {(const bf16_t*)X, (const bf16_t*)W, ldx / 2, ldw / 2, M, N, (K - 128) / 2, begin, steps, lane, wave, order};
-  Int8Sink<WM, WN, T> sink = {y + (size_t)part * M * ldy, ldy, a, w_scale, bias, M, N, lane, wave, vector, order};
+  Int8Sink<WM, WN, T> sink = {y + (size_t)part * M * ldy, ldy, a, w_scale, bias, M, N, lane, wave, order};
   wide_loop<WM, WN, Int8Sink<WM, WN, T>::STORES, WideInt8<ONCE, PARTS>>(lds, src, sink, first + idx - part * tiles, blocks, mine, steps);
 }
 
@@ -453,7 +453,7 @@ gemm_int8_wide_kernel(const int8_t* __restrict__ X, long ldx, const float* __res
 template <typename T>
 __global__ void __launch_bounds__(256)
 gemm_int8_join_kernel(const int* __restrict__ sums, long ldp, int parts, const float* __restrict__ a, const float* __restrict__ w_scale,
-                      const float* __restrict__ bias, T* __restrict__ y, long ldy, bool vector, int M, int N) {
+                      const float* __restrict__ bias, T* __restrict__ y, long ldy, int M, int N) {
   const int n = 4 * (blockIdx.x * 256 + threadIdx.x), m = blockIdx.y;
   if (n >= N) return;
   int4v sum = *(const int4v*)(sums + (size_t)m * ldp + n);
@@ -467,11 +467,13 @@ gemm_int8_join_kernel(const int* __restrict__ sums, long ldp, int parts, const f
     v[e] = (float)sum[e] * am * ws + bs;
   }
   T* row = y + (size_t)m * ldy + n;
-  if (vector && n + 3 < N) {
-    if constexpr (sizeof(T) == 4)
-      *(float4*)row = make_float4(v[0], v[1], v[2], v[3]);
-    else
-      *(uint2*)row = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+  if (n + 3 < N) {
+    if constexpr (sizeof(T) == 4) {
+      __builtin_memcpy(row, v, 16);
+    } else {
+      const uint2 w = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+      __builtin_memcpy(row, &w, 8);
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -564,7 +566,6 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
   CWM_REQUIRE(K >= 128, "linear_int8: the tiles of many rows take a K of 128 and more, not %d", K);
   CWM_REQUIRE(ldx < (1L << 23) && ldw < (1L << 23), "linear_int8: row strides too long for 32-bit offsets");
   CWM_REQUIRE(tile >= 1 && tile <= 4, "linear_int8: no tile %d", tile);
-  const bool vector = ldy % 8 == 0 && (uintptr_t)y % 16 == 0;
   CWM_REQUIRE(parts >= 1 && parts <= Kp / 128 && (parts == 1 || ((tile == 3 || tile == 4) && sums && (uintptr_t)sums % 16 == 0)),
               "linear_int8: K in %d parts with tile %d", parts, tile);
   if (parts > 1) {
@@ -573,7 +574,7 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
     const dim3 grid((unsigned)(m_tiles * n_tiles * parts));
 #define INT8_PARTS_RUN(WM, ONCE)                                                                                                              \
   hipLaunchKernelGGL((gemm_int8_wide_kernel<WM, 2, int, ONCE>), grid, dim3(512), 0, stream, (const int8_t*)X, ldx, a, (const int8_t*)W, ldw, \
-                     w_scale, bias, sums, ldp, true, M, N, K, (int)m_tiles, (int)n_tiles, parts)
+                     w_scale, bias, sums, ldp, M, N, K, (int)m_tiles, (int)n_tiles, parts)
     if (tile == 3 && m_tiles == 1)
       INT8_PARTS_RUN(2, true);
     else if (tile == 3)
@@ -585,14 +586,14 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
     if (int status = cwm_launch_status("linear_int8 (K in parts)")) return status;
     const dim3 join((unsigned)((N + 1023) / 1024), (unsigned)M);
     if (dtype == CWM_BF16)
-      hipLaunchKernelGGL((gemm_int8_join_kernel<bf16_t>), join, dim3(256), 0, stream, sums, ldp, parts, a, w_scale, bias, (bf16_t*)y, ldy, vector, M, N);
+      hipLaunchKernelGGL((gemm_int8_join_kernel<bf16_t>), join, dim3(256), 0, stream, sums, ldp, parts, a, w_scale, bias, (bf16_t*)y, ldy, M, N);
     else
-      hipLaunchKernelGGL((gemm_int8_join_kernel<float>), join, dim3(256), 0, stream, sums, ldp, parts, a, w_scale, bias, (float*)y, ldy, vector, M, N);
+      hipLaunchKernelGGL((gemm_int8_join_kernel<float>), join, dim3(256), 0, stream, sums, ldp, parts, a, w_scale, bias, (float*)y, ldy, M, N);
     return cwm_launch_status("linear_int8 (joining parts)");
   }
 #define INT8_WIDE_RUN(WM, WN, T, ONCE)                                                                                                      \
   hipLaunchKernelGGL((gemm_int8_wide_kernel<WM, WN, T, ONCE>), grid, dim3(512), 0, stream, (const int8_t*)X, ldx, a, (const int8_t*)W, ldw,  \
-                     w_scale, bias, (T*)y, ldy, vector, M, N, K, (int)m_tiles, (int)n_tiles, 1)
+                     w_scale, bias, (T*)y, ldy, M, N, K, (int)m_tiles, (int)n_tiles, 1)
 #define INT8_WIDE(WM, WN)                                                                                          \
   {                                                                                                                \
     const long m_tiles = (M + 32 * WM - 1) / (32 * WM), n_tiles = (N + 64 * WN - 1) / (64 * WN);                   \
