@@ -257,8 +257,11 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
     return (page >= 0 && page < num_pages) ? page : 0;
   };
   const int krel = 8 * (n >> 2) + (n & 3);
-  // as many tiles' registers as there is room for: 4 bits and heads of up to 128 three, others two
-  constexpr int BUFFERS = PAGE32 && BITS == 4 && !EXACT && HEAD_DIM <= 128 ? 3 : 2;
+  // As many tiles' registers as there is room for: three in the lightest case, else two where they fit beside sums and queries (by
+  // count, with 60 for the rest), else one, whose loads the other wavefronts' work hides (16,384 tokens of 8 heads of 256 in 8 bits,
+  // batch 8: 123 us, with two that spill 306; heads of 160, where two fit: 87 and, with one, 91).
+  constexpr int TILE_WORDS = 2 * Keys::KC + 2 * G + Keys::VC + 8, OTHER_WORDS = RT * (4 * D_TILES + 4 * G * PARTS) + 60;
+  constexpr int BUFFERS = PAGE32 && BITS == 4 && !EXACT && HEAD_DIM <= 128 ? 3 : 2 * TILE_WORDS + OTHER_WORDS <= (SPLIT ? 240 : 320) ? 2 : 1;
   constexpr int STEP = SPLIT ? TEAM : 1;  // wavefront w starts at the item's tile w and goes on in steps of TEAM tiles, or takes every tile
   // PAGE32: a tile lies in one page, whose number is read as a scalar a tile ahead
   auto look_up = [&](int kt) -> int {
