@@ -249,12 +249,10 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
   const Pair pick[2] = {__builtin_bit_cast(Pair, make_uint2(one, 0)), __builtin_bit_cast(Pair, make_uint2(0, one))};
   const C codes;
 
-  // page of a key; keys outside the item and slots without a page read page 0 and are masked
-  auto page_of = [&](int key, int& slot_in_page) -> int {
+  // the table's entry for a key; keys outside the item and slots without a page read page 0 and are masked
+  auto entry_of = [&](int key) -> int {
     const int lp = page_shift >= 0 ? (key >> page_shift) : (key / page_size);
-    slot_in_page = key - lp * page_size;
-    const int page = (key < key_end && lp < table_width) ? table[lp] : 0;
-    return (page >= 0 && page < num_pages) ? page : 0;
+    return key < key_end && lp < table_width ? table[lp] : 0;
   };
   const int krel = 8 * (n >> 2) + (n & 3);
   // As many tiles' registers as there is room for: three in the lightest case, else two where they fit beside sums and queries (by
@@ -263,12 +261,12 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
   constexpr int TILE_WORDS = 2 * Keys::KC + 2 * G + Keys::VC + 8, OTHER_WORDS = RT * (4 * D_TILES + 4 * G * PARTS) + 60;
   constexpr int BUFFERS = PAGE32 && BITS == 4 && !EXACT && HEAD_DIM <= 128 ? 3 : 2 * TILE_WORDS + OTHER_WORDS <= (SPLIT ? 240 : 320) ? 2 : 1;
   constexpr int STEP = SPLIT ? TEAM : 1;  // wavefront w starts at the item's tile w and goes on in steps of TEAM tiles, or takes every tile
-  // PAGE32: a tile lies in one page, whose number is read as a scalar a tile ahead
+  // PAGE32: a tile lies in one page, whose number is read as a scalar a tile ahead; else a lane's two are, of its keys and of its values
   auto look_up = [&](int kt) -> int {
     const int lp = min(page_shift >= 0 ? (kt >> page_shift) : (kt / page_size), table_width - 1);
     return PAGE32 ? table_s[lp] : 0;
   };
-  int page_ahead = 0;
+  int page_ahead = 0, k_ahead = 0, v_ahead = 0;
   const int tile0 = key_begin >> 5, tiles = ((key_end + 31) >> 5) - tile0;
   // the loads of the item's tile `t`, which may lie past its last one: then of nothing
   auto issue = [&](Keys& L, int t) {
@@ -292,9 +290,11 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
       for (int c = 0; c < PIECES; ++c) load_words<4>(head, vb + 256 * c + 16 * n, *(uint32_t(*)[4])&L.vc[4 * c]);
       if constexpr (Keys::VC % 4 != 0) load_words<2>(head, vb + 256 * PIECES + 8 * n, *(uint32_t(*)[2])&L.vc[4 * PIECES]);
     } else {
-      int ks, vs;
-      const uint8_t* kpage = base + (size_t)page_of(kt + krel, ks) * page_bytes;
-      const uint8_t* vpage = base + (size_t)page_of(kt + 8 * j, vs) * page_bytes;
+      const int kk = kt + krel, vk = kt + 8 * j;
+      const int ks = page_shift >= 0 ? kk & (page_size - 1) : kk % page_size, vs = page_shift >= 0 ? vk & (page_size - 1) : vk % page_size;
+      const uint8_t* kpage = base + (size_t)((unsigned)k_ahead < (unsigned)num_pages ? k_ahead : 0) * page_bytes;
+      const uint8_t* vpage = base + (size_t)((unsigned)v_ahead < (unsigned)num_pages ? v_ahead : 0) * page_bytes;
+      k_ahead = entry_of(kk + 32 * STEP), v_ahead = entry_of(vk + 32 * STEP);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         load_words<Keys::KC>(kpage + (uint32_t)(((ks + 4 * i) * 4 + j) * (Keys::KC * 4)), L.kc[i]);
@@ -446,6 +446,7 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
   if (tile < tiles) {
     Keys held[BUFFERS];
     page_ahead = look_up(32 * (tile0 + tile));
+    if constexpr (!PAGE32) k_ahead = entry_of(32 * (tile0 + tile) + krel), v_ahead = entry_of(32 * (tile0 + tile) + 8 * j);
 #pragma unroll
     for (int u = 0; u < BUFFERS - 1; ++u) issue(held[u], tile + u * STEP);
     for (bool more = true; more;) {
