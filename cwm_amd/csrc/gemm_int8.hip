@@ -6,7 +6,7 @@
 //
 // Few rows: every byte of W is read once, straight into the matrix instruction's operand, and the product is bound by that
 // reading (one row by 6,144 x 6,144: 13.2 us, 37.7 MB, of which a launch and the latencies of two reads are 5).
-// More rows: gemm_wide.h's loop.  Up to 64 rows it is bound by the reading of W (37 x 28,672 x 4,096: 23 us, 5.1 TB/s); 2,048 x
+// More rows: gemm_wide.h's loop.  Up to 64 rows it is bound by the reading of W (37 x 28,672 x 4,096: 21.8 us, 5.4 TB/s); 2,048 x
 // 43,008 x 6,144 runs at 2.2 POP/s in 490 us, bound by LDS and matrix cores in turn: by count a step's operands are read in 0.43 us and
 // multiplied in 0.43, and the step takes 0.85 (in bfloat16, with twice the products' time for as many bytes, the reads hide).
 #include <type_traits>
@@ -310,7 +310,7 @@ gemm_int8_few_kernel(const int8_t* __restrict__ X, long ldx, const float* __rest
 #define WIDE_BAND 8
 
 struct Int8Order {
-  int m_tiles, n_tiles;
+  int m_tiles, n_tiles, columns;  // of a tile: all that it has room for, or fewer
   __device__ __forceinline__ void place(int t, int& tm, int& tn) const {  // bands of WIDE_BAND row tiles, in a band column by column
     const int band = t / (WIDE_BAND * n_tiles), in_band = t - band * WIDE_BAND * n_tiles;
     const int rows = min(WIDE_BAND, m_tiles - band * WIDE_BAND);
@@ -334,7 +334,7 @@ struct Int8Source {
     constexpr int BM = WideShape<WM, WN>::BM, BN = WideShape<WM, WN>::BN;
     int tm, tn;
     order.place(tile, tm, tn);
-    const int m0 = tm * BM, n0 = tn * BN;
+    const int m0 = tm * BM, n0 = tn * order.columns, last = min(order.columns, N - n0) - 1;
     a = A + (size_t)m0 * lda;
     w = W + (size_t)n0 * ldw;
     first_step = tn % steps;
@@ -342,11 +342,11 @@ struct Int8Source {
     for (int i = 0; i < WideShape<WM, WN>::ND; ++i) {
       const int p = min(wave + 8 * i, WideShape<WM, WN>::PIECES - 1);
       const int row = 8 * p + (lane >> 3);
-      // rows past the matrix read its last one: their sums are not stored
+      // rows past the matrix, or the tile's columns, read the last one: their sums are not stored
       if (p < BM / 8)
         off[i] = (uint32_t)(((size_t)min(row, M - 1 - m0) * lda + 8 * ((lane & 7) ^ ((row >> 1) & 7))) * 2);
       else
-        off[i] = (uint32_t)(((size_t)min(row - BM, N - 1 - n0) * ldw + 8 * ((lane & 7) ^ wide_w_key<WN>(row - BM))) * 2);
+        off[i] = (uint32_t)(((size_t)min(row - BM, last) * ldw + 8 * ((lane & 7) ^ wide_w_key<WN>(row - BM))) * 2);
     }
   }
 };
@@ -366,7 +366,7 @@ struct Int8Sink {
     order.place(tile, tm, tn);
     const int r = lane & 15, j = lane >> 4, wm = wave >> 2, wn = wave & 3;
     const int m0 = tm * BM + wm * WM * 16 + r;
-    const int n0 = tn * BN + wn * WN * 16 + 4 * WN * j;
+    const int n0 = tn * order.columns + wn * WN * 16 + 4 * WN * j, end = min(N, (tn + 1) * order.columns);
     if constexpr (std::is_same<T, int>::value) {  // sums of a part of K: rows of whole tiles
 #pragma unroll
       for (int i = 0; i < WM; ++i)
@@ -389,7 +389,7 @@ struct Int8Sink {
       // Waited for here, by an instruction that the compiler knows of: loads that it takes to be under way at the loop's head
       // make it wait for all of the loop's own loads in every step (2,048 x 43,008 x 6,144 663 us, 1.24 us a step).
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-      const bool full = (tm + 1) * BM <= M && (tn + 1) * BN <= N;
+      const bool full = (tm + 1) * BM <= M && tn * order.columns + BN <= end;
 #pragma unroll
       for (int i = 0; i < WM; ++i) {
         const int m = m0 + 16 * i;
@@ -402,7 +402,7 @@ struct Int8Sink {
           for (int e = 0; e < 4; ++e) v[b][e] = (float)acc[i][b][e] * am[i] * ws[b][e] + bs[b][e];
 #pragma unroll
         for (int b = 0; b < WN; b += 2) {
-          if (n0 + 4 * b + 7 < N) {  // a row may begin anywhere: 16 bytes to any address
+          if (n0 + 4 * b + 7 < end) {  // a row may begin anywhere: 16 bytes to any address
             if constexpr (sizeof(T) == 4) {
               __builtin_memcpy(row + 4 * b, v[b], 16);
               __builtin_memcpy(row + 4 * b + 4, v[b + 1], 16);
@@ -414,7 +414,7 @@ struct Int8Sink {
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (n0 + 4 * b + e < N) Elem<T>::store(row + 4 * b + e, v[b + e / 4][e % 4]);
+              if (n0 + 4 * b + e < end) Elem<T>::store(row + 4 * b + e, v[b + e / 4][e % 4]);
           }
         }
       }
@@ -428,7 +428,7 @@ template <int WM, int WN, typename T, bool ONCE>
 __global__ void __launch_bounds__(512, 2)
 gemm_int8_wide_kernel(const int8_t* __restrict__ X, long ldx, const float* __restrict__ a, const int8_t* __restrict__ W, long ldw,
                       const float* __restrict__ w_scale, const float* __restrict__ bias, T* __restrict__ y, long ldy, int M, int N,
-                      int K, int m_tiles, int n_tiles, int parts) {
+                      int K, int m_tiles, int n_tiles, int columns, int parts) {
   typedef WideShape<WM, WN> Shape;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[Shape::S * Shape::STAGE];
   const int lane = threadIdx.x & 63;
@@ -440,13 +440,20 @@ gemm_int8_wide_kernel(const int8_t* __restrict__ X, long ldx, const float* __res
   const int per = total / groups, rest = total % groups;
   const int first = xcd * per + min(xcd, rest), count = per + (xcd < rest ? 1 : 0);
   const int mine = (count - idx + blocks - 1) / blocks;
-  const Int8Order order = {m_tiles, n_tiles};
+  const Int8Order order = {m_tiles, n_tiles, columns};
   constexpr bool PARTS = std::is_same<T, int>::value;
   const int all = (K + 127) / 128, part = PARTS ? (first + idx) / tiles : 0;
   const int begin = PARTS ? part * all / parts : 0, steps = PARTS ? (part + 1) * all / parts - begin : all;
   Int8Source<WM, WN> src = {(const bf16_t*)X, (const bf16_t*)W, ldx / 2, ldw / 2, M, N, (K - 128) / 2, begin, steps, lane, wave, order};
   Int8Sink<WM, WN, T> sink = {y + (size_t)part * M * ldy, ldy, a, w_scale, bias, M, N, lane, wave, order};
   wide_loop<WM, WN, Int8Sink<WM, WN, T>::STORES, WideInt8<ONCE, PARTS>>(lds, src, sink, first + idx - part * tiles, blocks, mine, steps);
+}
+
+// The columns of a tile where there is one tile of rows, and the reading of W is what counts: as many as give every compute unit the
+// same number of them (37 x 28,672 x 4,096: 224 tiles of 128 columns on 256 units 23.3 us, 256 of 112 21.8; 8 x 43,008 x 6,144 52 and 45.5).
+static int int8_columns(long N, int most, long tiles, int units) {
+  const long rounds = (tiles + units - 1) / units, columns = (N + rounds * units - 1) / (rounds * units);
+  return (int)(columns > most ? most : (columns + 7) / 8 * 8);
 }
 
 // The parts' sums, [parts][M][ldp], added, scaled and rounded.  A thread has four columns of a row.
@@ -574,7 +581,7 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
     const dim3 grid((unsigned)(m_tiles * n_tiles * parts));
 #define INT8_PARTS_RUN(WM, ONCE)                                                                                                              \
   hipLaunchKernelGGL((gemm_int8_wide_kernel<WM, 2, int, ONCE>), grid, dim3(512), 0, stream, (const int8_t*)X, ldx, a, (const int8_t*)W, ldw, \
-                     w_scale, bias, sums, ldp, M, N, K, (int)m_tiles, (int)n_tiles, parts)
+                     w_scale, bias, sums, ldp, M, N, K, (int)m_tiles, (int)n_tiles, 128, parts)
     if (tile == 3 && m_tiles == 1)
       INT8_PARTS_RUN(2, true);
     else if (tile == 3)
@@ -593,10 +600,12 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
   }
 #define INT8_WIDE_RUN(WM, WN, T, ONCE)                                                                                                      \
   hipLaunchKernelGGL((gemm_int8_wide_kernel<WM, WN, T, ONCE>), grid, dim3(512), 0, stream, (const int8_t*)X, ldx, a, (const int8_t*)W, ldw,  \
-                     w_scale, bias, (T*)y, ldy, M, N, K, (int)m_tiles, (int)n_tiles, 1)
+                     w_scale, bias, (T*)y, ldy, M, N, K, (int)m_tiles, (int)n_tiles, columns, 1)
 #define INT8_WIDE(WM, WN)                                                                                          \
   {                                                                                                                \
-    const long m_tiles = (M + 32 * WM - 1) / (32 * WM), n_tiles = (N + 64 * WN - 1) / (64 * WN);                   \
+    const long m_tiles = (M + 32 * WM - 1) / (32 * WM), all = (N + 64 * WN - 1) / (64 * WN);                       \
+    const int columns = m_tiles > 1 ? 64 * WN : int8_columns(N, 64 * WN, all, units);                              \
+    const long n_tiles = (N + columns - 1) / columns;                                                              \
     CWM_REQUIRE(m_tiles * n_tiles * (Kp / 128) < (1L << 31), "linear_int8: too many steps of tiles");                 \
     const dim3 grid((unsigned)(m_tiles * n_tiles < units ? m_tiles * n_tiles : units));                            \
     if (dtype == CWM_BF16 && m_tiles == 1)                                                                         \
