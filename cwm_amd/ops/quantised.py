@@ -350,7 +350,7 @@ def quant_paged_attention(
 
 # --------------------------------------------------------------------------- #
 INT8_MAX_K = 131072  # csrc/gemm_int8.hip: 127^2 K fits the 32 bits of a sum
-INT8_FEW_ROWS = 16
+INT8_FEW_ROWS, INT8_FEW_WEIGHTS = 16, 50_400_000
 INT8_FUSED_ROWS, INT8_FUSED_K = 4, 16384  # csrc/gemm_int8.hip: rows of x, and the columns of one row, that every block makes the integers of
 
 
@@ -450,14 +450,16 @@ _INT8_PARTS_US, _INT8_PARTS_BYTES = 5.0, 4e6  # of joining the parts of K: a lau
 
 @functools.lru_cache(maxsize=1024)
 def _int8_tile(m: int, n: int, k: int, units: int) -> Tuple[int, int]:
-    """The kernel for a product's sizes, and the parts it takes K in.  Up to four rows one launch does all (1 x 6,144 x 6,144 14.5 us, in
-    two launches 16.2); up to 16 W is read straight into the matrix instruction (8 x 6,144 x 6,144 18.4 us, tiles of 64 rows 27.1, with
-    K in parts 20.3; 16 x 28,672 x 4,096 42.1 and 27.1: there the tiles' loads, further ahead, are the faster ones); more rows take the
-    tile of least cost.  Where its tiles are fewer than the compute units, K is taken in parts (33 x 6,144 x 6,144 29.3 us, in five
-    parts 21.2; 64 x 4,096 x 14,336 64.0 and, in eight, 31.7; 64 x 8,192 x 1,024 15.3 and, in two, 20.3, which stays whole)."""
-    if m <= INT8_FUSED_ROWS and k <= INT8_FUSED_K // (m if m <= 2 else 4):
+    """The kernel for a product's sizes, and the parts it takes K in.  Up to four rows one launch does all, while W is not so large that
+    the tiles' loads, further ahead, are the faster ones (us in one launch, in two and by tiles: 1 x 6,144 x 6,144 12.5, 16.2, 19.6; 1 x
+    10,240 x 8,192 21.0, 26.2, 23.4; 1 x 28,672 x 4,096 26.2, 31.7, 24.3; 1 x 43,008 x 6,144 58, 65, 48); up to 16 rows W is read straight
+    into the matrix instruction, with half that limit (8 x 6,144 x 8,192 19.3, by tiles 20.1; 16 x 14,336 x 4,096 23.7 and 20.5; 8 x 28,672 x
+    2,048 22.4 and 16.4).  More rows take the tile of least cost, and where its tiles are fewer than the compute units, K in parts (33 x
+    6,144 x 6,144 29.3, in five parts 21.2; 64 x 4,096 x 14,336 64.0 and, in eight, 31.7; 64 x 8,192 x 1,024 15.3 and, in two, 20.3,
+    which stays whole)."""
+    if m <= INT8_FUSED_ROWS and k <= INT8_FUSED_K // (m if m <= 2 else 4) and n * k < 2 * INT8_FEW_WEIGHTS:
         return -1, 1
-    if k < 128 or (m <= INT8_FEW_ROWS and n * k < 1 << 26):
+    if k < 128 or (m <= INT8_FEW_ROWS and n * k < INT8_FEW_WEIGHTS):
         return 0, 1
     steps, best = -(-k // 128), None
     for tile, rows, columns, start, step in _INT8_TILES:
