@@ -210,3 +210,20 @@ def test_on_a_stream_of_its_own_and_captured():
         replayed = [t.clone() for t in out]
         torch.cuda.synchronize()
         assert all(torch.equal(a, ops.linear_int8(t, w, s)) for a, t in zip(replayed, source))
+
+
+def test_k_in_parts_captured():
+    w, s = (t.to(DEV) for t in _weight(300, 8192, 6))
+    x = _rows(40, 8192, torch.bfloat16, 7).to(DEV)
+    held, sources = x.clone(), (x, x.flip(0) * 3)
+    want = [ops.linear_int8(t, w, s) for t in sources]
+    assert torch.equal(want[0], ops.linear_int8(x, w, s, tile=1))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.linear_int8(held, w, s)
+    for i in (1, 0, 1):
+        held.copy_(sources[i])
+        graph.replay()
+        replayed = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, want[i]) and torch.equal(ops.linear_int8(sources[i], w, s), want[i])

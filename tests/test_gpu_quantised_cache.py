@@ -359,3 +359,33 @@ def test_on_a_stream_of_its_own_and_captured():
         replayed = [t.clone() for t in out]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(replayed, layer()))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_sequences_without_new_tokens(bits):
+    """Beside portions and decoded tokens: they have pages, and nothing to do."""
+    new, kv, dim = [0, 80, 1, 0], [64, 80, 2300, 0], 64
+    step, cache, q, keys, values = _case(new, kv, 32, 8, 2, dim, bits, torch.bfloat16, None, 18)
+    _close(_attend(step, cache, q, bits, None, 0.125), step, q, keys, values, bits, None, 0.125)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_portions_of_many_rows_captured(bits):
+    """A step whose lists are on the device already is captured, replayed with other queries and pages, with eager steps in between."""
+    new, kv, dim = [70, 1, 200], [500, 2100, 200], 128
+    step, cache, q, keys, values = _case(new, kv, 32, 12, 2, dim, bits, torch.bfloat16, None, 19)
+    other = _case(new, kv, 32, 12, 2, dim, bits, torch.bfloat16, None, 20)
+    cache, table, batch, qd = cache.to(DEV), step.table.to(DEV), step.batch(DEV), q.to(DEV)
+    sets = [(cache.clone(), table.clone(), qd.clone()), (other[1].to(DEV), other[0].table.to(DEV), other[2].to(DEV))]
+    run = lambda c, t, x: ops.quant_paged_attention(x, c, t, batch, None, dim ** -0.5, bits)  # noqa: E731
+    want = [run(*s) for s in sets]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(cache, table, qd)
+    for i in (1, 0, 1, 1, 0):
+        for to, source in zip((cache, table, qd), sets[i]):
+            to.copy_(source)
+        graph.replay()
+        replayed = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, want[i]) and torch.equal(run(*sets[i]), want[i])
