@@ -45,46 +45,36 @@ CWM_DEFINE_ERROR_API
 
 typedef const __attribute__((address_space(4))) int* scalar_ints;  // a uniform index is read by a scalar load
 
+// N words at an address that is a multiple of 4 bytes, in the widest pieces.
 template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
-  if constexpr (N % 4 == 0) {
+  const void* from = __builtin_assume_aligned(p, 4);
+  constexpr int FOURS = N / 4 * 4;
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const uint4 u = *(const uint4*)(p + 4 * i);
-      w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
-    }
-  } else if constexpr (N % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint2 u = *(const uint2*)(p + 4 * i);
-      w[i] = u.x, w[i + 1] = u.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = *(const uint32_t*)(p + 4 * i);
-  }
+  for (int i = 0; i < FOURS; i += 4) __builtin_memcpy(&w[i], (const uint8_t*)from + 4 * i, 16);
+  if constexpr (N > FOURS) __builtin_memcpy(&w[FOURS], (const uint8_t*)from + 4 * FOURS, 4 * (N - FOURS));
 }
 
 // The same through a buffer resource, which bounds the offsets: past its size a load gives zeros and reads nothing, so one of size
 // 0 takes the place of a branch around the loads.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <int N> __device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t r, uint32_t offset, uint32_t (&w)[N]) {
   constexpr int ONCE = 2;  // non-temporal: every block reads keys and values of its own
-  if constexpr (N % 4 == 0) {
+  constexpr int FOURS = N / 4 * 4;
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const u32x4 u = __builtin_amdgcn_raw_buffer_load_b128(r, offset + 4 * i, 0, ONCE);
-      w[i] = u[0], w[i + 1] = u[1], w[i + 2] = u[2], w[i + 3] = u[3];
-    }
-  } else if constexpr (N % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const u32x2 u = __builtin_amdgcn_raw_buffer_load_b64(r, offset + 4 * i, 0, ONCE);
-      w[i] = u[0], w[i + 1] = u[1];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, offset + 4 * i, 0, ONCE);
+  for (int i = 0; i < FOURS; i += 4) {
+    const u32x4 u = __builtin_amdgcn_raw_buffer_load_b128(r, offset + 4 * i, 0, ONCE);
+    w[i] = u[0], w[i + 1] = u[1], w[i + 2] = u[2], w[i + 3] = u[3];
+  }
+  if constexpr (N - FOURS == 3) {
+    const u32x3 u = __builtin_amdgcn_raw_buffer_load_b96(r, offset + 4 * FOURS, 0, ONCE);
+    w[FOURS] = u[0], w[FOURS + 1] = u[1], w[FOURS + 2] = u[2];
+  } else if constexpr (N - FOURS == 2) {
+    const u32x2 u = __builtin_amdgcn_raw_buffer_load_b64(r, offset + 4 * FOURS, 0, ONCE);
+    w[FOURS] = u[0], w[FOURS + 1] = u[1];
+  } else if constexpr (N - FOURS == 1) {
+    w[FOURS] = __builtin_amdgcn_raw_buffer_load_b32(r, offset + 4 * FOURS, 0, ONCE);
   }
 }
 
@@ -117,7 +107,7 @@ template <int BITS> struct KeyTile {
   static constexpr int KC = G * BITS / 4;
   // words of the values' codes: pieces of 16 bytes (four dimensions of 4 bits, two of 8), a last one of 8 where 32 dimensions are left
   static constexpr int VC = BITS == 4 ? 2 * G : 4 * G;
-  uint32_t kc[2][KC], kw[2][G], vc[VC], vw[8];
+  uint32_t kc[2][KC], kw[2][4 * QUADS], vc[VC], vw[8];  // zeros behind the words of a key
 };
 
 __device__ __forceinline__ float not_a_number() { return __uint_as_float(0x7fc00000u); }
@@ -282,7 +272,10 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         load_words<Keys::KC>(head, (uint32_t)(((ks + 4 * i) * 4 + j) * (Keys::KC * 4)), L.kc[i]);
-        load_words<G>(head, key_words_at + (uint32_t)(ks + 4 * i) * (G * 4), L.kw[i]);
+        uint32_t words[G];
+        load_words<G>(head, key_words_at + (uint32_t)(ks + 4 * i) * (G * 4), words);
+#pragma unroll
+        for (int g = 0; g < 4 * QUADS; ++g) L.kw[i][g] = g < G ? words[g % G] : 0u;
       }
       load_words<8>(head, value_words_at + (uint32_t)vs * 4, L.vw);
       const uint32_t vb = values_at + (uint32_t)(vs >> 3) * (HEAD_DIM * BITS);
@@ -298,7 +291,10 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         load_words<Keys::KC>(kpage + (uint32_t)(((ks + 4 * i) * 4 + j) * (Keys::KC * 4)), L.kc[i]);
-        load_words<G>(kpage + (key_words_at + (uint32_t)(ks + 4 * i) * (G * 4)), L.kw[i]);
+        uint32_t words[G];
+        load_words<G>(kpage + (key_words_at + (uint32_t)(ks + 4 * i) * (G * 4)), words);
+#pragma unroll
+        for (int g = 0; g < 4 * QUADS; ++g) L.kw[i][g] = g < G ? words[g % G] : 0u;
       }
       load_words<8>(vpage + (value_words_at + (uint32_t)vs * 4), L.vw);
       const uint32_t vb = values_at + (uint32_t)(vs >> 3) * (HEAD_DIM * BITS);
@@ -326,8 +322,7 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
       Frag8 words[QUADS];
 #pragma unroll
       for (int u = 0; u < QUADS; ++u)
-        words[u].u = make_uint4(L.kw[t][4 * u], 4 * u + 1 < G ? L.kw[t][(4 * u + 1) % G] : 0u, 4 * u + 2 < G ? L.kw[t][(4 * u + 2) % G] : 0u,
-                                4 * u + 3 < G ? L.kw[t][(4 * u + 3) % G] : 0u);
+        words[u].u = make_uint4(L.kw[t][4 * u], L.kw[t][4 * u + 1], L.kw[t][4 * u + 2], L.kw[t][4 * u + 3]);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         st[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(words[0].v, qs[rt][0].v, zero, 0, 0, 0);
@@ -343,7 +338,7 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
           const uint32_t c0 = L.kc[t][(2 * g) % Keys::KC], c1 = L.kc[t][(2 * g + 1) % Keys::KC];
           kf.u = make_uint4(codes.bytes(c0, 0), codes.bytes(c0, 2), codes.bytes(c1, 0), codes.bytes(c1, 2));
         }
-        const uint2 pair = make_uint2(L.kw[t][g / 2 * 2], g / 2 * 2 + 1 < G ? L.kw[t][(g / 2 * 2 + 1) % G] : 0u);
+        const uint2 pair = make_uint2(L.kw[t][g / 2 * 2], L.kw[t][g / 2 * 2 + 1]);
         const float4v step = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(Pair, pair), pick[g % 2], zero, 0, 0, 0);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
