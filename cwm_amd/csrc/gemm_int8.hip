@@ -502,6 +502,8 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
   CWM_REQUIRE(ldw % 16 == 0 && (uintptr_t)W % 16 == 0, "linear_int8: the weight's rows must be 16-byte aligned");
   CWM_REQUIRE(ldw >= K && ldy >= N, "linear_int8: row strides shorter than rows");
   const int x_size = x_dtype == CWM_BF16 ? 2 : 4, Kp = (K + 127) / 128 * 128;
+  CWM_REQUIRE(parts >= 1 && parts <= Kp / 128 && (parts == 1 || ((tile == 3 || tile == 4) && sums && (uintptr_t)sums % 16 == 0)),
+              "linear_int8: K in %d parts with tile %d", parts, tile);
   const int a_wave = (K / 128 + FEW_WAVES - 1) / FEW_WAVES;  // pieces of a wavefront of few rows
   // Two blocks a compute unit stay, each with the same number of rows of W: what one unit can have in flight is limited, so with
   // tiles dealt out one by one the units that get one more take that much longer (one row by 6,144 of 6,144: 384 tiles 14.6 us,
@@ -573,8 +575,6 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
   CWM_REQUIRE(K >= 128, "linear_int8: the tiles of many rows take a K of 128 and more, not %d", K);
   CWM_REQUIRE(ldx < (1L << 23) && ldw < (1L << 23), "linear_int8: row strides too long for 32-bit offsets");
   CWM_REQUIRE(tile >= 1 && tile <= 4, "linear_int8: no tile %d", tile);
-  CWM_REQUIRE(parts >= 1 && parts <= Kp / 128 && (parts == 1 || ((tile == 3 || tile == 4) && sums && (uintptr_t)sums % 16 == 0)),
-              "linear_int8: K in %d parts with tile %d", parts, tile);
   if (parts > 1) {
     const long m_tiles = tile == 3 ? (M + 63) / 64 : (M + 127) / 128, n_tiles = (N + 127) / 128, ldp = n_tiles * 128;
     CWM_REQUIRE(m_tiles * n_tiles * parts <= 65536 && M <= 65535, "linear_int8: too many tiles to take K in parts");

@@ -280,7 +280,9 @@ def quant_paged_attention(
 ) -> torch.Tensor:
     """Attention of the step's tokens over a quantised cache (`quant_kv_write`), prompt portions and decoded tokens in one
     call: `q` [T, Hq, hd] (float32 or bfloat16, rotated), `batch` the step's `StepBatch`, `window` the keys a query reads, its
-    own included (None: all).  Returns [T, Hq * hd] in q's type.  A query one of whose keys has no page gets NaN."""
+    own included (None: all).  Returns [T, Hq * hd] in q's type.  A query one of whose keys has no page gets NaN.
+    bfloat16 portions of more than 128 rows (tokens times query heads of a key/value head) unpack what they read of the cache to 16 bits for
+    the time of the call: 4 Hkv hd bytes a key."""
     KernelError, _check, _code = _base()
     _attention_plan, _check_mask, _half_blocks_built, _three_blocks_a_unit = _planning()
     _check_device(q, cache, block_table, batch.cu_q, batch.kv_len)

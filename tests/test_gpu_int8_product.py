@@ -118,8 +118,9 @@ def test_products_with_k_in_parts(tile):
                 assert torch.equal(ops.linear_int8(*given, out), ops.linear_int8(*given, out, tile))
     with pytest.raises(ops.KernelError, match="parts"):
         ops.linear_int8(*given, tile=tile, parts=6)
-    with pytest.raises(ops.KernelError, match="parts"):
-        ops.linear_int8(*given, tile=2, parts=2)
+    for other in (-1, 0, 1, 2):
+        with pytest.raises(ops.KernelError, match="parts"):
+            ops.linear_int8(given[0][:1], *given[1:], tile=other, parts=2)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
