@@ -66,34 +66,29 @@ def _units(device: torch.device) -> int:
     return _compute_units(device)
 
 
-def _stream() -> int:
-    """The current HIP stream of the current device, as a plain handle."""
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+# looked up once: the attributes of `torch` and `torch._C` cost a launch-bound call half a microsecond
+_INT32, _FLOAT32, _UINT8 = torch.int32, torch.float32, torch.uint8
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _check_device(*tensors: Optional[torch.Tensor]) -> None:
-    """All on one HIP device, and that the current one: kernels are launched on its stream."""
-    current = None
-    for t in tensors:
-        if t is None:
-            continue
-        if current is None:
-            if not t.is_cuda:
+def _check_device(first: torch.Tensor, *tensors: Optional[torch.Tensor]) -> int:
+    """That all are on one HIP device, and that the current one: kernels are launched on its stream.  Returns that stream's handle."""
+    current = _current_device() if first.is_cuda else None
+    if current is not None and first.get_device() == current:
+        for t in tensors:
+            if t is not None and t.get_device() != current:
                 break
-            current = torch._C._cuda_getDevice()
-        if t.get_device() != current:
-            break
-    else:
-        return
+        else:
+            return _current_stream(current)
     KernelError = _base()[0]
-    for t in tensors:
+    for t in (first, *tensors):
         if t is not None and not t.is_cuda:
             raise KernelError(f"cwm_amd kernels run on a HIP device only; got a tensor on {t.device}. There is no CPU path.")
-    raise KernelError(f"tensors are on {', '.join(sorted({str(t.device) for t in tensors if t is not None}))}, the current device is cuda:{current}")
+    raise KernelError(f"tensors are on {', '.join(sorted({str(t.device) for t in (first, *tensors) if t is not None}))}, the current device is cuda:{current}")
 
 
 def _check_vector(t: torch.Tensor, n: int, what: str) -> None:
-    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not _INT32 or t.numel() != n or not t.is_contiguous():
         raise _base()[0](f"{what} must be a contiguous int32 [T] tensor for {n} tokens, found {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
 
 
@@ -129,16 +124,16 @@ def _page_size(shape: Tuple[int, ...], n_kv: Optional[int], head_dim: int, bits:
         return 0, why
     token = _token_bytes(head_dim, bits)
     if len(shape) != 3 or min(shape) < 1 or (n_kv is not None and shape[1] != n_kv) or shape[2] % token != 0:
-        return 0, f"cache {shape} does not fit {n_kv or 'any'} heads of size {head_dim} in {bits} bits"
+        return 0, f"cache {tuple(shape)} does not fit {n_kv or 'any'} heads of size {head_dim} in {bits} bits"
     return shape[2] // token, quant_cache_limits(head_dim, shape[2] // token, bits)
 
 
 def _check_cache(cache: torch.Tensor, block_table: torch.Tensor, n_kv: Optional[int], head_dim: int, bits: int) -> int:
     """The tokens of a page of `cache`, a contiguous uint8 [pages, key/value heads, head bytes]."""
-    page_size, why = _page_size(tuple(cache.shape), n_kv, head_dim, bits)
-    if why is None and (cache.dtype != torch.uint8 or not cache.is_contiguous()):
+    page_size, why = _page_size(cache.shape, n_kv, head_dim, bits)
+    if why is None and (cache.dtype is not _UINT8 or not cache.is_contiguous()):
         why = f"the cache does not fit: it is contiguous and of bytes (uint8), found {cache.dtype} with strides {cache.stride()}"
-    if why is None and (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[1] < 1 or not block_table.is_contiguous()):
+    if why is None and (block_table.dtype is not _INT32 or block_table.dim() != 2 or block_table.shape[1] < 1 or not block_table.is_contiguous()):
         why = f"block_table must be a contiguous int32 [B, W] tensor, found {block_table.dtype} {tuple(block_table.shape)}"
     if why is not None:
         raise _base()[0](why)
@@ -171,7 +166,7 @@ def quant_kv_write(
     same angles.  No two tokens of a call may have the same place.  A group of values with an infinity or a NaN is
     held as NaN."""
     KernelError, _check, _code = _base()
-    _check_device(k, v, q, positions, inv_freq, cache, block_table, seq_of_token)
+    stream = _check_device(k, v, q, positions, inv_freq, cache, block_table, seq_of_token)
     if k.dim() != 3:
         raise KernelError("k must be [T, Hkv, hd] with contiguous heads")
     dtype = k.dtype
@@ -192,14 +187,14 @@ def quant_kv_write(
     page_size = _check_cache(cache, block_table, n_kv, hd, bits)
     _check_vector(positions, n_tokens, "positions")
     _check_vector(seq_of_token, n_tokens, "seq_of_token")
-    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != hd // 2 or not inv_freq.is_contiguous()):
+    if inv_freq is not None and (inv_freq.dtype is not _FLOAT32 or inv_freq.numel() != hd // 2 or not inv_freq.is_contiguous()):
         raise KernelError(f"the rotary table must be float32 [{hd // 2}]")
     function, lib = _entry("quant_cache", "cwm_quant_kv_write")
     n_seqs, width = block_table.shape
     status = function(
         k.data_ptr(), k_token, v.data_ptr(), v.stride(0), None if q is None else q.data_ptr(), q_token, code, positions.data_ptr(),
         seq_of_token.data_ptr(), None if inv_freq is None else inv_freq.data_ptr(), cache.data_ptr(), block_table.data_ptr(), n_seqs, width, page_size,
-        cache.shape[0], n_tokens, n_kv, n_q, hd, bits, _stream(),
+        cache.shape[0], n_tokens, n_kv, n_q, hd, bits, stream,
     )
     if status:
         _check(lib, status)
@@ -217,7 +212,7 @@ def quant_kv_read(
     """The keys and values, each [T, Hkv, head_dim] of `dtype` (float32 or bfloat16), that a quantised `cache` holds of the
     tokens at `positions` [T] of the sequences `seq_of_token` [T] (rows of the block table); zeros where no page is held."""
     _, _check, _code = _base()
-    _check_device(cache, block_table, positions, seq_of_token)
+    stream = _check_device(cache, block_table, positions, seq_of_token)
     page_size = _check_cache(cache, block_table, None, head_dim, bits)
     n_tokens = positions.numel()
     _check_vector(positions, n_tokens, "positions")
@@ -230,7 +225,7 @@ def quant_kv_read(
     n_seqs, width = block_table.shape
     status = function(
         k.data_ptr(), v.data_ptr(), code, positions.data_ptr(), seq_of_token.data_ptr(), cache.data_ptr(), block_table.data_ptr(), n_seqs, width,
-        page_size, pages, n_tokens, n_kv, head_dim, bits, _stream(),
+        page_size, pages, n_tokens, n_kv, head_dim, bits, stream,
     )
     if status:
         _check(lib, status)
@@ -285,7 +280,7 @@ def quant_paged_attention(
     the time of the call: 4 Hkv hd bytes a key."""
     KernelError, _check, _code = _base()
     _attention_plan, _check_mask, _half_blocks_built, _three_blocks_a_unit = _planning()
-    _check_device(q, cache, block_table, batch.cu_q, batch.kv_len)
+    stream = _check_device(q, cache, block_table, batch.cu_q, batch.kv_len)
     _check_mask(window, None, None)
     if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
         raise KernelError("q must be [T, Hq, hd] with contiguous heads")
@@ -315,9 +310,7 @@ def quant_paged_attention(
         partials = torch.empty(plan.n_partials * n_kv * 16 * (hd + 4), dtype=torch.float32, device=q.device)  # held until the last launch
         partial = partials.data_ptr()
     table, width = block_table.data_ptr(), block_table.shape[1]
-    first, lengths, work, wide, merge, stream = (
-        batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), plan.work.data_ptr(), plan.wide.data_ptr(), plan.merge.data_ptr(), _stream()
-    )
+    first, lengths, work, wide, merge = batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), plan.work.data_ptr(), plan.wide.data_ptr(), plan.merge.data_ptr()
     if plan.n_work or not unpacks:
         function, lib = _entry("attention_quant", "cwm_attention_quant", hd)
         status = function(
@@ -362,7 +355,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     for its scale.  The integers are a view of rows padded with zeros to a multiple of 128, which `linear_int8` likes best for
     its weights."""
     KernelError, _check, _code = _base()
-    _check_device(x)
+    stream = _check_device(x)
     if x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise KernelError("rows to quantise must be [M, K] with contiguous rows")
     code = _code(x.dtype)
@@ -371,7 +364,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     codes = torch.empty((m, padded), dtype=torch.int8, device=x.device)
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
     function, lib = _entry("gemm_int8", "cwm_quantize_rows")
-    status = function(x.data_ptr(), x.stride(0), code, codes.data_ptr(), padded, scale.data_ptr(), m, k, padded, _stream())
+    status = function(x.data_ptr(), x.stride(0), code, codes.data_ptr(), padded, scale.data_ptr(), m, k, padded, stream)
     if status:
         _check(lib, status)
     return codes[:, :k], scale
@@ -399,7 +392,7 @@ def linear_int8(
     aligned.  Returns [M, N] in `out_dtype` (default: x's).  `tile` (tests) names one of the kernels and
     `parts` in how many pieces it takes K."""
     KernelError, _check, _code = _base()
-    _check_device(x, weight, weight_scale, bias)
+    stream = _check_device(x, weight, weight_scale, bias)
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise KernelError(f"linear_int8: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
     m, k = x.shape
@@ -434,7 +427,7 @@ def linear_int8(
     function, lib = _entry("gemm_int8", "cwm_linear_int8")
     status = function(
         x.data_ptr(), x.stride(0), x_code, codes, scale, weight.data_ptr(), weight.stride(0) if n > 1 else max(k, weight.stride(0)),
-        weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), code, n, m, n, k, _units(x.device), tile, parts, joined, _stream(),
+        weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), code, n, m, n, k, _units(x.device), tile, parts, joined, stream,
     )
     if status:
         _check(lib, status)
