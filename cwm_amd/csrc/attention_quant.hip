@@ -531,9 +531,11 @@ attention_quant_kernel(const T* __restrict__ q, long q_stride, T* __restrict__ o
     float l_all = 0.f, mine = 0.f;
 #pragma unroll
     for (int w2 = 0; w2 < TEAM; ++w2) {
-      const float mw = team_m[w2][n];  // -inf: that wavefront had no tile, or none with a key of this row
+      // -inf: that wavefront had no tile, or none with a key of this row, and sums of zeros; or all scores were NaN, and so are the
+      // sums, which a factor of 0 leaves as they are
+      const float mw = team_m[w2][n];
       const float f = mw == neg_inf ? 0.f : __builtin_amdgcn_exp2f((mw - m_all) * scale_log2e);
-      l_all += mw == neg_inf ? 0.f : team_l[w2][n] * f;
+      l_all += team_l[w2][n] * f;
       if (w2 == wave) mine = f;
     }
     each_piece(0, [&](int d, int count, float4v v) {
@@ -601,12 +603,12 @@ attention_quant_merge_kernel(T* __restrict__ out, long out_stride, const float* 
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      // past the last partial, or of a chunk with no key of this row: nothing
-      const bool none = p0 + u * MERGE_WAVES >= count || m[u] == neg_inf;
-      const float f = none ? 0.f : __builtin_amdgcn_exp2f(m[u] - top);
-      l += none ? 0.f : f * lp[u];
+      if (p0 + u * MERGE_WAVES >= count) break;  // past the last partial
+      // -inf: a chunk with no key of this row, whose sums are zeros, or one whose scores were all NaN, which stays
+      const float f = m[u] == neg_inf ? 0.f : __builtin_amdgcn_exp2f(m[u] - top);
+      l += f * lp[u];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) o[i] += none ? 0.f : f * op[u][i];
+      for (int i = 0; i < PER; ++i) o[i] += f * op[u][i];
     }
   }
   if (lane == 0) l_of[wave] = l;

@@ -389,3 +389,41 @@ def test_portions_of_many_rows_captured(bits):
         replayed = out.clone()
         torch.cuda.synchronize()
         assert torch.equal(replayed, want[i]) and torch.equal(run(*sets[i]), want[i])
+
+
+@pytest.mark.parametrize("portion", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_cut_rows_keep_what_is_not_finite(bits, dtype, portion):
+    """Rows cut in chunks of 1,024 keys: a chunk whose keys are all not finite (the newest key, alone in the last one; a whole
+    chunk in the middle) has no largest score, and is not a chunk without keys.  Its reader gets NaN, its neighbour nothing of it."""
+    dim, group, heads = 64, 4, 2
+    new, kv = [1, 1, 1] + [60] * portion, [4097, 4097, 3000] + [5003] * portion
+    step, cache, q, keys, values = _case(new, kv, 64, group * heads, heads, dim, bits, dtype, None, 41)
+    keys[0][4096, 0, 3] = math.inf
+    keys[1][1024:2048, 1] = math.nan
+    if portion:
+        keys[3][2048:3072, 0, 40] = -math.inf
+    held.put_all(cache, step.table, kv, keys, values, bits)
+    got = _attend(step, cache, q, bits, None, 0.125).cpu().reshape(-1, heads, group * dim)
+    want = torch.zeros(got.shape[:2], dtype=torch.bool)
+    want[0, 0] = want[1, 1] = True
+    want[3:, 0] = True
+    assert torch.equal(torch.isnan(got).all(-1), want) and torch.isfinite(got[~want]).all()
+
+
+@pytest.mark.parametrize("portion", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_missing_chunk_is_seen_whatever_is_read_in_its_place(dtype, portion):
+    """All pages of a chunk missing, and the page that is read instead full of bytes of 255, whose words are NaN."""
+    dim, group, heads, bits, page = 64, 4, 1, 4, 64
+    new, kv = [1, 1] + [60] * portion, [4097, 3000] + [5003] * portion
+    step, _, q, keys, values = _case(new, kv, page, group * heads, heads, dim, bits, dtype, None, 42)
+    step.table[step.table == 0] = min(set(range(1, step.pool)) - set(step.table.reshape(-1).tolist()))
+    cache = torch.full((step.pool, *ops.quant_page_shape(heads, dim, page, bits)), 255, dtype=torch.uint8)
+    held.put_all(cache, step.table, kv, keys, values, bits)
+    step.table[0, 64] = -1  # the last chunk: one key
+    if portion:
+        step.table[2, 16:32] = 10 ** 6
+    got = _attend(step, cache, q, bits, None, 0.125).cpu()
+    assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all() and torch.isnan(got[2:]).all()
