@@ -451,9 +451,10 @@ quant_kv_read_kernel(T* __restrict__ k, T* __restrict__ v, const int* __restrict
 // tokens with 6 query heads to a key/value head is 96 blocks a head: the two launches take 8 and 78 us, one whose blocks
 // unpacked for themselves took 197).  `exponents` [pages][heads][PAGE / 32][2] has those of the
 // keys and of the values of every 32 tokens (half_parts.h), by the bounds that their words set.  List item: {sequence, first key (a
-// multiple of UNPACK_KEYS), page of the unpacked cache}; grid (items, heads, keys and values).  What a query must not read without a
-// NaN (a key without a page, a value held as NaN) becomes a key of NaN with a value of zeros: a masked score takes no part, where
-// zero times NaN would.
+// multiple of UNPACK_KEYS), page of the unpacked cache, first key that the sequence's queries read}; grid (items, heads, keys and
+// values).  What a query must not read without a NaN (a key without a page, a value held as NaN) becomes a key of NaN with a value
+// of zeros: a masked score takes no part, where zero times NaN would.  So does a key that a window has passed: what lies there may be
+// another sequence's by now, and must not set the exponent of its 32.
 #define UNPACK_KEYS 64
 // the largest magnitude that a word lets its group have; a NaN counts for nothing (fmaxf)
 template <int BITS> __device__ __forceinline__ float word_bound(uint32_t word) {
@@ -470,8 +471,8 @@ quant_unpack_kernel(uint16_t* __restrict__ out, int* __restrict__ exponents, int
   constexpr int H = 1 << (BITS - 1);
   constexpr int WORDS = BITS / 4;
   __shared__ float tops[UNPACK_KEYS / 16];
-  const int* item = list + (size_t)blockIdx.x * 3;
-  const int b = item[0], key0 = item[1], head = blockIdx.y;
+  const int* item = list + (size_t)blockIdx.x * 4;
+  const int b = item[0], key0 = item[1], first = item[3], head = blockIdx.y;
   const int end = kv_len[b];
   const QuantHead at = quant_head(page_size, D, BITS);
   const size_t plane = (size_t)n_kv_heads * out_page * D;
@@ -491,7 +492,7 @@ quant_unpack_kernel(uint16_t* __restrict__ out, int* __restrict__ exponents, int
   if (blockIdx.z == 0) {
     const int key = key0 + (threadIdx.x >> 2), j = threadIdx.x & 3;
     int slot;
-    const uint8_t* from = key < end ? page_of(key, slot) : nullptr;
+    const uint8_t* from = key >= first && key < end ? page_of(key, slot) : nullptr;
     uint32_t codes[G * WORDS] = {}, words[G];
     const bool held = from != nullptr;
     bool bad = !held;
@@ -528,7 +529,7 @@ quant_unpack_kernel(uint16_t* __restrict__ out, int* __restrict__ exponents, int
   if (threadIdx.x < UNPACK_KEYS) {
     const int key = key0 + threadIdx.x;
     int slot;
-    const uint8_t* from = key < end ? page_of(key, slot) : nullptr;
+    const uint8_t* from = key >= first && key < end ? page_of(key, slot) : nullptr;
     float most = from ? word_bound<BITS>(*(const uint32_t*)(from + at.value_words + (size_t)slot * 4)) : 0.f;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
@@ -556,12 +557,12 @@ quant_unpack_kernel(uint16_t* __restrict__ out, int* __restrict__ exponents, int
       const int place = BITS == 4 ? (e & 4) | ((e & 1) << 1) | ((e >> 1) & 1) : e;
       const int c = ((place < 4 ? codes.x : codes.y) >> (8 * (place & 3))) & 255;
       const float s = word_step(words[e]), z = word_offset(words[e]);
-      const bool nan = s != s;
+      const bool none = s != s || key + e < first;
       if constexpr (BITS == 4) {
-        x[0][e] = nan ? 0.f : fmaf(s, (float)((c & 15) - H), z) * down;
-        x[1][e] = nan ? 0.f : fmaf(s, (float)((c >> 4) - H), z) * down;
+        x[0][e] = none ? 0.f : fmaf(s, (float)((c & 15) - H), z) * down;
+        x[1][e] = none ? 0.f : fmaf(s, (float)((c >> 4) - H), z) * down;
       } else {
-        x[0][e] = nan ? 0.f : fmaf(s, (float)(c - H), z) * down;
+        x[0][e] = none ? 0.f : fmaf(s, (float)(c - H), z) * down;
       }
     }
     uint16_t* row = to + plane + ((size_t)((slot0 >> 3) + block) * D + (BITS == 4 ? 2 * u : u)) * 8;

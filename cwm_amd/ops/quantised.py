@@ -255,7 +255,7 @@ def _unpack_list(batch, group: int, window: Optional[int], device: torch.device)
             count = -(-n // UNPACK_PAGE) - lo
             table[b, lo : lo + count] = np.arange(pages, pages + count)
             keys = np.arange(first // UNPACK_KEYS * UNPACK_KEYS, n, UNPACK_KEYS)
-            items.append(np.stack([np.full_like(keys, b), keys, pages + keys // UNPACK_PAGE - lo], axis=1))
+            items.append(np.stack([np.full_like(keys, b), keys, pages + keys // UNPACK_PAGE - lo, np.full_like(keys, first)], axis=1))
             pages += count
         rows = np.concatenate(items).astype(np.int32)
         host = torch.from_numpy(np.concatenate([rows.reshape(-1), table.reshape(-1)]))
@@ -333,7 +333,7 @@ def quant_paged_attention(
             _check(lib, status)
         function, lib = _entry("attention_mfma", "cwm_attention_mfma", hd, "HALF_INPUTS")
         status = function(
-            q.data_ptr(), token, out.data_ptr(), n_q * hd, unpacked.data_ptr(), listed.data_ptr() + 12 * n_items, wide_width, first, lengths,
+            q.data_ptr(), token, out.data_ptr(), n_q * hd, unpacked.data_ptr(), listed.data_ptr() + 16 * n_items, wide_width, first, lengths,
             work, 0, 0, wide, plan.n_wide, plan.item_tiles, _three_blocks_a_unit(plan.n_wide * n_kv, plan.wide_shape, q.device),
             merge, plan.n_merge, plan.n_merge_mid, plan.n_merge_wide, partial, n_q, n_kv, hd, UNPACK_PAGE, n_pages,
             -1 if window is None else window - 1, 0, scale, 0.0, None, None, None, None, 0, exponents, stream,

@@ -427,3 +427,15 @@ def test_a_missing_chunk_is_seen_whatever_is_read_in_its_place(dtype, portion):
         step.table[2, 16:32] = 10 ** 6
     got = _attend(step, cache, q, bits, None, 0.125).cpu()
     assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all() and torch.isnan(got[2:]).all()
+
+
+@pytest.mark.parametrize("page", [8, 16, 32])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_keys_that_a_window_has_passed_may_hold_anything(bits, page):
+    """Portions: the pages before the window's first key belong to somebody else now, and hold numbers of 2^125."""
+    new, kv, dim, group, window = [100, 3], [400, 300], 64, 4, 50
+    step, cache, q, keys, values = _case(new, kv, page, group, 1, dim, bits, torch.bfloat16, window, 44)
+    spare = next(p for p in range(step.pool) if p not in step.table)
+    cache[spare] = 0x7E  # steps and offsets of 8.4e37
+    step.table[0, : (300 - window + 1) // page] = spare
+    _close(_attend(step, cache, q, bits, window, 0.125), step, q, keys, values, bits, window, 0.125)
