@@ -56,8 +56,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { return pack2
 
 // A library built with -DHALF_INPUTS=1 has the portions' kernel alone, over keys and values in float16 that were unpacked from a
 // cache of fewer bits, with exponents (half_parts.h) for every 32 keys: `exponents` [pages][heads][page size / 32][2], the keys'
-// and the values'.  Queries (bfloat16 as ever) are turned into float16 with an exponent a row, probabilities are float16: what was
+// and the values'.  Queries (bfloat16 as ever) are turned into float16 with an exponent a row: what was
 // held in few bits is rounded to 2^-12 of itself where bfloat16 would take 2^-9, and the result to bfloat16 once.
+// Weights are float16 too, 2^7 times what they are elsewhere (an addition to the exponent that every one of them has anyway, and their
+// sum is that much larger as well): up to 2^15, so that the small end of float16 lies at 2^-21 of the reference (below it they are off by up to 2^-32
+// of that) and not at 2^-14.  Without it 131,072 keys of a weight of just under 2^-25 were lost from a result, 2^-8 of it.
 // A score's exponent is part of its row's scale, or multiplied into a tile's scores where the keys have one; values with another
 // exponent than the sums have rescale the sums, in float32, as a new reference does.  That no tile of an item has exponents is the
 // rule, and found out once an item.
@@ -65,6 +68,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { return pack2
 #include "half_parts.h"
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 #define PACK_P pack2_f16
+#define P_EXPONENT 7
+#define P_REFERENCE(x) ((x) + P_EXPONENT)
 #define WIDE_MFMA(A, B, C) __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, (A).u), __builtin_bit_cast(half8, (B).u), C, 0, 0, 0)
 #define HALF_PARAMS , const int* __restrict__ exponents
 #define LOOK_FOR_EXPONENTS look_for_exponents();
@@ -72,6 +77,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 #define HALF_ARGS , exponents
 #else
 #define PACK_P pack_bf16
+#define P_REFERENCE(x) (x)
 #define WIDE_MFMA(A, B, C) __builtin_amdgcn_mfma_f32_16x16x32_bf16((A).v, (B).v, C, 0, 0, 0)
 #define HALF_PARAMS
 #define LOOK_FOR_EXPONENTS
@@ -161,7 +167,7 @@ __device__ __forceinline__ float tanh_of(float x) {
       ALPHA = __builtin_amdgcn_exp2f(fmaf(M_RUN, scale_log2e, neg_mc));                                      \
       L_RUN *= ALPHA;                                                                                        \
       M_RUN = m_new;                                                                                         \
-      NEG_MC = neg_mc;                                                                                       \
+      NEG_MC = P_REFERENCE(neg_mc);                                                                          \
     }                                                                                                        \
     float pv[8];                                                                                             \
     float psum = 0.f;                                                                                        \
@@ -1042,9 +1048,10 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
     if (!row_valid[rt]) continue;
 #ifdef HALF_INPUTS
     const float scale_log2e = row_scale[rt];
-    const float up = power_of_two(acc_exponent);
+    const float up = power_of_two(acc_exponent), down = power_of_two(-P_EXPONENT);
+    l_row *= down;
 #pragma unroll
-    for (int dt = 0; dt < D_TILES; ++dt) acc[rt][dt] *= up;
+    for (int dt = 0; dt < D_TILES; ++dt) acc[rt][dt] = acc[rt][dt] * down * up;
 #endif
     if (w[4] >= 0) {
       // the item's keys are cut into w[5] chunks and this block had one of them: its row tile t

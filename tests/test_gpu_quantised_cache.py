@@ -439,3 +439,21 @@ def test_keys_that_a_window_has_passed_may_hold_anything(bits, page):
     cache[spare] = 0x7E  # steps and offsets of 8.4e37
     step.table[0, : (300 - window + 1) // page] = spare
     _close(_attend(step, cache, q, bits, window, 0.125), step, q, keys, values, bits, window, 0.125)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_small_weights_of_portions_add_up(bits):
+    """A portion over one key that takes nearly all of the softmax, with a value of zeros, and thousands of keys of e^-18 of it, with
+    values of ones: the result is what the small weights make together.  A weight is off by 2^-32 of the row's largest at most, or by
+    2^-12 of itself, in all n 2^-32 and 2^-12 of the result; its exponential and the sums by under 2^-16 of it, and the result is rounded."""
+    new, kv, dim, group = [80], [4000], 64, 4
+    step, cache, q, keys, values = _case(new, kv, 32, group, 1, dim, bits, torch.bfloat16, None, 43)
+    keys[0][:], values[0][:], q[:] = 0.0, 1.0, 1.0
+    keys[0][5], values[0][5] = 2.25, 0.0  # a score of 64 * 2.25 / 8 = 18
+    held.put_all(cache, step.table, kv, keys, values, bits)
+    got = _attend(step, cache, q, bits, None, 0.125).cpu().double()
+    others = torch.arange(kv[0] - new[0], kv[0]).double()[:, None]  # a query at p reads p small ones
+    want = others * math.exp(-18) / (1 + others * math.exp(-18))
+    limit = others * 2.0 ** -32 + (2.0 ** -12 + 2.0 ** -16) * want
+    limit = limit + 2.0 ** -8 * (want + limit)
+    assert ((got - want).abs() <= limit).all(), float(((got - want).abs() / limit).max())
