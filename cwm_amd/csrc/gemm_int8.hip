@@ -1,5 +1,5 @@
 // y[M, N] = a[m] w[n] sum over k of X[m, k] W[n, k] (+ bias[n]): a product of 8-bit integers with a float32 scale for every
-// token and every output channel, and the kernel that makes the integers of a row: X[m, k] = round(x[m, k] / a[m]),
+// token and every output channel, and the kernel that makes the integers of a row: X[m, k] = round(x[m, k] / a[m]) within -127 .. 127,
 // a[m] = max_k |x[m, k]| / 127, ties to even, float32 throughout.  The sums are exact in 32 bits up to a K of 133,144 (127^2 K <
 // 2^31), so neither their order nor where K is cut shows in a result: y is rounded in the sum's conversion to float32 (beyond
 // 2^24), twice by the scales, and once to its type.
@@ -28,12 +28,14 @@ template <> __device__ __forceinline__ void load4<bf16_t>(const bf16_t* p, float
   x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u), x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
 }
 
-__device__ __forceinline__ int int8_of(float x, float a) {
-  return (int)rintf(x / a);  // a true quotient: ties are common among short numbers, and a product with 1 / a would decide them otherwise
-}
+// A true quotient: ties are common among short numbers, and a product with 1 / a would decide them otherwise.  It ends at 127: a
+// scale of one or two of float32's smallest steps (a row up to 2e-41 or so) is off by a large part of itself, and quotients would
+// reach 190.
+__device__ __forceinline__ int int8_of(float x, float a) { return (int)fminf(fmaxf(rintf(x / a), -127.f), 127.f); }
 
 // The integers of N numbers.  A product with 1 / a decides one except next to a tie, where it may be off by its own rounding (the
-// quotient is at most 127, a reciprocal off by 2^-23 and a product by 2^-24 make it 2.3e-5): there it is the quotient.
+// quotient is at most 127, a reciprocal off by 2^-23 and a product by 2^-24 make it 2.3e-5): there it is the quotient.  A scale with
+// a reciprocal is 2^-128 at least, off by 2^-22 of itself at most, and its quotients round to 127 at most.
 template <int N> __device__ __forceinline__ void int8_all(const float (&x)[N], float a, int (&c)[N]) {
   const float inv = __builtin_amdgcn_rcpf(a);  // an infinity for the smallest scales
   float r[N], off = 0.f;

@@ -351,9 +351,9 @@ INT8_FUSED_ROWS, INT8_FUSED_K = 4, 16384  # csrc/gemm_int8.hip: rows of x, and t
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """`x` [M, K] (float32 or bfloat16) as int8 [M, K] and a float32 scale a row [M]: the scale is the row's largest magnitude over
-    127, the integers x / scale rounded, ties to even.  A row of zeros has a scale of 0; one with an infinity or a NaN has a NaN
-    for its scale.  The integers are a view of rows padded with zeros to a multiple of 128, which `linear_int8` likes best for
-    its weights."""
+    127, the integers x / scale rounded, ties to even, and limited to -127 .. 127 (which tells in rows below 2.3e-41, whose scale
+    is a few of float32's smallest steps).  A row of zeros has a scale of 0; one with an infinity or a NaN has a NaN for its scale.
+    The integers are a view of rows padded with zeros to a multiple of 128, which `linear_int8` likes best for its weights."""
     KernelError, _check, _code = _base()
     stream = _check_device(x)
     if x.dim() != 2 or x.shape[1] < 1 or (x.shape[1] > 1 and x.stride(1) != 1):

@@ -228,3 +228,39 @@ def test_k_in_parts_captured():
         replayed = out.clone()
         torch.cuda.synchronize()
         assert torch.equal(replayed, want[i]) and torch.equal(ops.linear_int8(sources[i], w, s), want[i])
+
+
+@pytest.mark.parametrize("k", [16, 100, 4096])
+def test_integers_end_at_127(k):
+    """Rows whose largest is a few of float32's smallest steps: their scale is one such step, or two, and quotients pass 127."""
+    step = 2.0 ** -149
+    x = torch.zeros(6, k)
+    for m, top in enumerate((190, 127, 100, 64, 63, 191)):
+        x[m, 0], x[m, k - 1], x[m, 3] = top * step, -top * step, 7 * step
+    want, a = _quantised(x.clone())
+    steps = torch.where(a[:, None] > 0, torch.round(x.double() / a.double()[:, None]), torch.zeros_like(x, dtype=torch.float64)).clamp(-127, 127)
+    assert a.tolist() == [step, step, step, step, 0.0, 2 * step] and float(steps[0, 0]) == 127
+    codes, scale = ops.quantize_rows(x.to(DEV))
+    assert torch.equal(scale.cpu(), a) and torch.equal(codes.cpu().double(), steps)
+    if k % 16:
+        return
+    w, s = _weight(20, k, 8)
+    s = s * 2.0 ** 120
+    exact = (steps @ w.double().t()) * a.double()[:, None] * s.double()
+    for rows, tile in ((4, -1), (1, -1), (6, 0), (6, 3), (6, None)):
+        if tile == 3 and k < 128:
+            continue
+        y = ops.linear_int8(x[:rows].to(DEV), w.to(DEV), s.to(DEV), tile=tile)
+        off = (y.cpu().double() - exact[:rows]).abs()
+        assert (off <= 3.01 * 2.0 ** -24 * exact[:rows].abs()).all(), (rows, tile)
+
+
+def test_scales_that_are_subnormal():
+    """Around the scales whose reciprocal float32 just holds, 2^-128, and the smallest normal one."""
+    for k in (64, 100):
+        x = _rows(9, k, torch.float32, 21 + k)
+        x = x / x.abs().amax(1, keepdim=True) * 127
+        x = x * 2.0 ** torch.tensor([-125.0, -126, -126.9, -127, -127.5, -128, -129, -135, -140])[:, None]
+        codes, scale = ops.quantize_rows(x.to(DEV))
+        want, a = _quantised(x)
+        assert torch.equal(scale.cpu(), a) and torch.equal(codes.cpu(), want) and int(want.abs().max()) == 127
