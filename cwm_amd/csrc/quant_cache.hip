@@ -323,13 +323,15 @@ quant_kv_write_kernel(const T* __restrict__ k, long k_stride, const T* __restric
   codes_of<BITS>(x, word, c);
   uint8_t* const page = dst_page[tk];
   if (!mine || !page) return;
-  // sums of signed codes, and H on every one of them at the end: nothing is carried over
-  uint32_t codes[WORDS];
+  // sums of signed codes modulo 2^32, and H on every one of them at the end: nothing is carried over
+  uint32_t u[8], codes[WORDS];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) u[e] = (uint32_t)c[e];
   if constexpr (BITS == 4) {
-    codes[0] = ((((((c[7] * 16 + c[5]) * 16 + c[3]) * 16 + c[1]) * 16 + c[6]) * 16 + c[4]) * 16 + c[2]) * 16 + c[0] + 0x88888888u;
+    codes[0] = ((((((u[7] * 16 + u[5]) * 16 + u[3]) * 16 + u[1]) * 16 + u[6]) * 16 + u[4]) * 16 + u[2]) * 16 + u[0] + 0x88888888u;
   } else {
-    codes[0] = ((c[3] * 256 + c[2]) * 256 + c[1]) * 256 + c[0] + 0x80808080u;
-    codes[WORDS - 1] = ((c[7] * 256 + c[6]) * 256 + c[5]) * 256 + c[4] + 0x80808080u;
+    codes[0] = ((u[3] * 256 + u[2]) * 256 + u[1]) * 256 + u[0] + 0x80808080u;
+    codes[WORDS - 1] = ((u[7] * 256 + u[6]) * 256 + u[5]) * 256 + u[4] + 0x80808080u;
   }
   uint8_t* const to = page + (size_t)head * at.bytes;
   const int slot = dst_slot[tk];

@@ -457,3 +457,18 @@ def test_small_weights_of_portions_add_up(bits):
     limit = others * 2.0 ** -32 + (2.0 ** -12 + 2.0 ** -16) * want
     limit = limit + 2.0 ** -8 * (want + limit)
     assert ((got - want).abs() <= limit).all(), float(((got - want).abs() / limit).max())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_groups_whose_codes_are_nearly_all_the_lowest(bits):
+    """The words of codes 0 and 2H - 1 side by side, at every place of a group."""
+    dim, page, n = 64, 32, 32
+    step = held.Step([n], [n], page)
+    x = torch.full((n, 1, dim), -1.0)
+    for t in range(n):
+        x[t, 0, [t, 63 - t]] = 1.0
+    want = torch.zeros((step.pool, *ops.quant_page_shape(1, dim, page, bits)), dtype=torch.uint8)
+    cache, at = want.to(DEV), step.positions.long()
+    held.put_tokens(want, step.table[0, at // page].long(), at % page, x, x, bits)
+    ops.quant_kv_write(x.to(DEV), x.to(DEV), step.positions.to(DEV), None, cache, step.table.to(DEV), step.seq.to(DEV), bits)
+    assert torch.equal(cache.cpu(), want)
