@@ -89,6 +89,8 @@ def pool_sizes(
     if free_bytes is None:
         if device.type != "cuda":
             raise ValueError("max_seq must be given when no HIP device is used")
+        if model.runtime.weight_bits is not None:
+            torch.cuda.empty_cache()  # the memory of the matrices' originals is still the allocator's
         free_bytes, _total = torch.cuda.mem_get_info(device)
     # nine tenths of what is free after the reserve: the rest is slack for the allocator
     budget = int(0.9 * (free_bytes - int(args.prefill_gb * 1e9)))

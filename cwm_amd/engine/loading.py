@@ -11,7 +11,7 @@ import torch
 from ..config.registry import load_config, parse_config
 from ..models.model import Model
 from ..parts.base import Runtime
-from ..weights.loader import load_tensors
+from ..weights.loader import TensorsOnDemand, load_tensors, open_tensors
 from ..weights.random_init import random_tensor
 
 _DTYPES = {
@@ -68,7 +68,9 @@ def load_model(
     act_dtype = parse_dtype(dtype)
     arch, config = load_config(folder)
     model = Model(arch.build_plan(config), cache_bits)
-    tensors = load_tensors(folder, model.tensor_specs(), act_dtype, device, keep_float32)
+    # matrices that are held in fewer bits: layer by layer, so that a model that fits in those can be loaded
+    load = load_tensors if weight_bits is None else open_tensors
+    tensors = load(folder, model.tensor_specs(), act_dtype, device, keep_float32)
     copies = wants_stream_copies(model, act_dtype, device, stream_copies)
     model.bind(tensors, Runtime(device=device, act_dtype=act_dtype, stream_copies=copies, weight_bits=weight_bits))
     return model, config
@@ -91,10 +93,12 @@ def random_model(
     act_dtype = parse_dtype(dtype)
     arch, typed = parse_config(config)
     model = Model(arch.build_plan(typed), cache_bits)
-    tensors = {
-        name: random_tensor(name, spec, seed, std, norm_init, act_dtype, device)
-        for name, spec in model.tensor_specs().items()
-    }
+    specs = model.tensor_specs()
+    tensors: Mapping[str, torch.Tensor] = TensorsOnDemand(
+        specs, lambda name: random_tensor(name, specs[name], seed, std, norm_init, act_dtype, device)
+    )
+    if weight_bits is None:
+        tensors = dict(tensors)
     copies = wants_stream_copies(model, act_dtype, device, stream_copies)
     model.bind(tensors, Runtime(device=device, act_dtype=act_dtype, stream_copies=copies, weight_bits=weight_bits))
     return model, typed

@@ -142,14 +142,23 @@ class Model:
         if runtime.weight_bits is not None:
             self._check_weight_bits(runtime.weight_bits)
         self.runtime = runtime
+        several: Dict[str, torch.Tensor] = {}  # tensors that several parts may name, asked for once
+
+        def shared(name: str) -> torch.Tensor:
+            if name not in several:
+                several[name] = tensors[name]
+            return several[name]
+
         for layer, block in zip(self.plan.layers, self.blocks):
             prefix = layer.prefix
-            own = {n[len(prefix):]: t for n, t in tensors.items() if n.startswith(prefix)}
-            own.update({n: tensors[n[1:]] for n in block.tensor_specs() if is_absolute(n)})
+            # a layer's tensors are asked for here and held no longer than the layer itself holds them (`TensorsOnDemand`)
+            own = {n[len(prefix):]: tensors[n] for n in tensors if n.startswith(prefix)}
+            own.update({n: shared(n[1:]) for n in block.tensor_specs() if is_absolute(n)})
             block.bind(own, runtime)
+            del own
         for _role, prefix, part in self._ends:
             names = part.tensor_specs()
-            part.bind({name: tensors[prefix + name] for name in names}, runtime)
+            part.bind({name: shared(prefix + name) for name in names}, runtime)
 
     @property
     def replayable(self) -> bool:

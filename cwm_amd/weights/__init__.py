@@ -1,4 +1,4 @@
-from .loader import WeightError, load_tensors, target_dtype, weight_files
+from .loader import TensorsOnDemand, WeightError, load_tensors, open_tensors, target_dtype, weight_files
 from .random_init import random_tensor, random_tensors, write_random_model
 
 __all__ = [

@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import glob
 import os
-from typing import Dict, List, Mapping
+from typing import Callable, Dict, Iterable, Iterator, List, Mapping
 
 import torch
 
@@ -60,6 +60,29 @@ def target_dtype(
     raise WeightError(f"{name}: stored type {stored} is not supported (bfloat16, float16, float32, float64)")
 
 
+class TensorsOnDemand(Mapping[str, torch.Tensor]):
+    """Tensors by name that are made anew whenever one is asked for, and kept by nobody else: a model whose layers hold them in
+    another form (`Runtime.weight_bits`) then has the originals of one layer at a time beside what it holds."""
+
+    def __init__(self, names: Iterable[str], make: Callable[[str], torch.Tensor]) -> None:
+        self._names = dict.fromkeys(names)
+        self._make = make
+
+    def __getitem__(self, name: str) -> torch.Tensor:
+        if name not in self._names:
+            raise KeyError(name)
+        return self._make(name)
+
+    def __iter__(self) -> Iterator[str]:
+        return iter(self._names)
+
+    def __len__(self) -> int:
+        return len(self._names)
+
+    def __contains__(self, name: object) -> bool:
+        return name in self._names
+
+
 def load_tensors(
     folder: str,
     specs: Mapping[str, TensorSpec],
@@ -70,6 +93,17 @@ def load_tensors(
     """All tensors that `specs` names, checked and moved to `device`.  `keep_float32`: in
     bfloat16 mode, tensors stored in 32 bits all stay float32 (their products then run on the
     float32 kernel)."""
+    return dict(open_tensors(folder, specs, act_dtype, device, keep_float32))
+
+
+def open_tensors(
+    folder: str,
+    specs: Mapping[str, TensorSpec],
+    act_dtype: torch.dtype,
+    device: torch.device,
+    keep_float32: bool = False,
+) -> TensorsOnDemand:
+    """The same, checked, and each one read and moved to `device` when it is asked for."""
     from safetensors import safe_open
 
     where: Dict[str, str] = {}
@@ -106,13 +140,10 @@ def load_tensors(
             lines.append(f"  stored in more than one file ({len(duplicates)}): " + ", ".join(sorted(duplicates)))
         raise WeightError("\n".join(lines))
 
-    out: Dict[str, torch.Tensor] = {}
-    by_file: Dict[str, List[str]] = {}
-    for name, path in where.items():
-        by_file.setdefault(path, []).append(name)
-    for path, names in by_file.items():
-        with safe_open(path, framework="pt", device="cpu") as fh:
-            for name in names:
-                dtype = target_dtype(stored[name], specs[name].kind, act_dtype, name, specs[name].precision, keep_float32)
-                out[name] = fh.get_tensor(name).to(device=device, dtype=dtype).contiguous()
-    return out
+    dtypes = {name: target_dtype(stored[name], specs[name].kind, act_dtype, name, specs[name].precision, keep_float32) for name in where}
+    files = {path: safe_open(path, framework="pt", device="cpu") for path in dict.fromkeys(where.values())}
+
+    def read(name: str) -> torch.Tensor:
+        return files[where[name]].get_tensor(name).to(device=device, dtype=dtypes[name]).contiguous()
+
+    return TensorsOnDemand(where, read)
