@@ -1206,7 +1206,7 @@ def _attention_plan(
         wide_cut_below = -(-2 * _compute_units(device) // n_kv) if device.type == "cuda" else 0
         item_tiles = WIDE_TILES
         if device.type == "cuda" and halves:
-            item_tiles = wide_item_tiles(batch.q_lens, batch.kv_lens, group, n_kv, head_dim, wide_cut_below, _compute_units(device), packed)
+            item_tiles = wide_item_tiles(batch.q_lens, batch.kv_lens, group, n_kv, head_dim, wide_cut_below, _compute_units(device), packed, window)
         plan = build_plan(batch.q_lens, batch.kv_lens, group, window, wide_cut_below, chunk, finer, item_tiles, packed)
         flat = np.concatenate([plan.work.reshape(-1), plan.work_wide.reshape(-1), plan.merge.reshape(-1)]).astype(np.int32)
         host = torch.from_numpy(flat)

@@ -23,7 +23,13 @@ WIDE_CHUNK_FINE = 2048  # the same for a sequence with very few such blocks
 # Both, for a step whose cache holds 4 or 8 bits (`packed`).  us with 8,192 and 2,048 keys / 1,024 (32 query heads on 8 of 128): 513 tokens to
 # 3,585 keys 96 / 74, 100 to 6,000 96 / 58, 64 to 30,000 95 / 87, 300 to 1,300, 2,300, 300 and 800 65 / 65; chunks of 512 make the
 # last but one 117.
+# A chunk of a block's keys is a partial result of 128 rows in float32 (68 KB for a head of 128), written and read again: with chunks of one
+# length at any context 1,300 tokens at 131,072 keys left 4.2 GB of them.  So the chunks double until a sequence has at most
+# PACKED_WIDE_BLOCKS times the blocks with which every compute unit has two, 138 MB of heads of 128.  us with chunks of 1,024 and
+# with 2, 4 and 8 times those blocks (48 query heads on 8 of 128): 1,300 tokens to 131,072 keys 8,808 / 5,039, 4,985, 5,216; 512 to 131,072
+# 3,583 / 1,842, 1,872, 1,977; 300 to 30,000 403 / 363, 356, 399; 800 to 9,000 248 / 283, 222, 247; 1,300 to 4,000 182 / 166, 182, 182.
 PACKED_WIDE_CHUNK = 1024
+PACKED_WIDE_BLOCKS = 4
 # Most blocks of WIDE_TILES row tiles a compute unit, by the head size, of a launch that takes half as high ones instead.  Such a
 # block walks its keys alone, so with few blocks the longest one's walk is the launch: a tile of 32 keys costs it 1.4 us with 128
 # rows and 0.9 with 64, and twice as many blocks read keys from LDS.  Blocks of 128 rows, us with them and with 64 rows: heads of
@@ -99,7 +105,6 @@ def build_plan(
     so that it is the same whatever else the batch holds.  `few_heads`: see `chunk_keys`.  `wide_tiles`: row tiles of a wide
     item, WIDE_TILES or what `wide_item_tiles` answers (a sequence's items are counted in the former where that decides on a cut).
     `packed`: the step's cache holds 4 or 8 bits, see `chunk_keys` and PACKED_WIDE_CHUNK."""
-    wide_chunk, wide_chunk_fine = wide_chunks(packed)
     q = np.asarray(q_lens, dtype=np.int64)
     kv = np.asarray(kv_lens, dtype=np.int64)
     n_rows = q * group
@@ -119,7 +124,7 @@ def build_plan(
         wide_lo.append(lo[first])
         wide_hi.append(hi[last])
         wide_n_tiles.append(last - first + 1)
-        wide_cut.append(np.full(n_items, 0 if n_wide >= wide_cut_below else (wide_chunk if 8 * n_wide >= wide_cut_below else wide_chunk_fine)))
+        wide_cut.append(np.full(n_items, wide_chunk(n_wide, int(q[b]), int(kv[b]), window, wide_cut_below, packed)))
 
     # ---- all tiles of the other sequences at once, in the order (sequence, tile, chunk)
     small = np.nonzero(~is_wide)[0]
@@ -213,21 +218,35 @@ def wide_chunks(packed: bool) -> "tuple[int, int]":
     return (PACKED_WIDE_CHUNK, PACKED_WIDE_CHUNK) if packed else (WIDE_CHUNK, WIDE_CHUNK_FINE)
 
 
+def wide_chunk(n_wide: int, n_new: int, kv: int, window: Optional[int], wide_cut_below: int, packed: bool) -> int:
+    """Keys after which the blocks of many rows of a sequence with `n_wide` of them are cut, 0 if they are not (it has enough)."""
+    if n_wide >= wide_cut_below:
+        return 0
+    few, very_few = wide_chunks(packed)
+    chunk = few if 8 * n_wide >= wide_cut_below else very_few
+    if packed:
+        n_keys = kv if window is None else min(kv, window + n_new - 1)
+        while n_wide * -(-n_keys // chunk) > PACKED_WIDE_BLOCKS * wide_cut_below:
+            chunk *= 2
+    return chunk
+
+
 def wide_item_tiles(
-    q_lens: Sequence[int], kv_lens: Sequence[int], group: int, n_kv: int, head_dim: int, wide_cut_below: int, units: int, packed: bool = False
+    q_lens: Sequence[int], kv_lens: Sequence[int], group: int, n_kv: int, head_dim: int, wide_cut_below: int, units: int, packed: bool = False,
+    window: Optional[int] = None,
 ) -> int:
     """Row tiles of a wide item for a step of these lengths on `units` compute units: half of WIDE_TILES where blocks of
     WIDE_TILES are few (`WIDE_HALF_BLOCKS`; other head sizes have no such blocks).  A row's bits are the same either way unless
     its keys are cut, so a step with a cut sequence keeps the whole size, or first keys are kept beside a window, for which the
     caller does not ask."""
     blocks, most = 0, WIDE_HALF_BLOCKS.get(head_dim, 0) * units
-    wide_chunk, wide_chunk_fine = wide_chunks(packed)
     for q, kv in zip(q_lens, kv_lens):
         n_tiles = -(-q * group // ROWS_PER_TILE)
         if n_tiles <= SPLIT_MAX_TILES:
             continue
         n_wide = -(-n_tiles // WIDE_TILES)
-        if n_wide < wide_cut_below and kv > (wide_chunk if 8 * n_wide >= wide_cut_below else wide_chunk_fine):
+        cut = wide_chunk(n_wide, q, kv, window, wide_cut_below, packed)
+        if 0 < cut < kv:
             return WIDE_TILES
         blocks += n_wide * n_kv
     return WIDE_TILES // 2 if 0 < blocks <= most else WIDE_TILES

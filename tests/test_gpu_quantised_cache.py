@@ -472,3 +472,17 @@ def test_groups_whose_codes_are_nearly_all_the_lowest(bits):
     held.put_tokens(want, step.table[0, at // page].long(), at % page, x, x, bits)
     ops.quant_kv_write(x.to(DEV), x.to(DEV), step.positions.to(DEV), None, cache, step.table.to(DEV), step.seq.to(DEV), bits)
     assert torch.equal(cache.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_portions_whose_chunks_are_doubled(monkeypatch, dtype):
+    """Short chunks, so that a short context has more of them than a step may leave partial results of."""
+    from cwm_amd.ops import attention_plan
+
+    monkeypatch.setattr(attention_plan, "PACKED_WIDE_CHUNK", 128)
+    monkeypatch.setattr(attention_plan, "PACKED_WIDE_BLOCKS", 1)
+    new, kv, dim, bits = [100, 1], [3001, 500], 64, 4
+    for window in (None, 700):
+        step, cache, q, keys, values = _case(new, kv, 32, 32, 8, dim, bits, dtype, window, 46)
+        assert attention_plan.wide_chunk(4, 100, 3001, window, 64, True) == (256 if window is None else 128)
+        _close(_attend(step, cache, q, bits, window, 0.125), step, q, keys, values, bits, window, 0.125)

@@ -3,7 +3,9 @@
 import numpy as np
 import pytest
 
-from cwm_amd.ops.attention_plan import PACKED_WIDE_CHUNK, build_plan, capacity_until, chunk_keys, pad_plan, wide_chunks
+from cwm_amd.ops.attention_plan import (
+    PACKED_WIDE_BLOCKS, PACKED_WIDE_CHUNK, WIDE_TILES, build_plan, capacity_until, chunk_keys, pad_plan, wide_chunk, wide_chunks, wide_item_tiles,
+)
 
 
 def test_chunks():
@@ -33,3 +35,32 @@ def test_a_captured_step_holds_its_packed_lists():
         _, capacity = capacity_until(q, kv, 6, window, 64, 12000, packed=True)
         for t in range(0, 3900, 13):
             assert pad_plan(build_plan(q, [n + t for n in kv], 6, window, 64, packed=True), capacity) is not None, (window, t)
+
+
+@pytest.mark.parametrize("new,kv,window", [(1300, 131072, None), (512, 131072, None), (22, 10 ** 6, None), (64, 30000, None), (1300, 131072, 8192), (700, 701, None)])
+def test_partial_results_of_portions_do_not_grow_with_the_context(new, kv, window):
+    """The blocks of a sequence that is cut are at most four times those with which every compute unit has two (64 a key/value head), and one more
+    for each row of blocks, whose range need not begin at a cut."""
+    group, cut_below = 6, 64
+    n_wide = -(-new * group // (16 * WIDE_TILES))
+    plan = build_plan([new], [kv], group, window, cut_below, packed=True)
+    assert plan.work_wide.shape[0] <= PACKED_WIDE_BLOCKS * cut_below + n_wide
+    assert plan.n_partials <= WIDE_TILES * plan.work_wide.shape[0]
+    assert plan.n_partials * 8 * 16 * (128 + 4) * 4 <= 175e6  # bytes of eight heads of 128
+    alone = build_plan([new], [kv], group, window, cut_below, packed=True).work_wide
+    beside = build_plan([5, new, 300], [9, kv, 9000], group, window, cut_below, packed=True).work_wide
+    ranges = lambda w, b: sorted(tuple(int(x) for x in r[1:4]) for r in w if r[0] == b)  # noqa: E731
+    assert ranges(alone, 0) == ranges(beside, 1)
+
+
+def test_chunks_of_portions():
+    def cut(n_new, kv, window=None, group=4):
+        return wide_chunk(-(-n_new * group // 128), n_new, kv, window, 64, True)
+
+    assert [cut(64, 30000), cut(513, 3585, 2048), cut(300, 300), cut(64, 131072), cut(512, 131072), cut(1300, 131072)] == [1024, 1024, 1024, 1024, 8192, 32768]
+    assert cut(2048, 4096) == 0 and wide_chunk(10, 300, 10 ** 6, None, 64, False) == 8192 and wide_chunk(3, 70, 10 ** 6, None, 64, False) == 2048
+    assert cut(300, 131072, 2048) == 1024  # what a window reads counts, not what lies before it
+    assert wide_item_tiles([300, 40], [300, 500], 4, 8, 128, 64, 256, True) == 4
+    assert wide_item_tiles([300, 40], [300, 5000], 4, 8, 128, 64, 256, True) == WIDE_TILES
+    # a portion in a window that is shorter than its chunk may be cut at a multiple of it all the same
+    assert wide_item_tiles([300], [131072], 4, 8, 128, 64, 256, True, 700) == WIDE_TILES
