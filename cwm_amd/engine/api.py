@@ -40,8 +40,8 @@ class GenArgs:
     # output channel and quantise the activations token by token (dense decoder only; embedding and head stay as they are)
     expected_seq: int = -1  # not in the reference: tokens a typical request holds; how free memory is split between
     # layer groups when max_seq is negative (negative: the context length the model's configuration names)
-    prefill_gb: float = 2  # memory kept free for activations when max_seq is negative (with cache_bits also for one layer's keys and
-    # values, in 16 bits, of the sequences that have a prompt portion in a step)
+    prefill_gb: float = 2  # memory kept free for activations when max_seq is negative (what cache_bits unpacks for prompt portions
+    # is kept free beside it; with max_seq given, both are the caller's)
     gpu_gb: float = 74  # the reference's memory budget: ignored, free memory is measured
 
     sync_freq: int = 10  # decode steps that run back to back, each fed by the tokens the one before sampled on the

@@ -27,7 +27,8 @@ import torch
 from ..cache.manager import CacheManager
 from ..cache.storage import CacheStorage
 from ..models.model import Model
-from ..parts.base import PagedKVSpec
+from .. import ops
+from ..parts.base import PagedKVSpec, QuantKVSpec
 from ..sampling.sampler import RequestStream, Sampler, effective_temperature
 from .api import GenArgs, Packet
 from .loading import load_model, random_model
@@ -59,6 +60,9 @@ def pool_sizes(
     group is never made larger than `max_batch` requests can fill; what that saves goes to the
     keep-all group.  No pool is sized for the worst case of `max_batch` requests up front:
     when any group runs out of pages the scheduler preempts, whichever group it is.
+    With a cache of 4 or 8 bits the reserve also has what one layer's attention unpacks of it for prompt portions
+    (`ops.quant_attention_workspace`), for requests up to the model's context length, or `expected_seq` where that is longer; with
+    neither, up to all that the memory holds.
     `free_bytes` stands in for the measured free memory (tests).
     """
     page = args.cache_block
@@ -92,8 +96,9 @@ def pool_sizes(
         if model.runtime.weight_bits is not None:
             torch.cuda.empty_cache()  # the memory of the matrices' originals is still the allocator's
         free_bytes, _total = torch.cuda.mem_get_info(device)
+    reserve = int(args.prefill_gb * 1e9) + _unpacking_bytes(model, args, free_bytes, sum(per_page.values()) / page)
     # nine tenths of what is free after the reserve: the rest is slack for the allocator
-    budget = int(0.9 * (free_bytes - int(args.prefill_gb * 1e9)))
+    budget = int(0.9 * (free_bytes - reserve))
     expected = args.expected_seq if args.expected_seq > 0 else (model.plan.max_positions or 0)
     # pages that one expected request holds of each group
     share: Dict[Hashable, int] = {}
@@ -117,10 +122,26 @@ def pool_sizes(
     smallest = min(sizes.values())
     if smallest < 1:
         raise MemoryError(
-            f"{free_bytes / 1e9:.1f} GB of free memory less {args.prefill_gb} GB for activations leave no room for "
+            f"{free_bytes / 1e9:.1f} GB of free memory less {reserve / 1e9:g} GB for activations leave no room for "
             f"one page of {page} tokens in every layer group (bytes per page: {per_page})"
         )
     return sizes
+
+
+def _unpacking_bytes(model: Model, args: GenArgs, free_bytes: int, token_bytes: float) -> int:
+    """Bytes of the pools' memory that the attention of a layer may unpack keys and values to; a token of all layers has `token_bytes`."""
+    if model.runtime.act_dtype != torch.bfloat16:
+        return 0  # float32 portions read the codes as they are
+    keys = max(args.expected_seq, model.plan.max_positions or 0)
+    if keys <= 0:
+        keys = int(max(free_bytes, 0) / token_bytes)
+    units = torch.cuda.get_device_properties(model.runtime.device).multi_processor_count if model.runtime.device.type == "cuda" else 256
+    most = 0
+    for spec in model.cache_specs:
+        if isinstance(spec, QuantKVSpec):
+            kept = spec.keys_kept(args.max_prefill)
+            most = max(most, ops.quant_attention_workspace(spec.n_kv_heads, spec.head_dim, keys if kept is None else min(keys, kept), units))
+    return most
 
 
 class Engine:

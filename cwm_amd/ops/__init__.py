@@ -1530,6 +1530,6 @@ from .projected import (  # noqa: E402
     MAX_CONV_QK_CHANNELS, MAX_CONV_QK_TAPS, conv_qk_rope_write, latent_rows,
 )
 from .quantised import (  # noqa: E402
-    CACHE_BITS, INT8_MAX_K, QUANT_MAX_DIM, int8_limits, linear_int8, quant_cache_limits, quant_kv_read, quant_kv_write, quant_page_shape,
-    quant_paged_attention, quantize_rows,
+    CACHE_BITS, INT8_MAX_K, QUANT_MAX_DIM, int8_limits, linear_int8, quant_attention_workspace, quant_cache_limits, quant_kv_read, quant_kv_write,
+    quant_page_shape, quant_paged_attention, quantize_rows,
 )

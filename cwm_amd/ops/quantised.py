@@ -6,8 +6,9 @@ host; there is no CPU path."""
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 import functools
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import numpy as np
 import torch
@@ -234,6 +235,59 @@ def quant_kv_read(
 
 UNPACK_KEYS = 64  # csrc/quant_cache.hip
 UNPACK_PAGE = 256  # tokens of a page of the unpacked cache
+# Bytes of unpacked keys and values and of partial results that the portions of a step take at a time: the sequences of a step take turns,
+# one at least in a turn.  One of 131,072 keys and 8 heads of 128 has 512 MiB of keys and values, read in 5 ms: what two more launches cost is nothing.
+UNPACK_BYTES = 1 << 29
+
+
+def _portion_bytes(n_kv: int, head_dim: int, n_keys: int, n_slots: int) -> int:
+    """Bytes of the unpacked keys and values of a sequence of which portions read `n_keys`, and of `n_slots` partial results of a row tile."""
+    pages = -(-n_keys // UNPACK_PAGE) + 1  # a window need not begin with a page
+    return n_kv * (pages * (UNPACK_PAGE * head_dim * 4 + UNPACK_PAGE // 32 * 8) + n_slots * 16 * (head_dim + 4) * 4)
+
+
+def quant_attention_workspace(n_kv: int, head_dim: int, n_keys: int, units: int) -> int:
+    """The most bytes that `quant_paged_attention` takes for the portions of a step whose sequences hold up to `n_keys` keys, on `units`
+    compute units (bfloat16)."""
+    from .attention_plan import PACKED_WIDE_BLOCKS, WIDE_TILES
+
+    cut_below = -(-2 * units // n_kv)  # a sequence is cut if it has fewer blocks of WIDE_TILES row tiles, see `wide_chunk`
+    return max(UNPACK_BYTES, _portion_bytes(n_kv, head_dim, n_keys, (PACKED_WIDE_BLOCKS + 1) * cut_below * WIDE_TILES))
+
+
+def _turns(batch, group: int, window: Optional[int], n_kv: int, head_dim: int, device: torch.device) -> list:
+    """Pieces of the step that have some of its portions each, and the others as if they had no new tokens, where all of them would unpack
+    more than UNPACK_BYTES; none where they may go together.  Made once a step.  A row's result does not depend on what else is in its piece."""
+    key = ("quant_turns", group, window, n_kv, head_dim)
+    turns = batch.scratch.get(key)
+    if turns is None:
+        from .attention_plan import ROWS_PER_TILE, SPLIT_MAX_TILES, WIDE_TILES, first_keys, wide_chunk
+
+        cut_below = -(-2 * _units(device) // n_kv)
+        pieces: List[List[int]] = []
+        room = 0
+        for b, (m, n) in enumerate(zip(batch.q_lens, batch.kv_lens)):
+            tiles = -(-m * group // ROWS_PER_TILE)
+            if tiles <= SPLIT_MAX_TILES:
+                continue
+            n_wide = -(-tiles // WIDE_TILES)
+            cut = wide_chunk(n_wide, m, n, window, cut_below, True)
+            first = int(first_keys(n - m, window, None))
+            chunks = (n - 1) // cut - first // cut + 1 if cut else 1  # at most, of a block
+            needs = _portion_bytes(n_kv, head_dim, n - first, tiles * chunks if chunks > 1 else 0)
+            if not pieces or needs > room:
+                pieces.append([])
+                room = UNPACK_BYTES
+            pieces[-1].append(b)
+            room -= needs
+        turns = []
+        if len(pieces) > 1:
+            many = {b for piece in pieces for b in piece}
+            for i, piece in enumerate(pieces):
+                mine = set(piece) if i else set(piece) | set(range(len(batch.q_lens))) - many  # the first has the decoded tokens
+                turns.append(dataclasses.replace(batch, q_lens=[m if b in mine else 0 for b, m in enumerate(batch.q_lens)], scratch={}))
+        batch.scratch[key] = turns
+    return turns
 
 
 def _unpack_list(batch, group: int, window: Optional[int], device: torch.device):
@@ -277,9 +331,10 @@ def quant_paged_attention(
     call: `q` [T, Hq, hd] (float32 or bfloat16, rotated), `batch` the step's `StepBatch`, `window` the keys a query reads, its
     own included (None: all).  Returns [T, Hq * hd] in q's type.  A query one of whose keys has no page gets NaN.
     bfloat16 portions of more than 128 rows (tokens times query heads of a key/value head) unpack what they read of the cache to 16 bits for
-    the time of the call: 4 Hkv hd bytes a key."""
+    the time of the call: 4 Hkv hd bytes a key, for as many sequences at a time as 512 MiB hold, and for one at least
+    (`quant_attention_workspace`)."""
     KernelError, _check, _code = _base()
-    _attention_plan, _check_mask, _half_blocks_built, _three_blocks_a_unit = _planning()
+    _attention_plan, _check_mask, _half_blocks_built, _ = _planning()
     stream = _check_device(q, cache, block_table, batch.cu_q, batch.kv_len)
     _check_mask(window, None, None)
     if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
@@ -303,8 +358,24 @@ def quant_paged_attention(
         return out
     group = n_q // n_kv
     # bfloat16 queries of many rows: their keys and values are unpacked once, to float16, and read by the attention over a cache of 16 bits
-    plan = _attention_plan(batch, group, n_kv, hd, window, q.device, None, dtype == torch.bfloat16 and _half_blocks_built(n_kv, hd, UNPACK_PAGE), packed=True)
-    unpacks = plan.n_wide > 0 and dtype == torch.bfloat16
+    halves = dtype == torch.bfloat16 and _half_blocks_built(n_kv, hd, UNPACK_PAGE)
+    plan = _attention_plan(batch, group, n_kv, hd, window, q.device, None, halves, packed=True)
+    turns = _turns(batch, group, window, n_kv, hd, q.device) if plan.n_wide and dtype == torch.bfloat16 else ()
+    if not turns:
+        _attend(q, token, code, out, cache, block_table, batch, plan, n_q, n_kv, hd, page_size, pages, window, scale, bits, stream)
+    else:
+        for part in turns:
+            plan = _attention_plan(part, group, n_kv, hd, window, q.device, None, halves, packed=True)
+            _attend(q, token, code, out, cache, block_table, part, plan, n_q, n_kv, hd, page_size, pages, window, scale, bits, stream)
+    return out
+
+
+def _attend(q, token, code, out, cache, block_table, batch, plan, n_q, n_kv, hd, page_size, pages, window, scale, bits, stream) -> None:
+    """The launches of `quant_paged_attention`, whose arguments are checked, for the new tokens that `batch` counts."""
+    _check = _base()[1]
+    _three_blocks_a_unit = _planning()[3]
+    group = n_q // n_kv
+    unpacks = plan.n_wide > 0 and q.dtype == torch.bfloat16
     partials = partial = None
     if plan.n_partials:
         partials = torch.empty(plan.n_partials * n_kv * 16 * (hd + 4), dtype=torch.float32, device=q.device)  # held until the last launch
@@ -340,7 +411,6 @@ def quant_paged_attention(
         )
         if status:
             _check(lib, status)
-    return out
 
 
 # --------------------------------------------------------------------------- #

@@ -486,3 +486,29 @@ def test_portions_whose_chunks_are_doubled(monkeypatch, dtype):
         step, cache, q, keys, values = _case(new, kv, 32, 32, 8, dim, bits, dtype, window, 46)
         assert attention_plan.wide_chunk(4, 100, 3001, window, 64, True) == (256 if window is None else 128)
         _close(_attend(step, cache, q, bits, window, 0.125), step, q, keys, values, bits, window, 0.125)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_portions_that_take_turns(monkeypatch, bits):
+    """What a step unpacks is held for some of its sequences at a time: the rows are those of one piece, and the memory is bounded."""
+    from cwm_amd.ops import quantised
+
+    new, kv, dim, heads, group = [100, 1, 70, 200, 1, 90], [9000, 5000, 8200, 9300, 40, 90], 128, 2, 4
+    step, cache, q, _, _ = _case(new, kv, 32, group * heads, heads, dim, bits, torch.bfloat16, None, 47)
+    cache, table, qd = cache.to(DEV), step.table.to(DEV), q.to(DEV)
+    for window in (None, 700):
+        peaks, got = [], []
+        for most in (1 << 29, 1):
+            monkeypatch.setattr(quantised, "UNPACK_BYTES", most)
+            batch = step.batch(DEV)
+            run = lambda: ops.quant_paged_attention(qd, cache, table, batch, window, dim ** -0.5, bits)  # noqa: E731
+            run()
+            torch.cuda.synchronize()
+            torch.cuda.empty_cache()
+            before = torch.cuda.memory_allocated()
+            torch.cuda.reset_peak_memory_stats()
+            got.append(run())
+            peaks.append(torch.cuda.max_memory_allocated() - before)
+            assert torch.equal(got[-1], run())
+        assert torch.equal(*got) and torch.isfinite(got[0]).all()
+        assert peaks[1] < 0.6 * peaks[0]
