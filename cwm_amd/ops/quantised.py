@@ -19,14 +19,14 @@ CACHE_BITS = (4, 8)
 QUANT_MAX_DIM = 256  # csrc/quant_cache.h
 
 _P, _L, _I, _F = ctypes.c_void_p, ctypes.c_long, ctypes.c_int, ctypes.c_float
-# The C entry points by library, with their arguments' types: with these ctypes converts plain numbers by itself, which for
-# twenty arguments is 3 us less a call than objects made one by one.
+# The C entry points with their arguments' types, by name and the switches of a build that change them: with these ctypes converts
+# plain numbers by itself, which for twenty arguments is 3 us less a call than objects made one by one.
 _ARGTYPES = {
     "cwm_quant_kv_write": (_P, _L, _P, _L, _P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P),
     "cwm_quant_kv_read": (_P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P),
     "cwm_attention_quant": (_P, _L, _I, _P, _L, _P, _P, _I, _P, _P, _P, _I, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P),
     "cwm_quant_unpack": (_P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _I, _P),
-    "cwm_attention_mfma": (
+    ("cwm_attention_mfma", "HALF_INPUTS"): (
         _P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P, _P, _I, _P, _P,
     ),
     "cwm_quantize_rows": (_P, _L, _I, _P, _L, _P, _I, _I, _I, _P),
@@ -37,12 +37,12 @@ _entries: dict = {}
 
 def _entry(library: str, name: str, head_dim: Optional[int] = None, *switches: str):
     """The entry point `name` of a library built for a head size with the named switches, and the library (for its error message)."""
-    found = _entries.get((name, head_dim))
+    found = _entries.get((library, name, head_dim, switches))
     if found is None:
         lib = _build.load(library, None if head_dim is None else {"HEAD_DIM": head_dim, **dict.fromkeys(switches, 1)})
         function = lib[name]  # an object of its own: other callers of the library hand in objects of ctypes
-        function.argtypes = _ARGTYPES[name]
-        found = _entries[(name, head_dim)] = (function, lib)
+        function.argtypes = _ARGTYPES[(name, *switches) if switches else name]
+        found = _entries[(library, name, head_dim, switches)] = (function, lib)
     return found
 
 

@@ -178,3 +178,29 @@ def test_the_product_has_no_cpu_path():
         ops.linear_int8(**_product_args())
     with pytest.raises(ops.KernelError, match="HIP device"):
         ops.quantize_rows(torch.zeros(2, 16))
+
+
+def test_entry_points_are_those_of_their_build(monkeypatch):
+    """A library's builds export the same names with other arguments: none gets another's, and one whose arguments are not known is refused."""
+    from cwm_amd.ops import quantised
+
+    class Library(dict):
+        def __missing__(self, name):
+            self[name] = type("Function", (), {})()
+            return self[name]
+
+    built = {}
+
+    def load(library, defines=None):
+        return built.setdefault((library, tuple(sorted((defines or {}).items()))), Library())
+
+    monkeypatch.setattr(quantised, "_entries", {})
+    monkeypatch.setattr(quantised._build, "load", load)
+    half = quantised._entry("attention_mfma", "cwm_attention_mfma", 64, "HALF_INPUTS")
+    assert half[0] is built["attention_mfma", (("HALF_INPUTS", 1), ("HEAD_DIM", 64))]["cwm_attention_mfma"] and len(half[0].argtypes) == 37
+    assert quantised._entry("attention_mfma", "cwm_attention_mfma", 64, "HALF_INPUTS") is half
+    assert quantised._entry("attention_mfma", "cwm_attention_mfma", 128, "HALF_INPUTS") is not half
+    for switches in ((), ("KEPT_KEYS",)):
+        with pytest.raises(KeyError):
+            quantised._entry("attention_mfma", "cwm_attention_mfma", 64, *switches)
+    assert quantised._entry("quant_cache", "cwm_quant_kv_read") is quantised._entry("quant_cache", "cwm_quant_kv_read")
