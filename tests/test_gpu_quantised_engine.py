@@ -149,3 +149,49 @@ def test_the_command_line_takes_the_options(tmp_path):
     assert done.returncode == 0, done.stderr[-2000:]
     with open(out) as fh:
         assert len(json.loads(fh.readline())["tokens"]) == 6
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_the_layers_matrices_are_in_8_bits(tmp_path, dtype):
+    """Each matrix of a layer, on rows whose integers are known (whole numbers up to 127, so their scale is 1 and no code tips): the product with
+    the held integers within the roundings of its scales, which that with the matrix itself is not; and all that a step multiplies goes through them."""
+    folder = models.make_folder(tmp_path, "tiny_d", seed=3, dtype=dtype)
+    weights = models.read_folder(folder)[1]
+    model, _ = load_model(folder, dtype, DEV, weight_bits=8)
+    g = torch.Generator().manual_seed(1)
+    for i, block in enumerate(model.blocks):
+        name = lambda n: weights[f"layers.{i}.{n}.weight"].float()  # noqa: E731
+        w1, w3 = (name(f"feed_forward.{n}").reshape(-1, 8, model.dim) for n in ("w1", "w3"))
+        joined = [
+            (block.mixer.qkv, torch.cat([name(f"attention.{n}") for n in ("wq", "wk", "wv")])),
+            (block.mixer.wo, name("attention.wo")),
+            (block.feed_forward.gate_up, torch.stack([w1, w3], 1).flatten(0, 2)),
+            (block.feed_forward.down, name("feed_forward.w2")),
+        ]
+        for held_matrix, matrix in joined:
+            k = matrix.shape[1]
+            x = torch.randint(-127, 128, (5, k), generator=g).double()
+            x[:, 3] = 127
+            scale = (matrix.abs().amax(1) / torch.full((matrix.shape[0],), 127.0)).double()
+            want = x @ (torch.round(matrix / scale.float()[:, None]).double() * scale[:, None]).T
+            got = held_matrix(x.to(DEV, getattr(torch, dtype)), out_dtype=torch.float32).cpu().double()
+            limit = 3.01 * 2.0 ** -24 * want.abs() + 1e-30
+            assert held_matrix.weight is None and held_matrix.codes.dtype == torch.int8
+            assert ((got - want).abs() <= limit).all() and not ((x @ matrix.double().T - want).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("cache_bits,weight_bits", [(None, 8), (4, 8), (8, None)])
+def test_fewer_bits_are_not_left_out(tmp_path, monkeypatch, cache_bits, weight_bits):
+    """The engine's logits lie as far from the plain decoder's on its own values as holding the values in fewer bits moves them: half of that
+    at least (the held values are the same, the rounding of the activations is another draw of equal size).  A model that ignores an option lies at 1e-5 of it."""
+    folder = models.make_folder(tmp_path, "tiny_d", seed=3, dtype="float32")
+    tokens = traces.random_tokens(5, 60, configs.get("tiny_d")["vocab_size"])
+    model, _ = load_model(folder, "float32", DEV, cache_bits=cache_bits, weight_bits=weight_bits)
+    full = torch.from_numpy(models.plain_logits(folder, {"a": tokens})["a"]).double()
+    want = torch.from_numpy(_plain(monkeypatch, folder, tokens, cache_bits, weight_bits)).double()
+    calls = []
+    product = ops.linear_int8
+    monkeypatch.setattr(ops, "linear_int8", lambda *a, **k: calls.append(1) or product(*a, **k))
+    got, _ = _logits(model, tokens, [60])
+    assert len(calls) == (4 * len(model.blocks) if weight_bits else 0)
+    assert float((got.double() - full).norm()) >= 0.5 * float((want - full).norm())
