@@ -627,8 +627,6 @@ attention_quant_merge_kernel(T* __restrict__ out, long out_stride, const float* 
   Elem<T>::store(out + (size_t)(q0 + ti) * out_stride + (size_t)(g * group + r - ti * group) * HEAD_DIM + d, sum / total);
 }
 
-extern "C" int cwm_attention_quant_head_dim() { return HEAD_DIM; }
-
 extern "C" int cwm_attention_quant(const void* q, long q_stride, int dtype, void* out, long out_stride, const void* cache, const int* block_table,
                                    int table_width, const int* cu_q, const int* kv_len, const int* work, int n_work, const int* work_wide,
                                    int n_work_wide, int wide_tiles, const int* merge, int n_merge, float* partial, int n_q_heads, int n_kv_heads,

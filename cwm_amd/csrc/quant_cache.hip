@@ -648,8 +648,6 @@ extern "C" int cwm_quant_kv_read(void* k, void* v, int dtype, const int* positio
   return cwm_launch_status("quant_kv_read");
 }
 
-extern "C" int cwm_quant_unpack_keys() { return UNPACK_KEYS; }
-
 extern "C" int cwm_quant_unpack(void* out, int* exponents, int out_page, const int* list, int n_items, const void* cache, const int* block_table, int table_width,
                                 int page_size, int num_pages, const int* kv_len, int n_kv_heads, int head_dim, int bits, hipStream_t stream) {
   QUANT_REQUIRE_SIZES("quant_unpack");
