@@ -506,7 +506,12 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
   const int x_size = x_dtype == CWM_BF16 ? 2 : 4, Kp = (K + 127) / 128 * 128;
   CWM_REQUIRE(parts >= 1 && parts <= Kp / 128 && (parts == 1 || ((tile == 3 || tile == 4) && sums && (uintptr_t)sums % 16 == 0)),
               "linear_int8: K in %d parts with tile %d", parts, tile);
-  const int a_wave = (K / 128 + FEW_WAVES - 1) / FEW_WAVES;  // pieces of a wavefront of few rows
+  // Pieces of W that a wavefront of few rows has in flight at a time.  A round loads that many whether K has them or not, so of four and
+  // six it takes what loads fewer in all, and six where that is equal (us with four and with six: one row by 6,144 columns of 6,144
+  // 14.2 and 13.4, of 8,192 14.3 and 17.8; by 4,096 of 7,168 11.5 and 13.8, of 9,216 14.8 and 14.3, of 12,288 15.1 and 15.0, of 16,384
+  // 18.4 and 19.3; eight rows by 4,096 of 16,384 28.3 and 30.6).
+  const int a_wave = (K / 128 + FEW_WAVES - 1) / FEW_WAVES;  // pieces of a wavefront in all
+  const int ahead = a_wave <= 2 ? 2 : (a_wave + 3) / 4 * 4 < (a_wave + 5) / 6 * 6 ? 4 : 6;
   // Two blocks a compute unit stay, each with the same number of rows of W: what one unit can have in flight is limited, so with
   // tiles dealt out one by one the units that get one more take that much longer (one row by 6,144 of 6,144: 384 tiles 14.6 us,
   // 512 blocks of 12 rows 13.2).
@@ -520,9 +525,9 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
                      0l, (const float*)nullptr, (const TX*)x, x_stride, x_aligned, (const int8_t*)W, ldw, w_scale, bias, (T*)y, ldy, M, N, K, few_rows)
 #define INT8_FUSED_AHEAD(TX, T, ROWS)     \
   {                                       \
-    if (a_wave <= 2)                      \
+    if (ahead == 2)                       \
       INT8_FUSED_RUN(TX, T, ROWS, 2);     \
-    else if (a_wave <= 4 || a_wave == 8)  \
+    else if (ahead == 4)                  \
       INT8_FUSED_RUN(TX, T, ROWS, 4);     \
     else                                  \
       INT8_FUSED_RUN(TX, T, ROWS, 6);     \
@@ -561,9 +566,9 @@ extern "C" int cwm_linear_int8(const void* x, long x_stride, int x_dtype, void* 
 #define INT8_FEW_ROWS(T)               \
   if (rt == 4)                         \
     INT8_FEW(T, 4, 2);                 \
-  else if (a_wave <= 2)                \
+  else if (ahead == 2)                 \
     INT8_FEW(T, 1, 2);                 \
-  else if (a_wave <= 4 || a_wave == 8) \
+  else if (ahead == 4)                 \
     INT8_FEW(T, 1, 4);                 \
   else                                 \
     INT8_FEW(T, 1, 6)

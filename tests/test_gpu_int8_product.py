@@ -264,3 +264,15 @@ def test_scales_that_are_subnormal():
         codes, scale = ops.quantize_rows(x.to(DEV))
         want, a = _quantised(x)
         assert torch.equal(scale.cpu(), a) and torch.equal(codes.cpu(), want) and int(want.abs().max()) == 127
+
+
+@pytest.mark.parametrize("pieces", [1, 2, 3, 4, 5, 6, 7, 8, 9, 12, 13, 16])
+def test_pieces_in_flight(pieces):
+    """Every number of pieces a wavefront, at its smallest and largest K, with an end inside a piece: up to four rows in one launch, and in two."""
+    for k in (1024 * (pieces - 1) + 128, 1024 * pieces - 112, 1024 * pieces):
+        for m, tile in ((1, -1), (3, -1), (9, 0)):
+            if tile < 0 and k > 16384 // (1 if m == 1 else 4):
+                continue
+            x = _rows(m, k, torch.bfloat16, k + m)
+            w, s = _weight(40, k, k)
+            _check(x, w, s, None, torch.bfloat16, tile)
