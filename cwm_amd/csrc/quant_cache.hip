@@ -537,7 +537,7 @@ quant_unpack_kernel(uint16_t* __restrict__ out, int* __restrict__ exponents, int
     for (int off = 1; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
     if ((threadIdx.x & 31) == 0) {
       tops[threadIdx.x >> 5] = most;
-      exponents_to[(threadIdx.x >> 5) * 2 + 1] = half_exponent(most);
+      exponents_to[(threadIdx.x >> 5) * 2 + 1] = half_exponent(most, VALUES_LEAST);
     }
   }
   __syncthreads();
@@ -552,7 +552,7 @@ quant_unpack_kernel(uint16_t* __restrict__ out, int* __restrict__ exponents, int
       codes = *(const uint2*)(from + at.values + ((size_t)(slot >> 3) * UNITS + u) * 8);
       get_words<8>((const uint32_t*)(from + at.value_words) + slot, words);
     }
-    const float down = power_of_two(-half_exponent(tops[block >> 2]));
+    const float down = power_of_two(-half_exponent(tops[block >> 2], VALUES_LEAST));
     float x[BITS == 4 ? 2 : 1][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {

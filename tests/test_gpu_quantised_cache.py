@@ -512,3 +512,14 @@ def test_portions_that_take_turns(monkeypatch, bits):
             assert torch.equal(got[-1], run())
         assert torch.equal(*got) and torch.isfinite(got[0]).all()
         assert peaks[1] < 0.6 * peaks[0]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_portions_over_values_far_apart(bits):
+    """Sums of 2^64 that are brought to the exponent of a tile of values of 2^-70, the lowest there is, and back."""
+    new, kv, dim, group = [80], [480], 64, 4
+    step, cache, q, keys, values = _case(new, kv, 32, group, 1, dim, bits, torch.bfloat16, None, 48, sharpen=0.1)
+    values[0][:320] = (1 + values[0][:320].abs()) * 2.0 ** 55
+    values[0][320:448] *= 2.0 ** -70
+    held.put_all(cache, step.table, kv, keys, values, bits)
+    _close(_attend(step, cache, q, bits, None, 0.125), step, q, keys, values, bits, None, 0.125)
