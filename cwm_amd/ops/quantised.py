@@ -496,7 +496,7 @@ def linear_int8(
         joined = sums.data_ptr()
     function, lib = _entry("gemm_int8", "cwm_linear_int8")
     status = function(
-        x.data_ptr(), x.stride(0), x_code, codes, scale, weight.data_ptr(), weight.stride(0) if n > 1 else max(k, weight.stride(0)),
+        x.data_ptr(), x.stride(0), x_code, codes, scale, weight.data_ptr(), weight.stride(0) if n > 1 else k,
         weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), code, n, m, n, k, _units(x.device), tile, parts, joined, stream,
     )
     if status:

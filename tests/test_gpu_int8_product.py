@@ -255,6 +255,20 @@ def test_integers_end_at_127(k):
         assert (off <= 3.01 * 2.0 ** -24 * exact[:rows].abs()).all(), (rows, tile)
 
 
+def test_a_single_column_with_any_stride():
+    """One output channel: the stride between rows of the weight counts for nothing."""
+    x = _rows(5, 64, torch.bfloat16, 4)
+    for stride in (64, 72, 4099):
+        w, s = _weight(1, 64, 9, stride=stride)
+        assert w.stride(0) == stride
+        for rows in (1, 5):
+            _check(x[:rows], w.clone(), s, None, torch.float32)
+            given = torch.zeros(1, stride, dtype=torch.int8, device=DEV)
+            given[:, :64] = w.to(DEV)
+            y = ops.linear_int8(x[:rows].to(DEV), given[:, :64], s.to(DEV), out_dtype=torch.float32)
+            assert torch.equal(y, ops.linear_int8(x[:rows].to(DEV), w.to(DEV).clone(memory_format=torch.contiguous_format), s.to(DEV), out_dtype=torch.float32))
+
+
 def test_scales_that_are_subnormal():
     """Around the scales whose reciprocal float32 just holds, 2^-128, and the smallest normal one."""
     for k in (64, 100):
