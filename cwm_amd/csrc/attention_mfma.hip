@@ -1048,10 +1048,10 @@ attention_lds_kernel(const bf16_t* __restrict__ q, long q_stride, bf16_t* __rest
     if (!row_valid[rt]) continue;
 #ifdef HALF_INPUTS
     const float scale_log2e = row_scale[rt];
-    const float up = power_of_two(acc_exponent), down = power_of_two(-P_EXPONENT);
-    l_row *= down;
+    const float up = power_of_two(acc_exponent - P_EXPONENT);
+    l_row *= power_of_two(-P_EXPONENT);
 #pragma unroll
-    for (int dt = 0; dt < D_TILES; ++dt) acc[rt][dt] = acc[rt][dt] * down * up;
+    for (int dt = 0; dt < D_TILES; ++dt) acc[rt][dt] *= up;
 #endif
     if (w[4] >= 0) {
       // the item's keys are cut into w[5] chunks and this block had one of them: its row tile t

@@ -334,7 +334,7 @@ def quant_paged_attention(
     the time of the call: 4 Hkv hd bytes a key, for as many sequences at a time as 512 MiB hold, and for one at least
     (`quant_attention_workspace`)."""
     KernelError, _check, _code = _base()
-    _attention_plan, _check_mask, _half_blocks_built, _ = _planning()
+    _attention_plan, _check_mask, _half_blocks_built, _three_blocks_a_unit = _planning()
     stream = _check_device(q, cache, block_table, batch.cu_q, batch.kv_len)
     _check_mask(window, None, None)
     if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
@@ -360,57 +360,47 @@ def quant_paged_attention(
     # bfloat16 queries of many rows: their keys and values are unpacked once, to float16, and read by the attention over a cache of 16 bits
     halves = dtype == torch.bfloat16 and _half_blocks_built(n_kv, hd, UNPACK_PAGE)
     plan = _attention_plan(batch, group, n_kv, hd, window, q.device, None, halves, packed=True)
-    turns = _turns(batch, group, window, n_kv, hd, q.device) if plan.n_wide and dtype == torch.bfloat16 else ()
-    if not turns:
-        _attend(q, token, code, out, cache, block_table, batch, plan, n_q, n_kv, hd, page_size, pages, window, scale, bits, stream)
-    else:
-        for part in turns:
-            plan = _attention_plan(part, group, n_kv, hd, window, q.device, None, halves, packed=True)
-            _attend(q, token, code, out, cache, block_table, part, plan, n_q, n_kv, hd, page_size, pages, window, scale, bits, stream)
+    unpacks = plan.n_wide > 0 and dtype == torch.bfloat16
+    pieces = unpacks and _turns(batch, group, window, n_kv, hd, q.device)
+    for piece in pieces or (batch,):
+        if pieces:
+            plan = _attention_plan(piece, group, n_kv, hd, window, q.device, None, halves, packed=True)
+        partials = partial = unpacked = None  # a piece's memory is free for the next one
+        if plan.n_partials:
+            partials = torch.empty(plan.n_partials * n_kv * 16 * (hd + 4), dtype=torch.float32, device=q.device)  # held until the last launch
+            partial = partials.data_ptr()
+        table, width = block_table.data_ptr(), block_table.shape[1]
+        first, lengths, work, wide, merge = batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), plan.work.data_ptr(), plan.wide.data_ptr(), plan.merge.data_ptr()
+        if plan.n_work or not unpacks:
+            function, lib = _entry("attention_quant", "cwm_attention_quant", hd)
+            status = function(
+                q.data_ptr(), token, code, out.data_ptr(), n_q * hd, cache.data_ptr(), table, width, first, lengths, work, plan.n_work, wide,
+                0 if unpacks else plan.n_wide, plan.item_tiles, merge, 0 if unpacks else plan.n_merge, partial, n_q, n_kv, hd, page_size, pages,
+                -1 if window is None else window - 1, scale, bits, stream,
+            )
+            if status:
+                _check(lib, status)
+        if unpacks:
+            listed, n_items, wide_width, n_pages = _unpack_list(piece, group, window, q.device)
+            held = n_pages * 2 * n_kv * UNPACK_PAGE * hd * 2  # bytes; behind them two exponents for every 32 keys of a head
+            unpacked = torch.empty(held + n_pages * n_kv * (UNPACK_PAGE // 32) * 8, dtype=torch.uint8, device=q.device)
+            exponents = unpacked.data_ptr() + held
+            function, lib = _entry("quant_cache", "cwm_quant_unpack")
+            status = function(
+                unpacked.data_ptr(), exponents, UNPACK_PAGE, listed.data_ptr(), n_items, cache.data_ptr(), table, width, page_size, pages, lengths, n_kv, hd, bits, stream,
+            )
+            if status:
+                _check(lib, status)
+            function, lib = _entry("attention_mfma", "cwm_attention_mfma", hd, "HALF_INPUTS")
+            status = function(
+                q.data_ptr(), token, out.data_ptr(), n_q * hd, unpacked.data_ptr(), listed.data_ptr() + 16 * n_items, wide_width, first, lengths,
+                work, 0, 0, wide, plan.n_wide, plan.item_tiles, _three_blocks_a_unit(plan.n_wide * n_kv, plan.wide_shape, q.device),
+                merge, plan.n_merge, plan.n_merge_mid, plan.n_merge_wide, partial, n_q, n_kv, hd, UNPACK_PAGE, n_pages,
+                -1 if window is None else window - 1, 0, scale, 0.0, None, None, None, None, 0, exponents, stream,
+            )
+            if status:
+                _check(lib, status)
     return out
-
-
-def _attend(q, token, code, out, cache, block_table, batch, plan, n_q, n_kv, hd, page_size, pages, window, scale, bits, stream) -> None:
-    """The launches of `quant_paged_attention`, whose arguments are checked, for the new tokens that `batch` counts."""
-    _check = _base()[1]
-    _three_blocks_a_unit = _planning()[3]
-    group = n_q // n_kv
-    unpacks = plan.n_wide > 0 and q.dtype == torch.bfloat16
-    partials = partial = None
-    if plan.n_partials:
-        partials = torch.empty(plan.n_partials * n_kv * 16 * (hd + 4), dtype=torch.float32, device=q.device)  # held until the last launch
-        partial = partials.data_ptr()
-    table, width = block_table.data_ptr(), block_table.shape[1]
-    first, lengths, work, wide, merge = batch.cu_q.data_ptr(), batch.kv_len.data_ptr(), plan.work.data_ptr(), plan.wide.data_ptr(), plan.merge.data_ptr()
-    if plan.n_work or not unpacks:
-        function, lib = _entry("attention_quant", "cwm_attention_quant", hd)
-        status = function(
-            q.data_ptr(), token, code, out.data_ptr(), n_q * hd, cache.data_ptr(), table, width, first, lengths, work, plan.n_work, wide,
-            0 if unpacks else plan.n_wide, plan.item_tiles, merge, 0 if unpacks else plan.n_merge, partial, n_q, n_kv, hd, page_size, pages,
-            -1 if window is None else window - 1, scale, bits, stream,
-        )
-        if status:
-            _check(lib, status)
-    if unpacks:
-        listed, n_items, wide_width, n_pages = _unpack_list(batch, group, window, q.device)
-        held = n_pages * 2 * n_kv * UNPACK_PAGE * hd * 2  # bytes; behind them two exponents for every 32 keys of a head
-        unpacked = torch.empty(held + n_pages * n_kv * (UNPACK_PAGE // 32) * 8, dtype=torch.uint8, device=q.device)
-        exponents = unpacked.data_ptr() + held
-        function, lib = _entry("quant_cache", "cwm_quant_unpack")
-        status = function(
-            unpacked.data_ptr(), exponents, UNPACK_PAGE, listed.data_ptr(), n_items, cache.data_ptr(), table, width, page_size, pages, lengths, n_kv, hd, bits, stream,
-        )
-        if status:
-            _check(lib, status)
-        function, lib = _entry("attention_mfma", "cwm_attention_mfma", hd, "HALF_INPUTS")
-        status = function(
-            q.data_ptr(), token, out.data_ptr(), n_q * hd, unpacked.data_ptr(), listed.data_ptr() + 16 * n_items, wide_width, first, lengths,
-            work, 0, 0, wide, plan.n_wide, plan.item_tiles, _three_blocks_a_unit(plan.n_wide * n_kv, plan.wide_shape, q.device),
-            merge, plan.n_merge, plan.n_merge_mid, plan.n_merge_wide, partial, n_q, n_kv, hd, UNPACK_PAGE, n_pages,
-            -1 if window is None else window - 1, 0, scale, 0.0, None, None, None, None, 0, exponents, stream,
-        )
-        if status:
-            _check(lib, status)
 
 
 # --------------------------------------------------------------------------- #
