@@ -18,7 +18,7 @@
 // float32 queries: q and b in three bfloat16 parts each, codes without an offset (c - H is exact in bfloat16).
 //
 // Decoded tokens are bound by the reading of the cache: eight sequences of 32,768 tokens, 48 query heads on 8 of 128, 4 bits: 310 MB in
-// 62 us (5.0 TB/s; a plain read has 6.9) and 5 for joining the chunks; in bfloat16 the same step reads 1,074 MB in 178.  A wavefront's
+// 62 us (5.0 TB/s; a plain read has 6.9) and 5 for joining the chunks; in bfloat16 the same step reads 1,074 MB in 178 (6.0 TB/s).  A wavefront's
 // loads run two tiles ahead of its arithmetic; eight wavefronts a block instead of four take 77 us.  A step of few keys is bound by its
 // latencies (1,000 keys: 11.4 us).
 //
