@@ -523,3 +523,27 @@ def test_portions_over_values_far_apart(bits):
     values[0][320:448] *= 2.0 ** -70
     held.put_all(cache, step.table, kv, keys, values, bits)
     _close(_attend(step, cache, q, bits, None, 0.125), step, q, keys, values, bits, None, 0.125)
+
+
+def test_portions_that_take_turns_captured(monkeypatch):
+    """The pieces of a step in one graph, replayed with other queries, with eager steps in between."""
+    from cwm_amd.ops import quantised
+
+    monkeypatch.setattr(quantised, "UNPACK_BYTES", 1)
+    new, kv, dim, bits = [70, 1, 100, 60], [500, 2100, 3000, 60], 64, 4
+    step, cache, q, _, _ = _case(new, kv, 32, 12, 2, dim, bits, torch.bfloat16, None, 49)
+    cache, table, batch = cache.to(DEV), step.table.to(DEV), step.batch(DEV)
+    sets = [q.to(DEV), q.flip(0).to(DEV)]
+    held_q = sets[0].clone()
+    run = lambda x: ops.quant_paged_attention(x, cache, table, batch, None, dim ** -0.5, bits)  # noqa: E731
+    want = [run(x) for x in sets]
+    assert len(quantised._turns(batch, 6, None, 2, dim, held_q.device)) == 3
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(held_q)
+    for i in (1, 0, 1, 1, 0):
+        held_q.copy_(sets[i])
+        graph.replay()
+        replayed = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, want[i]) and torch.equal(run(sets[i]), want[i])
